@@ -33,7 +33,7 @@ NVCC_FLAGS = [
 # Approximate exponentials, divisions and roots wherever a result leaves in bf16 anyway.  Sources whose fp32 results stand in
 # for fp32 torch operations are compiled without; -ftz alone keeps an exp2f at one instruction.
 FAST_MATH = ["--use_fast_math"]
-PRECISE = {"delta_chunk.cu": [], "delta_chunk_vec.cu": ["-ftz=true"], "gates.cu": []}
+PRECISE = {"delta_chunk.cu": [], "delta_chunk_vec.cu": ["-ftz=true"], "gates.cu": [], "logprobs.cu": []}
 HOST_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
 HOST_LIBS = ["-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-ltorch"]
 

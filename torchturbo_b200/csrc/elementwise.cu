@@ -12,6 +12,7 @@
 //   AdamW     : torch fused AdamW math on fp32 shards                  (engine/backends/fsdp2/optimizers/adamw.py:226-251)
 #include <type_traits>
 #include "common.cuh"
+#include "act.cuh"
 #include "rowops.cuh"
 
 namespace ttb {
@@ -372,24 +373,6 @@ layernorm_bwd_kernel(const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* 
 //   act 0: identity, 1: GELU (tanh approximation), 2: GELU (erf).   x [R, C], bias [C], residual [R, C]; C % 8 == 0
 // Backward: dx = dy * act'(x + bias) ; dbias = column sum of dx (partials per block, reduced by colsum_kernel).
 // ============================================================================
-__device__ __forceinline__ float act_fwd(float v, int act) {
-  if (act == 1) {
-    const float u = 0.7978845608028654f * (v + 0.044715f * v * v * v);
-    return 0.5f * v * (1.f + tanhf(u));
-  }
-  if (act == 2) return 0.5f * v * (1.f + erff(v * 0.7071067811865476f));
-  return v;
-}
-__device__ __forceinline__ float act_grad(float v, int act) {
-  if (act == 1) {
-    const float u = 0.7978845608028654f * (v + 0.044715f * v * v * v);
-    const float t = tanhf(u);
-    return 0.5f * (1.f + t) + 0.5f * v * (1.f - t * t) * 0.7978845608028654f * (1.f + 3.f * 0.044715f * v * v);
-  }
-  if (act == 2) return 0.5f * (1.f + erff(v * 0.7071067811865476f)) + v * 0.3989422804014327f * __expf(-0.5f * v * v);
-  return 1.f;
-}
-
 __global__ void bias_act_fwd_kernel(const __nv_bfloat16* __restrict__ x, const __nv_bfloat16* __restrict__ bias,
                                     const __nv_bfloat16* __restrict__ residual, __nv_bfloat16* __restrict__ y,
                                     long long R, int C, int act) {

@@ -9,6 +9,29 @@ namespace ttb {
 
 struct EpFuseArgs;   // gemm.cu
 
+// What follows a product in its epilogue (GemmArgs.epi 2 to 4)
+struct TailArgs {
+  // 2: C = residual + dropout(act(product + bias)), product + bias also stored as `pre`
+  const void* bias;                    // bf16 [N] or null
+  int act;                             // act.cuh
+  void* pre;                           // bf16 [M, ld of C] or null
+  unsigned drop_t;                     // philox.cuh; 0: nothing is dropped
+  float drop_scale;
+  unsigned long long seed;
+  const unsigned long long* seed_dev;  // in place of `seed` where not null
+  long long first_row;
+  // 3 and 4: rows of logits that are not stored
+  const long long* targets;            // [M]; outside of [0, vocab): none
+  long long vocab;
+  // 3: for every tile and half of its columns, of each row's logits: largest, sum of exponentials, sum of exponentials times distances
+  float* part;                         // [3 or 2][slots][M], see logprobs.cu
+  float* target_logit;                 // [M]
+  int entropy;
+  // 4: C = gradient of the logits of columns first_col .. first_col + N - 1
+  const float *lse, *ent, *dlogp, *dent;   // [M]; `ent` and `dent` may be null
+  long long first_col;
+};
+
 struct GemmArgs {
   const void* A;      // bf16
   long long lda;      // elements: row stride of A's memory matrix
@@ -29,7 +52,7 @@ struct GemmArgs {
   const int* group_rows;
   int groups_k;
   long long total_rows;  // grouped-K: total rows of A/B memory matrices
-  int epi;            // 0 store, 1 swiglu
+  int epi;            // 0 store, 1 swiglu; with `tail` 2 bias + activation + dropout + residual, 3 softmax statistics, 4 gradient of logits
   int F;
   const float* row_scale;
   void* preact;
@@ -39,6 +62,7 @@ struct GemmArgs {
   const float* alpha;            // optional device scalar multiplied into the product (plain stores only)
   float* split_ws;               // optional fp32 [k_splits, M, N]: the product is formed in k_splits pieces, then added up
   int k_splits;
+  const TailArgs* tail;
 };
 
 // inputs of the chunk-parallel delta-rule kernels (delta_chunk.cuh)
@@ -55,6 +79,12 @@ struct DeltaChunkIn {
 }  // namespace ttb
 
 TTB_EXPORT int ttb_gemm_bf16(const ttb::GemmArgs*, void*);
+TTB_EXPORT int ttb_logprobs_slots(int);
+TTB_EXPORT int ttb_logprobs_join(const float*, const float*, const long long*, int, long long, long long, float*, float*, float*, void*);
+TTB_EXPORT int ttb_dropout(const void*, const void*, void*, int, long long, int, unsigned, float, unsigned long long, const unsigned long long*,
+                            long long, int, void*);
+TTB_EXPORT int ttb_tail_bwd(const void*, const void*, void*, float*, void*, int, long long, int, int, unsigned, float, unsigned long long,
+                            const unsigned long long*, long long, int, void*);
 TTB_EXPORT int ttb_rmsnorm_fwd(const void*, const void*, const void*, void*, void*, float*, long long, int, float, int, void*);
 TTB_EXPORT int ttb_rmsnorm_bwd(const void*, const void*, const void*, const float*, const void*, void*, float*, void*, int, long
                             long, int, int, int, void*);

@@ -9,8 +9,8 @@
 //     device array (64-aligned, pad rows are zero).
 // Epilogues: plain store (bf16 or fp32, optional accumulate / residual add) and
 // SwiGLU (gate and up column panels are loaded side by side into one 256-wide
-// accumulator; out = silu(g) * u * row_scale, pre-activations optionally kept).
-//
+// accumulator; out = silu(g) * u * row_scale, pre-activations optionally kept); and, in gemm_tails.cuh, what follows a biased projection
+// (bias, activation, dropout, residual) and rows of logits that are not stored (softmax statistics, and their gradient).
 //
 // Expert-parallel fusion (grouped-M only, both optional, see `EpFuse`):
 //   * push prologue: two extra warps per CTA copy this rank's routed token rows (plus routing weight and a
@@ -28,7 +28,10 @@
 // Replaces cuBLAS `F.linear`, `grouped_gemm.ops.gmm` and the torch.compile'd
 // SwiGLU of the reference (ops/providers/cuda/grouped_matmul.py:19-36,
 // ops/providers/cuda/swiglu.py:26-36, models/modules/moe/experts.py:181-254).
+#include "act.cuh"
+#include "fastdiv.cuh"
 #include "peer.cuh"
+#include "philox.cuh"
 #include <cstring>
 
 namespace ttb {
@@ -37,7 +40,7 @@ constexpr int BM = 128;
 constexpr int BK = 64;
 constexpr unsigned KID_GEMM = 1;
 
-enum Epi : int { EPI_STORE = 0, EPI_SWIGLU = 1 };
+enum Epi : int { EPI_STORE = 0, EPI_SWIGLU = 1, EPI_TAIL = 2, EPI_LSE = 3, EPI_DLOGITS = 4 };
 
 // Expert-parallel fusion parameters (device side).
 struct EpFuse {
@@ -67,17 +70,17 @@ struct EpFuse {
   int ret_rows;               // rows of every rank's return buffer (tags at or past it are refused)
 };
 
-// n / d for 0 <= n < 2^31 by a multiplication: with 2^s >= d and m = ceil(2^(31 + s) / d), m d exceeds 2^(31 + s) by less than 2^s, so
-// that n m / 2^(31 + s) stays below the next whole number.
-struct FastDiv {
-  uint32_t mul, shift;
-  __device__ __forceinline__ int operator()(int n) const { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul) >> shift); }
+// see TailArgs (entries.h)
+struct TailParams {
+  const __nv_bfloat16* bias;
+  int act, has_pre, pre_z, entropy;   // pre_z: plane of the map of C that the pre-activations are stored in, C's own is the other
+  DropoutParams drop;
+  const long long* targets;
+  long long vocab;
+  float *part, *target_logit;
+  const float *lse, *ent, *dlogp, *dent;
+  long long first_col;
 };
-static FastDiv fast_div(int d) {
-  uint32_t s = 0;
-  while ((1ull << s) < static_cast<uint64_t>(d)) ++s;
-  return FastDiv{static_cast<uint32_t>(((1ull << (31 + s)) + d - 1) / d), 31 + s};
-}
 
 struct GemmParams {
   EpFuse ep;
@@ -101,15 +104,17 @@ struct GemmParams {
   int tma_out;            // plain bf16 rows: stored by the copy engine through the map of C
   FastDiv by_group, by_band, by_rest;   // tile counts: of a group, of a whole band, rows of the last band
   int k_splits, kb_per_split;  // > 1: "group" g covers k-blocks [g, g + 1) * kb_per_split of one product, stored at C[g]
+  TailParams tail;
 };
 
-template <int BN, bool PAIR>
+template <int BN, bool PAIR, int EPI>
 struct SmemLayout {
   static constexpr int A_BYTES = BM * BK * 2;
   static constexpr int B_BYTES = (PAIR ? BN / 2 : BN) * BK * 2;   // a CTA of a pair holds half of the tile's columns
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int STAGES = (BN == 256 && !PAIR) ? 4 : 6;
-  static constexpr int EPI_STAGE_BYTES = 32 * 32 * 4;   // one 32-row x 32-column fp32 chunk per epilogue warp
+  // results and pre-activations of a warp's 64 columns are parked side by side, which costs a stage
+  static constexpr int STAGES = ((BN == 256 && !PAIR) ? 4 : 6) - (EPI == EPI_TAIL ? 1 : 0);
+  static constexpr int EPI_STAGE_BYTES = 32 * 32 * 4 * (EPI == EPI_TAIL ? 2 : 1);   // one 32-row x 32-column fp32 chunk per epilogue warp
   static constexpr int EPI_BYTES = 8 * EPI_STAGE_BYTES;
   static constexpr int TOTAL = STAGES * STAGE_BYTES + EPI_BYTES + 1024 /*align*/ + 256 /*barriers*/;
 };
@@ -133,11 +138,15 @@ __device__ __forceinline__ uint32_t epi_piece_addr64(uint32_t base, int row, int
   return base + row * 64 + ((piece ^ ((row >> 1) & 3)) << 4);
 }
 
+}  // namespace ttb
+#include "gemm_tails.cuh"
+namespace ttb {
+
 template <int BN, bool A_MN, bool B_MN, int EPI, bool PAIR>
-__global__ void __launch_bounds__(GEMM_THREADS_PUSH, 1)
+__global__ void __launch_bounds__(EPI < EPI_TAIL ? GEMM_THREADS_PUSH : GEMM_THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
             const GemmParams p) {
-  using L = SmemLayout<BN, PAIR>;
+  using L = SmemLayout<BN, PAIR, EPI>;
   constexpr int STAGES = L::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -413,6 +422,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       const bool row_ok = row < p.M;
       const uint32_t t_row = tmem_base + acc * BN + (static_cast<uint32_t>(lane_group * 32) << 16);
       const long long gbase = static_cast<long long>(g) * p.c_group_stride;
+      TailRow<EPI> tail;      // what the tail reads of this row, asked for ahead of the wait for the products
+      if constexpr (EPI >= EPI_TAIL) tail.fetch(p, row, nt * BN + col_half * (BN / 2));
       if (!mbar_wait(&tfull[acc], acc_phase, KID_GEMM, 4, consumer_budget)) { ok = false; break; }
       tc_fence_after();
       auto release = [&]() {      // the accumulator has been read
@@ -425,6 +436,15 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       };
 
+      if constexpr (EPI >= EPI_TAIL) {
+        uint8_t* stage_at = epi_stage + (warp - 2) * L::EPI_STAGE_BYTES;
+        const uint32_t at = t_row + col_half * (BN / 2);
+        const int first = nt * BN + col_half * (BN / 2);
+        if constexpr (EPI == EPI_TAIL) tail_store<BN>(p, tmC, tail, stage_at, at, first, row_base, lane, release);
+        else if constexpr (EPI == EPI_LSE) tail_stats<BN>(p, tail, at, first, 2 * nt + col_half, row, release);
+        else tail_dlogits<BN>(p, tmC, tail, stage_at, at, first, row_base, lane, release);
+        continue;
+      }
       if (EPI == EPI_STORE && p.tma_out) {
         // Plain bf16 rows, 64 columns at a time: parked as bf16 (128 bytes a row, the copy engine's swizzle) and handed to the copy
         // engine, which clips at the edges of C.  An SM's ordinary stores leave at 32 bytes a clock however they are shaped, and a warp
@@ -639,7 +659,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             }
           }
         }
-      } else {
+      } else if constexpr (EPI == EPI_SWIGLU) {
         // SwiGLU: accumulator columns [0,BN/2) = gate, [BN/2,BN) = up, for output columns n0..n0+BN/2.
         constexpr int HALF = BN / 2;
         const int n0 = nt * HALF;
@@ -730,7 +750,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       }
       release();
     }
-    if (EPI == EPI_STORE && p.tma_out && lane == 0) bulk_wait_all();
+    if ((EPI == EPI_STORE ? p.tma_out : EPI == EPI_TAIL || EPI == EPI_DLOGITS) && lane == 0) bulk_wait_all();
     if (p.ep.scat_on) __threadfence_system();   // this thread's peer stores are ordered before the "returned" flag
   } else if (p.ep.push_on) {
     // ------------------------------------------------------------ push warps (warps 10..11)
@@ -905,9 +925,36 @@ split_sum_kernel(const float* __restrict__ ws, int splits, int M, int N, void* C
   }
 }
 
+// The same for a product with a tail: eight columns per thread.
+__global__ void __launch_bounds__(256)
+split_tail_kernel(const float* __restrict__ ws, int splits, int M, int N, __nv_bfloat16* C, long long ldc, __nv_bfloat16* pre,
+                  const __nv_bfloat16* __restrict__ residual, long long ldr, const TailParams q) {
+  const long long idx = static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int nv = N / 8;
+  if (idx >= static_cast<long long>(M) * nv) return;
+  const long long r = idx / nv;
+  const int g = static_cast<int>(idx - r * nv);
+  const long long plane = static_cast<long long>(M) * N;
+  const float* src = ws + r * N + 8 * g;
+  float f[8] = {};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) {
+    const float4 u = *reinterpret_cast<const float4*>(src + s * plane), v = *reinterpret_cast<const float4*>(src + s * plane + 4);
+    f[0] += u.x; f[1] += u.y; f[2] += u.z; f[3] += u.w;
+    f[4] += v.x; f[5] += v.y; f[6] += v.z; f[7] += v.w;
+  }
+  add_bias8(f, q.bias, 8 * g);
+  if (pre) *reinterpret_cast<uint4*>(pre + r * ldc + 8 * g) = pack8(f);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = act_fwd(f[j], q.act);
+  if (q.drop.t) dropout8(f, dropout_draws(q.drop.first_row + r, g, dropout_key(q.drop)), q.drop.t, q.drop.scale);
+  if (residual) add8(f, *reinterpret_cast<const uint4*>(residual + r * ldr + 8 * g));
+  *reinterpret_cast<uint4*>(C + r * ldc + 8 * g) = pack8(f);
+}
+
 template <int BN, bool A_MN, bool B_MN, int EPI, bool PAIR>
 static int launch(const GemmArgs& a, cudaStream_t stream) {
-  using L = SmemLayout<BN, PAIR>;
+  using L = SmemLayout<BN, PAIR, EPI>;
   CUtensorMap tmA, tmB, tmC;
   // ---- A map (2D)
   {
@@ -990,6 +1037,14 @@ static int launch(const GemmArgs& a, cudaStream_t stream) {
   p.F = a.F; p.row_scale = a.row_scale; p.alpha = a.alpha;
   p.preact = reinterpret_cast<__nv_bfloat16*>(a.preact); p.ld_preact = a.ld_preact;
   p.k_splits = 1; p.kb_per_split = 0;
+  memset(&p.tail, 0, sizeof(p.tail));
+  if (a.tail) {
+    const TailArgs& t = *a.tail;
+    p.tail.bias = reinterpret_cast<const __nv_bfloat16*>(t.bias); p.tail.act = t.act;
+    p.tail.drop = DropoutParams{t.drop_t, t.drop_scale, t.seed, t.seed_dev, t.first_row};
+    p.tail.targets = t.targets; p.tail.vocab = t.vocab; p.tail.part = t.part; p.tail.target_logit = t.target_logit; p.tail.entropy = t.entropy;
+    p.tail.lse = t.lse; p.tail.ent = t.ent; p.tail.dlogp = t.dlogp; p.tail.dent = t.dent; p.tail.first_col = t.first_col;
+  }
   const bool split = a.split_ws != nullptr && a.k_splits > 1;
   if (split) {
     const int nkb = (a.K + BK - 1) / BK;
@@ -1011,6 +1066,17 @@ static int launch(const GemmArgs& a, cudaStream_t stream) {
     const uint64_t str[2] = {static_cast<uint64_t>(a.ldc) * 2, static_cast<uint64_t>(a.groups_k > 0 ? a.c_group_stride : a.ldc * a.M) * 2};
     const uint32_t box[3] = {64, 32, 1};
     int r = make_tmap_bf16(&tmC, a.C, 3, dims, str, box);
+    if (r) return 30000 + r;
+  }
+  if (EPI == EPI_TAIL || EPI == EPI_DLOGITS) {
+    // C and the pre-activations, equally wide and high, are two planes of one map: their distance is its outermost stride
+    const uintptr_t c = reinterpret_cast<uintptr_t>(a.C), pre = reinterpret_cast<uintptr_t>(a.tail->pre);
+    p.tail.has_pre = a.tail->pre != nullptr;
+    p.tail.pre_z = pre > c;
+    const uint64_t dims[3] = {static_cast<uint64_t>(a.N), static_cast<uint64_t>(a.M), pre ? 2ull : 1ull};
+    const uint64_t str[2] = {static_cast<uint64_t>(a.ldc) * 2, pre ? (pre > c ? pre - c : c - pre) : static_cast<uint64_t>(a.ldc) * a.M * 2};
+    const uint32_t box[3] = {64, 32, 1};
+    int r = make_tmap_bf16(&tmC, reinterpret_cast<const void*>(pre && pre < c ? pre : c), 3, dims, str, box);
     if (r) return 30000 + r;
   }
   constexpr int RASTER_M = PAIR ? 8 : 16;
@@ -1042,7 +1108,12 @@ static int launch(const GemmArgs& a, cudaStream_t stream) {
     const int grid = static_cast<int>(total < a.num_sms ? total : a.num_sms);
     kfn<<<grid, p.ep.push_on ? GEMM_THREADS_PUSH : GEMM_THREADS, L::TOTAL, stream>>>(tmA, tmB, tmC, p);
   }
-  if (split) {
+  if (split && a.tail) {
+    const long long n = static_cast<long long>(a.M) * (a.N / 8);
+    split_tail_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(
+        a.split_ws, p.k_splits, a.M, a.N, reinterpret_cast<__nv_bfloat16*>(a.C), a.ldc, reinterpret_cast<__nv_bfloat16*>(a.tail->pre),
+        reinterpret_cast<const __nv_bfloat16*>(a.residual), a.ldr, p.tail);
+  } else if (split) {
     const long long n = static_cast<long long>(a.M) * (a.N / 4);
     split_sum_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(
         a.split_ws, p.k_splits, a.M, a.N, a.C, a.ldc, a.c_fp32, a.accumulate, reinterpret_cast<const __nv_bfloat16*>(a.residual), a.ldr,
@@ -1091,7 +1162,7 @@ TTB_EXPORT int ttb_gemm_bf16(const ttb::GemmArgs* args, void* stream_ptr) {
   if (a.residual && ((a.ldr % 8) || (reinterpret_cast<uintptr_t>(a.residual) & 15))) return 904;
   if (a.epi == EPI_SWIGLU && ((a.F % 8) || a.c_fp32 || (a.preact && (a.ld_preact % 8)))) return 905;
   if (a.alpha && a.epi != EPI_STORE) return 905;
-  if (a.split_ws && (a.epi != EPI_STORE || a.tile_group || a.groups_k > 0 || a.ep || (a.N % 8) || (reinterpret_cast<uintptr_t>(a.split_ws) & 15)))
+  if (a.split_ws && ((a.epi != EPI_STORE && a.epi != EPI_TAIL) || a.tile_group || a.groups_k > 0 || a.ep || (a.N % 8) || (reinterpret_cast<uintptr_t>(a.split_ws) & 15)))
     return 909;
   if (a.ep) {
     const EpFuseArgs& e = *a.ep;
@@ -1103,6 +1174,23 @@ TTB_EXPORT int ttb_gemm_bf16(const ttb::GemmArgs* args, void* stream_ptr) {
     if (e.scat_on && (a.epi != EPI_STORE || a.c_fp32 || a.accumulate || a.residual || (a.N % 32) || !e.row_tag ||
                       !e.done_counter || (e.off_ret % 16)))
       return 908;
+  }
+  if (a.epi >= EPI_TAIL) {
+    if (!a.tail || a.epi > EPI_DLOGITS || a.a_mn || a.b_mn || a.tile_group || a.groups_k > 0 || a.ep || a.alpha || a.accumulate || a.c_fp32) return 911;
+    if (a.epi == EPI_TAIL && ((a.N % 8) || (reinterpret_cast<uintptr_t>(a.tail->pre) & 15) || (reinterpret_cast<uintptr_t>(a.tail->bias) & 15))) return 912;
+    if (a.epi != EPI_TAIL && (a.split_ws || a.residual || !a.tail->targets)) return 912;
+    const bool wide = a.N > 128, pair = wide && pays_in_pairs(a);
+    if (a.epi == EPI_TAIL && a.split_ws && a.k_splits > 1)
+      return wide ? (pair ? launch<256, false, false, EPI_STORE, true>(a, stream) : launch<256, false, false, EPI_STORE, false>(a, stream))
+                  : launch<128, false, false, EPI_STORE, false>(a, stream);
+#define TTB_TAIL(E) \
+  if (a.epi == E) \
+    return wide ? (pair ? launch<256, false, false, E, true>(a, stream) : launch<256, false, false, E, false>(a, stream)) \
+                : launch<128, false, false, E, false>(a, stream);
+    TTB_TAIL(EPI_TAIL)
+    TTB_TAIL(EPI_LSE)
+    TTB_TAIL(EPI_DLOGITS)
+#undef TTB_TAIL
   }
   const bool wide = (a.epi == EPI_SWIGLU) ? true : (a.N > 128);
   const bool pair = wide && pays_in_pairs(a);

@@ -1,0 +1,264 @@
+// Epilogues of gemm.cu for what follows a biased projection and for rows of logits that are not stored.  Included by gemm.cu alone.
+//
+//   tail_store    C = residual + dropout(act(z)), z = product + bias; z itself is kept in bf16 where the backward needs it (it reads z for
+//                 act'(z) only).  Everything up to C's one rounding stays fp32.
+//   tail_stats    of each row's logits in this tile and half of its columns: largest, sum of exponentials, and for the entropy their sum
+//                 weighted by the distance from the largest (logprobs.cu joins them).  All in powers of two: with m the largest times
+//                 log2(e) as rounded to fp32, d = l log2(e) - m is one fma, 2^d one instruction, and log2 sum 2^(l log2 e) = m + log2 s is
+//                 exact in m whatever its rounding was.
+//   tail_dlogits  gradient of the logits, formed again from the same operands:  p = 2^(l log2 e - lse log2 e),
+//                 dl = g (1[target] - p) - e p (l - lse + H), one rounding to bf16 (the type in which the two products behind it take it).
+#pragma once
+
+namespace ttb {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  return make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+}
+__device__ __forceinline__ void add8(float (&f)[8], const uint4& u) {
+  const float2 a = unpack_bf16(u.x), b = unpack_bf16(u.y), c = unpack_bf16(u.z), d = unpack_bf16(u.w);
+  f[0] += a.x; f[1] += a.y; f[2] += b.x; f[3] += b.y; f[4] += c.x; f[5] += c.y; f[6] += d.x; f[7] += d.y;
+}
+__device__ __forceinline__ void add_bias8(float (&f)[8], const __nv_bfloat16* bias, int col) {
+  if (bias) add8(f, __ldg(reinterpret_cast<const uint4*>(bias + col)));
+}
+// a load that stays where it is written: it has to be under way while the products are waited for
+__device__ __forceinline__ uint4 load16_here(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What an epilogue thread reads of its row (one row a thread) before the accumulator is there
+template <int EPI>
+struct TailRow {
+  __device__ __forceinline__ void fetch(const GemmParams&, int, int) {}
+};
+template <>
+struct TailRow<EPI_TAIL> {
+  uint4 res[8];      // 64 columns of the residual
+  const __nv_bfloat16* src;
+  long long row;
+  __device__ __forceinline__ void fetch8(const GemmParams& p, int col, int i) {
+    if (src && col + 8 * i < p.N) res[i] = load16_here(src + col + 8 * i);
+  }
+  __device__ __forceinline__ void fetch(const GemmParams& p, int r, int col) {
+    row = r;
+    src = p.residual && r < p.M ? p.residual + static_cast<long long>(r) * p.ldr : nullptr;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      res[i] = make_uint4(0u, 0u, 0u, 0u);
+      fetch8(p, col, i);
+    }
+  }
+};
+template <>
+struct TailRow<EPI_LSE> {
+  long long target;
+  __device__ __forceinline__ void fetch(const GemmParams& p, int r, int) { target = r < p.M ? __ldg(p.tail.targets + r) : -1; }
+};
+template <>
+struct TailRow<EPI_DLOGITS> {
+  long long target;      // column of this product, or one that it does not have
+  float lse2, g, e, shift;
+  __device__ __forceinline__ void fetch(const GemmParams& p, int r, int) {
+    const TailParams& q = p.tail;
+    target = -1;
+    lse2 = g = e = shift = 0.f;
+    if (r >= p.M) return;
+    const long long t = __ldg(q.targets + r);
+    if (t >= 0 && t < q.vocab) {
+      target = t - q.first_col;
+      g = q.dlogp ? __ldg(q.dlogp + r) : 0.f;
+    }
+    const float lse = __ldg(q.lse + r);
+    lse2 = lse * LOG2E;
+    if (q.dent) {
+      e = __ldg(q.dent + r);
+      shift = __ldg(q.ent + r);
+    }
+  }
+};
+
+template <int ACT>
+__device__ __forceinline__ void tail_chunk(const GemmParams& p, TailRow<EPI_TAIL>& tr, int i0, const uint32_t (&v)[32], uint32_t sy, int col0,
+                                           int next_col, PhiloxKey key, int lane) {
+  const TailParams& q = p.tail;
+#pragma unroll
+  for (int i = i0; i < i0 + 4; ++i) {
+    const int col = col0 + 8 * i;
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(v[8 * (i - i0) + j]);
+    if (col < p.N) add_bias8(f, q.bias, col);
+    if (q.has_pre) {
+      const uint4 z = pack8(f);
+      st_shared_v4(epi_piece_addr(sy + 4096, lane, i), z.x, z.y, z.z, z.w);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = act_fwd(f[j], ACT);
+    if (q.drop.t) dropout8(f, dropout_draws(q.drop.first_row + tr.row, col >> 3, key), q.drop.t, q.drop.scale);
+    if (p.residual) {
+      add8(f, tr.res[i]);
+      if (next_col >= 0) tr.fetch8(p, next_col, i);
+    }
+    const uint4 y = pack8(f);
+    st_shared_v4(epi_piece_addr(sy, lane, i), y.x, y.y, y.z, y.w);
+  }
+}
+
+// `at`: TMEM address of this warp's rows and first column, `first` that column in C
+template <int BN, typename Release>
+__device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMap& tmC, TailRow<EPI_TAIL>& tr, uint8_t* stage_at, uint32_t at,
+                                           int first, int row_base, int lane, Release release) {
+  const TailParams& q = p.tail;
+  const uint32_t sy = smem_u32(stage_at);
+  PhiloxKey key{0u, 0u};
+  if (q.drop.t) key = dropout_key(q.drop);
+  bool held = true;
+#pragma unroll 1
+  for (int c = 0; c < BN / 2; c += 64) {
+    const int col0 = first + c;
+    if (col0 >= p.N || row_base >= p.M) break;      // uniform across the warp
+    if (lane == 0) bulk_wait_read_all();            // the copy engine has read what was parked before
+    __syncwarp();
+    const int next_col = c + 64 < BN / 2 ? col0 + 64 : -1;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      uint32_t v[32];
+      tmem_ld_32x32b_x32(at + c + 32 * h, v);
+      tmem_ld_wait();
+      if (h == 1 && c + 64 >= BN / 2) {
+        release();
+        held = false;
+      }
+      if (q.act == 1) tail_chunk<1>(p, tr, 4 * h, v, sy, col0, next_col, key, lane);
+      else if (q.act == 2) tail_chunk<2>(p, tr, 4 * h, v, sy, col0, next_col, key, lane);
+      else tail_chunk<0>(p, tr, 4 * h, v, sy, col0, next_col, key, lane);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      if (q.has_pre) tma_store_3d(&tmC, stage_at + 4096, col0, row_base, q.pre_z);
+      tma_store_3d(&tmC, stage_at, col0, row_base, q.has_pre ? 1 - q.pre_z : 0);
+      bulk_commit_group();
+    }
+  }
+  if (held) release();
+}
+
+template <int BN, typename Release>
+__device__ __forceinline__ void tail_stats(const GemmParams& p, const TailRow<EPI_LSE>& tr, uint32_t at, int first, int slot, int row,
+                                           Release release) {
+  const TailParams& q = p.tail;
+  float m = -1e30f, s = 0.f, w = 0.f;      // of no column at all: a weight of zero
+#pragma unroll 1
+  for (int c = 0; c < BN / 2; c += 32) {
+    const int col0 = first + c;
+    if (col0 >= p.N) break;                         // uniform across the warp
+    uint32_t v[32];
+    tmem_ld_32x32b_x32(at + c, v);
+    tmem_ld_wait();
+    if (col0 + 32 > p.N) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (col0 + i >= p.N) v[i] = __float_as_uint(-1e30f);
+    }
+    const long long hit = tr.target - col0;
+    if (hit >= 0 && hit < 32) {
+      float l = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (hit == i) l = __uint_as_float(v[i]);
+      q.target_logit[row] = l;
+    }
+    float top = m;
+    float big = __uint_as_float(v[0]);
+#pragma unroll
+    for (int i = 1; i < 31; i += 2) big = fmax3(big, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+    big = fmaxf(big, __uint_as_float(v[31]));
+    top = fmaxf(m, big * LOG2E);
+    const float down = exp2_approx(m - top);
+    if (q.entropy) w = down * fmaf(s, m - top, w);
+    s *= down;
+    m = top;
+    float a0 = 0.f, a1 = 0.f, b0 = 0.f, b1 = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; i += 2) {
+      const float d0 = fmaf(__uint_as_float(v[i]), LOG2E, -m), d1 = fmaf(__uint_as_float(v[i + 1]), LOG2E, -m);
+      const float e0 = exp2_approx(d0), e1 = exp2_approx(d1);
+      a0 += e0; a1 += e1;
+      if (q.entropy) { b0 = fmaf(e0, d0, b0); b1 = fmaf(e1, d1, b1); }
+    }
+    s += a0 + a1;
+    w += b0 + b1;
+  }
+  release();
+  if (row < p.M) {
+    const long long slots = 2ll * p.n_tiles, plane = slots * p.M;
+    float* dst = q.part + slot * static_cast<long long>(p.M) + row;
+    dst[0] = m;
+    dst[plane] = s;
+    if (q.entropy) dst[2 * plane] = w;
+  }
+}
+
+template <int BN, typename Release>
+__device__ __forceinline__ void tail_dlogits(const GemmParams& p, const CUtensorMap& tmC, const TailRow<EPI_DLOGITS>& tr, uint8_t* stage_at,
+                                             uint32_t at, int first, int row_base, int lane, Release release) {
+  const uint32_t sy = smem_u32(stage_at);
+  const bool silent = tr.g == 0.f && tr.e == 0.f;     // zeros, whatever the row holds
+  const float ln2 = 0.6931471805599453f;
+  bool held = true;
+#pragma unroll 1
+  for (int c = 0; c < BN / 2; c += 64) {
+    const int col0 = first + c;
+    if (col0 >= p.N || row_base >= p.M) break;      // uniform across the warp
+    uint32_t v[2][32];
+    tmem_ld_32x32b_x32(at + c, v[0]);
+    tmem_ld_32x32b_x32(at + c + 32, v[1]);
+    tmem_ld_wait();
+    if (c + 64 >= BN / 2) {
+      release();
+      held = false;
+    }
+    const long long hit = tr.target - col0;
+    const bool here = hit >= 0 && hit < 64;
+    if (lane == 0) bulk_wait_read_all();
+    __syncwarp();
+    if (silent) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) st_shared_v4(epi_piece_addr(sy, lane, i), 0u, 0u, 0u, 0u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float d = fmaf(__uint_as_float(v[i >> 2][(8 * i + j) & 31]), LOG2E, -tr.lse2);
+          const float pr = exp2_approx(d);
+          f[j] = -pr * (p.tail.dent ? fmaf(tr.e, fmaf(d, ln2, tr.shift), tr.g) : tr.g);
+          if (here && hit == 8 * i + j) f[j] += tr.g;
+        }
+        const uint4 y = pack8(f);
+        st_shared_v4(epi_piece_addr(sy, lane, i), y.x, y.y, y.z, y.w);
+      }
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_3d(&tmC, stage_at, col0, row_base, 0);
+      bulk_commit_group();
+    }
+  }
+  if (held) release();
+}
+
+}  // namespace ttb

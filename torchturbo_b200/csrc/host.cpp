@@ -146,9 +146,20 @@ PyObject* wrap_all(const Ts&... ts) {
 // rows x last dimension
 Tensor rows2d(const Tensor& t) { return t.dim() == 2 ? t.contiguous() : t.reshape({-1, t.size(-1)}).contiguous(); }
 Tensor like_shape(const Tensor& t2, const Tensor& x) { return x.dim() == 2 ? t2 : t2.view(x.sizes()); }
+int logprobs_slots(int columns) { return ttb_logprobs_slots(columns); }
 int kda_gate_row_blocks(long long rows, int heads) { return ttb_kda_gate_row_blocks(rows, heads); }
 int row_blocks(long long rows, const Tensor& t) { return static_cast<int>(std::max<long long>(1, std::min<long long>(rows, 2 * sms(t)))); }
 at::ScalarType out_type(bool f32out) { return f32out ? at::kFloat : at::kBFloat16; }
+
+// into how many pieces along K a product is cut (kernels.gemm_splits)
+long long k_splits(long long M, long long N, long long K, int num_sms) {
+  PyObject* r = PyObject_CallFunction(g_gemm_splits, "LLLi", M, N, K, num_sms);
+  if (!r) throw Raised{};
+  const long long s = PyLong_AsLongLong(r);
+  Py_DECREF(r);
+  if (s == -1 && PyErr_Occurred()) throw Raised{};
+  return s;
+}
 
 // ---------------------------------------------------------------------------------------------
 // GEMM
@@ -232,11 +243,7 @@ PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Tensor ws;
     int kernels = 1;
     if (K >= 4096 && !swiglu && !tile_group.defined() && !ep) {
-      PyObject* r = PyObject_CallFunction(g_gemm_splits, "LLLi", M, N, K, g.num_sms);
-      if (!r) throw Raised{};
-      const long long s = PyLong_AsLongLong(r);
-      Py_DECREF(r);
-      if (s == -1 && PyErr_Occurred()) throw Raised{};
+      const long long s = k_splits(M, N, K, g.num_sms);
       if (s > 1) {
         ws = empty({s, M, N}, at::kFloat, a);
         g.split_ws = f32w(ws); g.k_splits = static_cast<int>(s);
@@ -244,6 +251,184 @@ PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
       }
     }
     launch("ttb_gemm_bf16", kernels, [&](void* st) { return ttb_gemm_bf16(&g, st); });
+    return wrap(out);
+  });
+}
+
+// ---------------------------------------------------------------------------------------------
+// products with a tail (gemm_tails.cuh), dropout
+// ---------------------------------------------------------------------------------------------
+// t, scale, seed or the tensor that holds it, first row
+struct Dropout {
+  unsigned t;
+  float scale;
+  unsigned long long seed;
+  Tensor seed_dev;
+  long long first_row;
+  const unsigned long long* dev() const { return static_cast<const unsigned long long*>(at_(seed_dev)); }
+};
+Dropout dropout_args(Args& in, const Tensor& like) {
+  Dropout d;
+  d.t = static_cast<unsigned>(in.integer());
+  d.scale = static_cast<float>(in.real());
+  d.seed = static_cast<unsigned long long>(in.integer());
+  d.seed_dev = in.optional();
+  d.first_row = in.integer();
+  need(!d.seed_dev.defined() || (d.seed_dev.scalar_type() == at::kLong && d.seed_dev.numel() == 1 && d.seed_dev.device() == like.device()),
+       "a seed tensor is one int64 value on the device of the rows");
+  return d;
+}
+void need_rows(const Tensor& t, long long rows, long long cols, const Tensor& like, const char* what) {
+  need(is_bf16(t) && t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && t.stride(1) == 1 && t.device() == like.device(), what);
+}
+GemmArgs product(const Tensor& a, const Tensor& b) {
+  need(is_bf16(a) && is_bf16(b) && a.dim() == 2 && b.dim() == 2 && a.size(1) == b.size(1) && a.device() == b.device(), "operands must be bf16 matrices with equal rows' lengths, on one device");
+  need(a.stride(1) == 1 && b.stride(1) == 1, "operands must be contiguous along their last dimension");
+  need(a.size(0) < (1ll << 31) && b.size(0) < (1ll << 31) && a.size(1) < (1ll << 31), "fewer than 2^31 rows and columns");
+  check_device(a);
+  GemmArgs g{};
+  g.A = a.const_data_ptr(); g.lda = a.stride(0);
+  g.B = b.const_data_ptr(); g.ldb = b.stride(0);
+  g.b_groups = 1;
+  g.M = static_cast<int>(a.size(0)); g.N = static_cast<int>(b.size(0)); g.K = static_cast<int>(a.size(1));
+  g.num_sms = sms(a);
+  return g;
+}
+
+PyObject* linear_tail(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args in(args, n, 11);
+    const Tensor &x = in.tensor(), &w = in.tensor();
+    const Tensor bias = in.optional();
+    ttb::TailArgs t{};
+    t.act = static_cast<int>(in.integer());
+    const Tensor residual = in.optional();
+    const Dropout d = dropout_args(in, x);
+    const bool want_pre = in.flag();
+    GemmArgs g = product(x, w);
+    const long long M = g.M, N = g.N;
+    const Tensor y = empty({M, N}, at::kBFloat16, x), pre = want_pre ? empty({M, N}, at::kBFloat16, x) : Tensor();
+    if (M == 0 || N == 0) return wrap_all(y, pre);
+    if (bias.defined()) {
+      need(is_bf16(bias) && bias.numel() == N && bias.is_contiguous() && bias.device() == x.device(), "the bias is one bf16 value a column");
+      t.bias = bias.const_data_ptr();
+    }
+    if (residual.defined()) {
+      need_rows(residual, M, N, x, "the residual is bf16 and has the shape of the result");
+      g.residual = residual.const_data_ptr(); g.ldr = residual.stride(0);
+    }
+    t.pre = to_(pre);
+    t.drop_t = d.t; t.drop_scale = d.scale; t.seed = d.seed; t.seed_dev = d.dev(); t.first_row = d.first_row;
+    g.C = y.data_ptr(); g.ldc = N;
+    g.epi = 2; g.tail = &t;
+    Tensor ws;
+    const long long s = g.K >= 4096 ? k_splits(M, N, g.K, g.num_sms) : 1;
+    if (s > 1) {
+      ws = empty({s, M, N}, at::kFloat, x);
+      g.split_ws = f32w(ws); g.k_splits = static_cast<int>(s);
+    }
+    launch("ttb_gemm_bf16", s > 1 ? 2 : 1, [&](void* st) { return ttb_gemm_bf16(&g, st); });
+    return wrap_all(y, pre);
+  });
+}
+
+PyObject* tail_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args in(args, n, 10);
+    const Tensor& dy = in.tensor();
+    const Tensor z = in.optional();
+    const int act = static_cast<int>(in.integer());
+    const Dropout d = dropout_args(in, dy);
+    const bool want_db = in.flag(), f32out = in.flag();
+    check_device(dy);
+    need(dy.dim() == 2 && is_bf16(dy) && dy.is_contiguous(), "gradients: bf16 rows without gaps");
+    need(!z.defined() || (is_bf16(z) && z.is_contiguous() && z.sizes() == dy.sizes() && z.device() == dy.device()), "pre-activations: bf16 rows without gaps");
+    const long long R = dy.size(0), C = dy.size(1);
+    const bool own = act != 0 || d.t != 0;
+    const Tensor dz = own ? empty_rows(dy) : dy;
+    const int grid = row_blocks(R, dy);
+    const Tensor part = want_db ? empty({grid, C}, at::kFloat, dy) : Tensor();
+    const Tensor db = !want_db ? Tensor() : R ? empty({C}, out_type(f32out), dy) : at::zeros({C}, plain(dy).dtype(out_type(f32out)));
+    if (R && (own || want_db))
+      launch("ttb_tail_bwd", want_db ? 2 : 1, [&](void* st) {
+        return ttb_tail_bwd(at_(dy), at_(z), own ? to_(dz) : nullptr, f32w(part), to_(db), !f32out, R, static_cast<int>(C), act, d.t, d.scale, d.seed,
+                            d.dev(), d.first_row, grid, st);
+      });
+    return wrap_all(dz, db);
+  });
+}
+
+PyObject* dropout(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args in(args, n, 7);
+    const Tensor& x = in.tensor();
+    const Tensor residual = in.optional();
+    const Dropout d = dropout_args(in, x);
+    check_device(x);
+    auto fits = [&](const Tensor& t) { return t.is_contiguous() && reinterpret_cast<uintptr_t>(at_(t)) % 16 == 0; };
+    need(x.dim() == 2 && (is_bf16(x) || x.scalar_type() == at::kFloat) && fits(x), "bf16 or fp32 rows without gaps on a 16-byte boundary");
+    need(!residual.defined() || (residual.scalar_type() == x.scalar_type() && residual.sizes() == x.sizes() && fits(residual) && residual.device() == x.device()),
+         "the residual has the type, shape and layout of the rows");
+    need(x.size(1) < (1ll << 31) - 8, "rows of fewer than 2^31 values");
+    const Tensor y = empty_rows(x);
+    if (x.numel())
+      launch("ttb_dropout", 1, [&](void* st) {
+        return ttb_dropout(at_(x), at_(residual), to_(y), !is_bf16(x), x.size(0), static_cast<int>(x.size(1)), d.t, d.scale, d.seed, d.dev(), d.first_row,
+                           sms(x), st);
+      });
+    return wrap(y);
+  });
+}
+
+// log-probabilities of `targets`, log-sum-exp of every row of logits and, if wanted, its entropy
+PyObject* logprobs_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args in(args, n, 4);
+    const Tensor &h = in.tensor(), &w = in.tensor(), &targets = in.tensor();
+    const bool want_ent = in.flag();
+    GemmArgs g = product(h, w);
+    const long long M = g.M;
+    need(targets.scalar_type() == at::kLong && targets.dim() == 1 && targets.is_contiguous() && targets.numel() == M && targets.device() == h.device(),
+         "targets: one int64 value a row");
+    need(g.N > 0 && g.K > 0, "a vocabulary and hidden states of at least one value");
+    const Tensor logp = empty({M}, at::kFloat, h), lse = empty({M}, at::kFloat, h), ent = want_ent ? empty({M}, at::kFloat, h) : Tensor();
+    if (M == 0) return wrap_all(logp, lse, ent);
+    const int slots = logprobs_slots(g.N);
+    const Tensor part = empty({want_ent ? 3 : 2, slots, M}, at::kFloat, h), hit = empty({M}, at::kFloat, h);
+    ttb::TailArgs t{};
+    t.targets = static_cast<const long long*>(at_(targets)); t.vocab = g.N;
+    t.part = f32w(part); t.target_logit = f32w(hit); t.entropy = want_ent;
+    g.epi = 3; g.tail = &t;
+    launch("ttb_gemm_bf16", 1, [&](void* st) { return ttb_gemm_bf16(&g, st); });
+    launch("ttb_logprobs_join", 1, [&](void* st) {
+      return ttb_logprobs_join(f32(part), f32(hit), t.targets, slots, M, g.N, f32w(logp), f32w(lse), f32w(ent), st);
+    });
+    return wrap_all(logp, lse, ent);
+  });
+}
+
+// gradient of the logits of columns first_col .. first_col + w.size(0) - 1 of a vocabulary, into `out`
+PyObject* logprobs_dlogits(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args in(args, n, 10);
+    const Tensor &h = in.tensor(), &w = in.tensor(), &targets = in.tensor(), &lse = in.tensor();
+    const Tensor ent = in.optional(), dlogp = in.optional(), dent = in.optional();
+    ttb::TailArgs t{};
+    t.first_col = in.integer();
+    t.vocab = in.integer();
+    const Tensor& out = in.tensor();
+    GemmArgs g = product(h, w);
+    need(targets.scalar_type() == at::kLong && targets.is_contiguous() && targets.numel() == g.M && targets.device() == h.device(), "targets: one int64 value a row");
+    for (const Tensor& r : {lse, ent, dlogp, dent})
+      need(!r.defined() || (r.scalar_type() == at::kFloat && r.is_contiguous() && r.numel() == g.M && r.device() == h.device()), "statistics and gradients: one fp32 value a row");
+    need(!dent.defined() || ent.defined(), "the entropy's gradient needs the entropy");
+    need_rows(out, g.M, g.N, h, "the gradient is bf16, a row for each of the hidden states");
+    if (g.M == 0 || g.N == 0) return wrap(out);
+    t.targets = static_cast<const long long*>(at_(targets));
+    t.lse = f32(lse); t.ent = f32(ent); t.dlogp = f32(dlogp); t.dent = f32(dent);
+    g.C = out.data_ptr(); g.ldc = out.stride(0);
+    g.epi = 4; g.tail = &t;
+    launch("ttb_gemm_bf16", 1, [&](void* st) { return ttb_gemm_bf16(&g, st); });
     return wrap(out);
   });
 }
@@ -826,7 +1011,8 @@ PyObject* setup(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* launches(PyObject*, PyObject* const*, Py_ssize_t) { return PyLong_FromLongLong(g_launches.load(std::memory_order_relaxed)); }
 
 #define ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {ENTRY(setup), ENTRY(launches), ENTRY(gemm), ENTRY(rmsnorm_fwd), ENTRY(rmsnorm_bwd), ENTRY(layernorm_fwd), ENTRY(layernorm_bwd),
+PyMethodDef methods[] = {ENTRY(setup), ENTRY(launches), ENTRY(gemm), ENTRY(linear_tail), ENTRY(tail_bwd), ENTRY(dropout), ENTRY(logprobs_fwd),
+                         ENTRY(logprobs_dlogits), ENTRY(rmsnorm_fwd), ENTRY(rmsnorm_bwd), ENTRY(layernorm_fwd), ENTRY(layernorm_bwd),
                          ENTRY(bias_act_fwd), ENTRY(bias_act_bwd), ENTRY(qknorm_rope_fwd), ENTRY(qknorm_rope_bwd), ENTRY(qkv_rope_fwd), ENTRY(qkv_rope_bwd), ENTRY(gdn_gate_fwd),
                          ENTRY(gdn_gate_bwd), ENTRY(scale), ENTRY(copy_words), ENTRY(kda_gate_fwd), ENTRY(kda_gate_bwd), ENTRY(delta_prep), ENTRY(delta_out), ENTRY(delta_bwd_pre),
                          ENTRY(delta_state_scan), ENTRY(rope), ENTRY(swiglu_fwd),

@@ -1,0 +1,60 @@
+// Log-probabilities of rows of logits that the output head's product (gemm_tails.cuh) has left as statistics of pieces of the
+// vocabulary: with m_i the largest logit of piece i times log2(e), s_i the sum of 2^(l log2 e - m_i) over it and w_i the same sum weighted
+// by its exponents,
+//   M = max m_i,  S = sum s_i 2^(m_i - M),  W = sum 2^(m_i - M) (w_i + s_i (m_i - M)),
+//   lse = (M + log2 S) ln 2,   log p(target) = l_target - lse,   entropy = (log2 S - W / S) ln 2.
+// Compiled without approximate logarithms: the results are fp32 and meant to be.
+#include "common.cuh"
+
+namespace ttb {
+
+// 32 rows a block (neighbouring lanes, neighbouring rows), the pieces dealt out to its warps; joined in a fixed order.
+constexpr int JOIN_WARPS = 16;
+
+__global__ void __launch_bounds__(32 * JOIN_WARPS)
+logprobs_join_kernel(const float* __restrict__ part, const float* __restrict__ target_logit, const long long* __restrict__ targets, int slots,
+                     long long M, long long V, float* __restrict__ logp, float* __restrict__ lse, float* __restrict__ ent) {
+  __shared__ float sm[3][JOIN_WARPS][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long row = static_cast<long long>(blockIdx.x) * 32 + lane;
+  const long long plane = static_cast<long long>(slots) * M;
+  float m = -1e30f, s = 0.f, w = 0.f;
+  auto join = [&](float m2, float s2, float w2) {
+    const float top = fmaxf(m, m2), a = exp2f(m - top), b = exp2f(m2 - top);
+    if (ent) w = a * (w + s * (m - top)) + b * (w2 + s2 * (m2 - top));
+    s = s * a + s2 * b;
+    m = top;
+  };
+  if (row < M) {
+#pragma unroll 4
+    for (int i = warp; i < slots; i += JOIN_WARPS) {
+      const float* src = part + i * M + row;
+      join(src[0], src[plane], ent ? src[2 * plane] : 0.f);
+    }
+  }
+  sm[0][warp][lane] = m; sm[1][warp][lane] = s; sm[2][warp][lane] = w;
+  __syncthreads();
+  if (warp != 0 || row >= M) return;
+  for (int i = 1; i < JOIN_WARPS; ++i) join(sm[0][i][lane], sm[1][i][lane], sm[2][i][lane]);
+  const float ln2 = 0.6931471805599453f, l2 = log2f(s), all = (m + l2) * ln2;
+  const long long t = targets[row];
+  logp[row] = t >= 0 && t < V ? target_logit[row] - all : 0.f;
+  lse[row] = all;
+  if (ent) ent[row] = (l2 - w / s) * ln2;
+}
+
+}  // namespace ttb
+
+// pieces that the product of N columns leaves for each row: two for every tile of its columns (gemm.cu)
+TTB_EXPORT int ttb_logprobs_slots(int N) { return N > 128 ? 2 * ((N + 255) / 256) : 2 * ((N + 127) / 128); }
+
+// part: fp32 [3 with `ent`, else 2][slots][M]
+TTB_EXPORT int ttb_logprobs_join(const float* part, const float* target_logit, const long long* targets, int slots, long long M, long long V,
+                                 float* logp, float* lse, float* ent, void* stream) {
+  using namespace ttb;
+  if (M == 0) return 0;
+  logprobs_join_kernel<<<static_cast<unsigned>((M + 31) / 32), 32 * JOIN_WARPS, 0, static_cast<cudaStream_t>(stream)>>>(
+      part, target_logit, targets, slots, M, V, logp, lse, ent);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 400 + static_cast<int>(e);
+}

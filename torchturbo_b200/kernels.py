@@ -204,6 +204,36 @@ def gemm(
 
 
 # --------------------------------------------------------------------------------------
+# products with a tail, dropout
+# --------------------------------------------------------------------------------------
+def linear_tail(x, weight, bias, act, residual, drop, want_pre):
+    """(y, z): ``y = residual + dropout(act(z))`` with ``z = x @ weight.T + bias``; ``z`` (bf16) is None unless `want_pre`.
+    ``drop``: `ops.dropout.Dropout`."""
+    return host().linear_tail(x, weight, bias, ACT[act], residual, drop.t, drop.scale, drop.seed, drop.seed_tensor, drop.first_row, want_pre)
+
+
+def tail_bwd(dy, z, act, drop, want_db, db_dtype=torch.float32):
+    """(dz, db) of `linear_tail`: ``dz = dropout(dy) * act'(z)`` (``dy`` itself where nothing is applied), ``db`` its column sums or None."""
+    return host().tail_bwd(dy, z, ACT[act], drop.t, drop.scale, drop.seed, drop.seed_tensor, drop.first_row, want_db, _is_f32(db_dtype))
+
+
+def dropout(x, residual, drop):
+    """``residual + dropout(x)`` on ``[R, C]`` bf16 or fp32 rows."""
+    return host().dropout(x, residual, drop.t, drop.scale, drop.seed, drop.seed_tensor, drop.first_row)
+
+
+def logprobs_fwd(hidden, weight, targets, want_entropy: bool):
+    """(logp, lse, entropy) fp32 per row of ``hidden @ weight.T``, whose values are not stored; ``logp`` is 0 where the target lies
+    outside the vocabulary, ``entropy`` None unless wanted."""
+    return host().logprobs_fwd(hidden, weight, targets, want_entropy)
+
+
+def logprobs_dlogits(hidden, weight, targets, lse, entropy, dlogp, dent, first_col: int, vocab: int, out):
+    """Gradient of the logits of the columns that ``weight`` (rows ``first_col ..`` of the head's) covers, bf16, into ``out``."""
+    return host().logprobs_dlogits(hidden, weight, targets, lse, entropy, dlogp, dent, first_col, vocab, out)
+
+
+# --------------------------------------------------------------------------------------
 # RMSNorm
 # --------------------------------------------------------------------------------------
 def rmsnorm_fwd(x, weight, eps, residual=None, one_plus_w=False):

@@ -7,6 +7,7 @@ tensors always take the kernel path and raise if the library is missing.
 """
 from __future__ import annotations
 
+import dataclasses
 import math
 
 import torch
@@ -16,6 +17,7 @@ from torch.autograd import forward_ad
 from ... import kernels as K
 from ...runtime import TurboDevice
 from ..base import OpImpl, OpImplKind
+from ..dropout import dropout_args
 from ..moe import MoEPermutation
 from ..registry import register_op
 from . import native as N
@@ -339,6 +341,106 @@ class B200BiasAct(_B200Op):
         if not _ok(x, bias, residual) or Cn % 8 or Cn > 16384 or act not in K.ACT:
             return N.bias_act_ref(x, bias, act, residual)
         return BiasActFn.apply(x, bias, act, residual)
+
+
+# ------------------------------------------------------------------------------------------------
+# biased linear with activation, dropout and residual; dropout
+# ------------------------------------------------------------------------------------------------
+def _operand(t: torch.Tensor) -> torch.Tensor:
+    """A matrix as the copy engine can read it: values of a row side by side, rows apart by at least their length and by a
+    multiple of 16 bytes, from a 16-byte boundary on."""
+    if t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0:
+        return t
+    return _aligned(t)
+
+
+def _matrix(t):
+    """Rows of the last dimension.  Outside of the Functions: what one of them returns is then no view, and may be changed in place."""
+    return t if t is None or t.dim() == 2 else t.reshape(-1, t.shape[-1])
+
+
+def _with_seed(drop, seed_tensor):
+    return drop if seed_tensor is None else dataclasses.replace(drop, seed_tensor=seed_tensor)
+
+
+def _graph_of_gradients(y, inputs, needs, dys):
+    """Gradients by way of the separate operations that `y` was made of, for a backward whose own graph is wanted (a kernel leaves none)."""
+    grads = iter(torch.autograd.grad(y, [t for t, n in zip(inputs, needs) if n], dys, create_graph=True, allow_unused=True))
+    return tuple(next(grads) if n else None for n in needs)
+
+
+class LinearBiasActFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, bias, residual, act, drop):
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        back = need_x or need_w or need_b
+        y, z = K.linear_tail(_operand(x), _operand(w), _aligned(bias) if bias is not None else None, act,
+                             _operand(residual) if residual is not None else None, drop, back and K.ACT[act] != 0)
+        if back:
+            # the seed is saved like an operand: moving it on before the backward is an error and not another mask
+            ctx.save_for_backward(x, w, bias, z, drop.seed_tensor)
+            ctx.act, ctx.drop = act, drop
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        dx = dw = db = None
+        if need_x or need_w or need_b:
+            x, w, bias, z, seed = ctx.saved_tensors
+            drop = _with_seed(ctx.drop, seed)
+            if torch.is_grad_enabled():
+                y = N.linear_bias_act_ref(x, w, bias, ctx.act, None, drop)
+                dx, dw, db = _graph_of_gradients(y, (x, w, bias), (need_x, need_w, need_b), dy)
+            else:
+                dz, db = K.tail_bwd(_aligned(dy), z, ctx.act, drop, need_b, bias.dtype if need_b else BF16)
+                if need_x:
+                    dx = K.gemm(dz, _operand(w), b_mn=True)
+                if need_w:
+                    dw = _weight_grad(w, dz, _operand(x))
+        return dx, dw, db, dy if need_r else None, None, None
+
+
+@_custom("linear_bias_act", "tcgen05_linear_bias_act")
+class B200LinearBiasAct(_B200Op):
+    """Bias, activation, dropout and residual in the product's epilogue; in training the pre-activations leave beside the result.  The
+    backward is one pass over them and the incoming gradient, and the two products."""
+
+    def __call__(self, x, weight, bias=None, act=None, *, residual=None, dropout_p=0.0, seed=None, first_row=0):
+        N.check_linear_bias_act(x, weight, bias, act, residual)
+        if not _ok(x, weight, bias, residual) or x.shape[-1] % 8 or weight.shape[0] % 8 or not weight.numel() or weight.shape[0] > 16384:
+            return N.TorchLinearBiasAct()(x, weight, bias, act, residual=residual, dropout_p=dropout_p, seed=seed, first_row=first_row)
+        shape = x.shape[:-1] + weight.shape[:1]
+        y = LinearBiasActFn.apply(_matrix(x), weight, bias, _matrix(residual), act, dropout_args(dropout_p, seed, first_row))
+        return y if y.shape == shape else y.view(shape)
+
+
+class DropoutFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, drop):
+        ctx.save_for_backward(drop.seed_tensor)
+        ctx.drop = drop
+        return K.dropout(_aligned(x), _aligned(residual) if residual is not None else None, drop)
+
+    @staticmethod
+    def backward(ctx, dy):
+        drop = _with_seed(ctx.drop, *ctx.saved_tensors)
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = DropoutFn.apply(dy, None, drop) if torch.is_grad_enabled() else K.dropout(_aligned(dy), None, drop)
+        return dx, dy if ctx.needs_input_grad[1] else None, None
+
+
+@_custom("dropout", "b200_dropout")
+class B200Dropout(_B200Op):
+    """One pass each way; the mask is drawn in it.  bf16 and fp32 rows of any width."""
+
+    def __call__(self, x, p, seed=None, *, residual=None, scale=1.0, first_row=0):
+        N.check_dropout(x, residual)
+        if not x.is_cuda or x.dtype not in (BF16, torch.float32) or not x.numel():
+            return N.TorchDropout()(x, p, seed, residual=residual, scale=scale, first_row=first_row)
+        y = DropoutFn.apply(_matrix(x), _matrix(residual), dropout_args(p, seed, first_row, scale))
+        return y if y.shape == x.shape else y.view(x.shape)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -833,6 +935,93 @@ class B200LinearCrossEntropy(_B200Op):
         if not _ok(hidden, weight) or ignore_index >= 0 or hidden.shape[-1] % 8 or weight.shape[0] % 8:
             return N.TorchLinearCrossEntropy()(hidden, weight, labels, chunk_size=chunk_size, ignore_index=ignore_index)
         return LinearCrossEntropyFn.apply(hidden, weight, labels, chunk_size)
+
+
+class LinearLogprobsFn(torch.autograd.Function):
+    """Log-probabilities (and entropies) of rows of logits that are never stored.
+
+    Forward: the product's epilogue keeps each row's softmax statistics for every piece of the vocabulary that a tile covers, and a
+    second kernel joins them.  Backward: the vocabulary goes in pieces; each forms its logits again, turned into their gradient in
+    the epilogue, and adds to the hidden states' gradient (in fp32 where there is more than one piece) and writes its own rows of
+    the weight's.  What lies in memory at a time is one piece of the gradient of the logits."""
+
+    PIECE = 2 ** 28      # values of a piece
+
+    @staticmethod
+    def pieces(rows: int, vocab: int) -> int:
+        """Columns of a piece: equal ones, of whole 256-column tiles."""
+        count = max(1, -(-rows * vocab // LinearLogprobsFn.PIECE))
+        return -(-vocab // (256 * count)) * 256
+
+    @staticmethod
+    def forward(ctx, hidden, weight, targets, want_entropy):
+        logp, lse, ent = K.logprobs_fwd(_operand(hidden), _operand(weight), targets, want_entropy)
+        ctx.save_for_backward(hidden, weight, targets, lse, ent)
+        ctx.set_materialize_grads(False)
+        return (logp, ent) if want_entropy else logp
+
+    @staticmethod
+    def backward(ctx, dlogp, dent=None):
+        hidden, weight, targets, lse, ent = ctx.saved_tensors
+        need_h, need_w = ctx.needs_input_grad[:2]
+        if (dlogp is None and dent is None) or not (need_h or need_w):
+            return None, None, None, None
+        if torch.is_grad_enabled():
+            outs = N.TorchLinearLogprobs()(hidden, weight, targets, want_entropy=dent is not None)
+            pairs = [(y, g) for y, g in zip(outs, (dlogp, dent)) if g is not None]
+            return *_graph_of_gradients([y for y, _ in pairs], (hidden, weight), (need_h, need_w), [g for _, g in pairs]), None, None
+        h2, w2 = _operand(hidden), _operand(weight)
+        (T, H), V = h2.shape, w2.shape[0]
+        gs = [g.float().contiguous() if g is not None else None for g in (dlogp, dent)]
+        mg = getattr(weight, "main_grad", None) if need_w else None
+        dw = torch.empty(V, H, dtype=BF16, device=h2.device) if need_w and mg is None else None
+        if not T:
+            return torch.zeros_like(hidden) if need_h else None, dw.zero_() if dw is not None else None, None, None
+        step = LinearLogprobsFn.pieces(T, V)
+        buf = torch.empty(T * min(step, -(-V // 8) * 8), dtype=BF16, device=h2.device)
+        dh = None
+        for s in range(0, V, step):
+            n = min(step, V - s)
+            piece = w2[s:s + n]
+            dl = buf[:T * (-(-n // 8) * 8)].view(T, -1)[:, :n]
+            K.logprobs_dlogits(h2, piece, targets, lse, ent if dent is not None else None, *gs, s, V, dl)
+            if need_h:
+                if step >= V:
+                    dh = K.gemm(dl, piece, b_mn=True)
+                else:
+                    dh = K.gemm(dl, piece, b_mn=True, out=dh, out_dtype=torch.float32, accumulate=dh is not None)
+            if need_w:
+                if mg is not None:
+                    K.gemm(dl, h2, a_mn=True, b_mn=True, out=mg[s:s + n], accumulate=True)
+                else:
+                    K.gemm(dl, h2, a_mn=True, b_mn=True, out=dw[s:s + n])
+        return dh.to(BF16) if need_h else None, dw, None, None
+
+
+@_custom("linear_logprobs", "tcgen05_linear_logprobs")
+class B200LinearLogprobs(_B200Op):
+    def __call__(self, hidden, weight, targets, *, want_entropy: bool = False):
+        N.check_linear_logprobs(hidden, weight, targets)
+        if not _ok(hidden, weight) or hidden.shape[-1] % 8:
+            return N.TorchLinearLogprobs()(hidden, weight, targets, want_entropy=want_entropy)
+        flat = targets if targets.dim() == 1 else targets.reshape(-1)
+        out = LinearLogprobsFn.apply(_matrix(hidden), weight, flat.long().contiguous(), want_entropy)
+        logp, ent = out if want_entropy else (out, None)
+        if targets.dim() == 1:
+            return logp, ent
+        return logp.view(targets.shape), ent.view(targets.shape) if want_entropy else None
+
+
+@_custom("linear_cross_entropy", "tcgen05_linear_cross_entropy_pieces", priority=50)
+class B200LinearCrossEntropyPieces(_B200Op):
+    """The loss from `linear_logprobs`: fp32 logits that are formed once for the loss and once more for its gradient, none kept.  Selected
+    by name (an override of `linear_cross_entropy`) where the kept logits of the other form, `2 T V` bytes, are too many."""
+
+    def __call__(self, hidden, weight, labels, *, chunk_size: int = 4096, ignore_index: int = -100):
+        if ignore_index >= 0:
+            return N.TorchLinearCrossEntropy()(hidden, weight, labels, chunk_size=chunk_size, ignore_index=ignore_index)
+        h2 = hidden.reshape(-1, hidden.shape[-1])
+        return -B200LinearLogprobs()(h2, weight, labels.reshape(-1))[0].sum()
 
 
 # ------------------------------------------------------------------------------------------------

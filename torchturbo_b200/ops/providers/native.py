@@ -12,6 +12,7 @@ import torch
 import torch.nn.functional as F
 
 from ..base import OpImpl, OpImplKind
+from ..dropout import dropout_args, dropout_ref, wide_float
 from ..moe import MoEPermutation
 from ..registry import register_op
 
@@ -86,6 +87,60 @@ class TorchBiasAct(OpImpl):
 
     def __call__(self, x, bias, act=None, *, residual=None):
         return bias_act_ref(x, bias, act, residual)
+
+
+def check_dropout(x, residual) -> None:
+    if x.dim() == 0 or not x.is_floating_point():
+        raise ValueError("dropout takes rows of floating-point values")
+    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError(f"the residual must have the shape, type and device of the rows, got {tuple(residual.shape)} {residual.dtype} on {residual.device}")
+
+
+@_native("dropout")
+class TorchDropout(OpImpl):
+    """`residual + dropout(x)` with a mask that the seed and an element's place decide (`ops.dropout`): the same on every device and in
+    the backward, which draws it again.  `scale` multiplies what stays besides `1 / (1 - p)`; `first_row` is the place of the
+    first row among the rows of the whole (all dimensions but the last count rows)."""
+
+    def __call__(self, x, p, seed=None, *, residual=None, scale=1.0, first_row=0):
+        check_dropout(x, residual)
+        return dropout_ref(x, dropout_args(p, seed, first_row, scale), residual)
+
+
+def check_linear_bias_act(x, weight, bias, act, residual) -> None:
+    if x.dim() == 0 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"rows of {x.shape[-1] if x.dim() else 0} values do not fit a weight of shape {tuple(weight.shape)}")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError(f"the bias must have {weight.shape[0]} values, got shape {tuple(bias.shape)}")
+    if act not in _BIAS_ACTS:
+        raise ValueError(f"unknown activation {act!r}")
+    if residual is not None and residual.shape != x.shape[:-1] + weight.shape[:1]:
+        raise ValueError(f"the residual must have the shape of the result, got {tuple(residual.shape)}")
+    for t in (weight, bias, residual):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"operands live on {x.device} and {t.device}")
+
+
+_BIAS_ACTS = (None, "none", "identity", "gelu_tanh", "gelu_pytorch_tanh", "gelu", "gelu_erf")
+
+
+def linear_bias_act_ref(x, weight, bias, act, residual, drop):
+    wide = wide_float(x)
+    v = F.linear(x.to(wide), weight.to(wide), bias.to(wide) if bias is not None else None)
+    if act in ("gelu_tanh", "gelu_pytorch_tanh"):
+        v = F.gelu(v, approximate="tanh")
+    elif act in ("gelu", "gelu_erf"):
+        v = F.gelu(v)
+    return dropout_ref(v, drop, residual).to(x.dtype)
+
+
+@_native("linear_bias_act")
+class TorchLinearBiasAct(OpImpl):
+    """`residual + dropout(act(x W^T + bias))`, in fp32 and rounded once.  `dropout_p`, `seed` and `first_row` as in `dropout`."""
+
+    def __call__(self, x, weight, bias=None, act=None, *, residual=None, dropout_p=0.0, seed=None, first_row=0):
+        check_linear_bias_act(x, weight, bias, act, residual)
+        return linear_bias_act_ref(x, weight, bias, act, residual, dropout_args(dropout_p, seed, first_row))
 
 
 @_native("qkv_bias_rope")
@@ -239,6 +294,38 @@ class TorchLinearCrossEntropy(OpImpl):
             lg = F.linear(h2[s:s + chunk_size], weight).float()
             total = total + F.cross_entropy(lg, l2[s:s + chunk_size], reduction="sum", ignore_index=ignore_index)
         return total
+
+
+def check_linear_logprobs(hidden, weight, targets) -> None:
+    if hidden.dim() == 0 or weight.dim() != 2 or hidden.shape[-1] != weight.shape[1] or not weight.numel():
+        raise ValueError(f"hidden states of shape {tuple(hidden.shape)} do not fit a head of shape {tuple(weight.shape)}")
+    if targets.shape != hidden.shape[:-1] or targets.is_floating_point():
+        raise ValueError(f"targets are one token id for each hidden state, got {tuple(targets.shape)} {targets.dtype}")
+    if weight.device != hidden.device or targets.device != hidden.device:
+        raise ValueError(f"operands live on {hidden.device}, {weight.device} and {targets.device}")
+
+
+@_native("linear_logprobs")
+class TorchLinearLogprobs(OpImpl):
+    """(`log softmax(hidden W^T)[target]`, entropy of every row's distribution or None), fp32.  Targets outside of the vocabulary (-100
+    and the like) have a log-probability of 0 and no gradient through it; the entropy counts for every row.  The plain
+    formulation forms the logits in chunks of rows, which autograd keeps."""
+
+    def __call__(self, hidden, weight, targets, *, want_entropy: bool = False, chunk: int = 1024):
+        check_linear_logprobs(hidden, weight, targets)
+        wide = wide_float(hidden)
+        h2, t2 = hidden.reshape(-1, hidden.shape[-1]), targets.reshape(-1).long()
+        logps, ents = [h2.new_zeros(0, dtype=wide)], [h2.new_zeros(0, dtype=wide)]
+        for s in range(0, h2.shape[0], chunk):
+            lq = F.log_softmax(F.linear(h2[s:s + chunk].to(wide), weight.to(wide)), dim=-1)
+            t = t2[s:s + chunk]
+            ok = (t >= 0) & (t < weight.shape[0])
+            lp = lq.gather(1, torch.where(ok, t, 0).unsqueeze(1)).squeeze(1)
+            logps.append(torch.where(ok, lp, torch.zeros_like(lp)))
+            if want_entropy:
+                ents.append(-(lq.exp() * lq).sum(-1))
+        shape = targets.shape
+        return torch.cat(logps).view(shape), torch.cat(ents).view(shape) if want_entropy else None
 
 
 # ------------------------------------------------------------------------------------------------
