@@ -2,7 +2,6 @@
 #include <algorithm>
 
 #include "act.cuh"
-#include "common.cuh"
 #include "fastdiv.cuh"
 #include "philox.cuh"
 #include "rowops.cuh"
@@ -141,8 +140,8 @@ tail_bwd_kernel(const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __res
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float2 v = unpack_bf16(zs[j]);
-        f[2 * j] *= act_grad(v.x, ACT);
-        f[2 * j + 1] *= act_grad(v.y, ACT);
+        f[2 * j] *= act_slope<ACT>(v.x);
+        f[2 * j + 1] *= act_slope<ACT>(v.y);
       }
     }
 #pragma unroll

@@ -410,6 +410,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
+    [[maybe_unused]] uint32_t tail_side = 0;
     Tile x = fetch(walker), next;
     for (int t = walker; t < total_tiles && ok; t += walkers, x = next) {
       int k0, nkb;
@@ -440,7 +441,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         uint8_t* stage_at = epi_stage + (warp - 2) * L::EPI_STAGE_BYTES;
         const uint32_t at = t_row + col_half * (BN / 2);
         const int first = nt * BN + col_half * (BN / 2);
-        if constexpr (EPI == EPI_TAIL) tail_store<BN>(p, tmC, tail, stage_at, at, first, row_base, lane, release);
+        if constexpr (EPI == EPI_TAIL) tail_store<BN>(p, tmC, tail, stage_at, at, first, row_base, lane, tail_side, release);
         else if constexpr (EPI == EPI_LSE) tail_stats<BN>(p, tail, at, first, 2 * nt + col_half, row, release);
         else tail_dlogits<BN>(p, tmC, tail, stage_at, at, first, row_base, lane, release);
         continue;
@@ -946,7 +947,10 @@ split_tail_kernel(const float* __restrict__ ws, int splits, int M, int N, __nv_b
   add_bias8(f, q.bias, 8 * g);
   if (pre) *reinterpret_cast<uint4*>(pre + r * ldc + 8 * g) = pack8(f);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = act_fwd(f[j], q.act);
+  for (int j = 0; j < 8; j += 2) {
+    if (q.act == 1) act_pair<1>(f[j], f[j + 1]);
+    else if (q.act == 2) act_pair<2>(f[j], f[j + 1]);
+  }
   if (q.drop.t) dropout8(f, dropout_draws(q.drop.first_row + r, g, dropout_key(q.drop)), q.drop.t, q.drop.scale);
   if (residual) add8(f, *reinterpret_cast<const uint4*>(residual + r * ldr + 8 * g));
   *reinterpret_cast<uint4*>(C + r * ldc + 8 * g) = pack8(f);

@@ -43,20 +43,23 @@ struct TailRow {
 };
 template <>
 struct TailRow<EPI_TAIL> {
-  uint4 res[8];      // 64 columns of the residual
+  uint4 res[4], bias[4];      // of 32 columns
   const __nv_bfloat16* src;
   long long row;
-  __device__ __forceinline__ void fetch8(const GemmParams& p, int col, int i) {
-    if (src && col + 8 * i < p.N) res[i] = load16_here(src + col + 8 * i);
+  __device__ __forceinline__ void fetch32(const GemmParams& p, int col) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool in = col + 8 * i < p.N;
+      if (src && in) res[i] = load16_here(src + col + 8 * i);
+      if (p.tail.bias && in) bias[i] = load16_here(p.tail.bias + col + 8 * i);
+    }
   }
   __device__ __forceinline__ void fetch(const GemmParams& p, int r, int col) {
     row = r;
     src = p.residual && r < p.M ? p.residual + static_cast<long long>(r) * p.ldr : nullptr;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      res[i] = make_uint4(0u, 0u, 0u, 0u);
-      fetch8(p, col, i);
-    }
+    for (int i = 0; i < 4; ++i) res[i] = bias[i] = make_uint4(0u, 0u, 0u, 0u);
+    fetch32(p, col);
   }
 };
 template <>
@@ -87,68 +90,89 @@ struct TailRow<EPI_DLOGITS> {
   }
 };
 
-template <int ACT>
-__device__ __forceinline__ void tail_chunk(const GemmParams& p, TailRow<EPI_TAIL>& tr, int i0, const uint32_t (&v)[32], uint32_t sy, int col0,
-                                           int next_col, PhiloxKey key, int lane) {
-  const TailParams& q = p.tail;
+// 32 values plus 32 packed ones
+__device__ __forceinline__ void add32(float (&f)[32], const uint4 (&u)[4]) {
 #pragma unroll
-  for (int i = i0; i < i0 + 4; ++i) {
-    const int col = col0 + 8 * i;
-    float f[8];
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(v[8 * (i - i0) + j]);
-    if (col < p.N) add_bias8(f, q.bias, col);
-    if (q.has_pre) {
-      const uint4 z = pack8(f);
-      st_shared_v4(epi_piece_addr(sy + 4096, lane, i), z.x, z.y, z.z, z.w);
+    for (int j = 0; j < 4; ++j) {
+      float& a = f[8 * i + 2 * j];
+      float& b = f[8 * i + 2 * j + 1];
+      f2_unpack(f2_add(f2_pack(a, b), f2_pack(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u))), a, b);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = act_fwd(f[j], ACT);
-    if (q.drop.t) dropout8(f, dropout_draws(q.drop.first_row + tr.row, col >> 3, key), q.drop.t, q.drop.scale);
-    if (p.residual) {
-      add8(f, tr.res[i]);
-      if (next_col >= 0) tr.fetch8(p, next_col, i);
-    }
-    const uint4 y = pack8(f);
-    st_shared_v4(epi_piece_addr(sy, lane, i), y.x, y.y, y.z, y.w);
   }
 }
+__device__ __forceinline__ void park32(uint32_t at, int lane, int piece, const float (&f)[32]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    st_shared_v4(epi_piece_addr(at, lane, piece + i), pack_bf16(f[8 * i], f[8 * i + 1]), pack_bf16(f[8 * i + 2], f[8 * i + 3]),
+                 pack_bf16(f[8 * i + 4], f[8 * i + 5]), pack_bf16(f[8 * i + 6], f[8 * i + 7]));
+}
+template <int ACT>
+__device__ __forceinline__ void act32(float (&f)[32]) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 2) act_pair<ACT>(f[i], f[i + 1]);
+}
 
-// `at`: TMEM address of this warp's rows and first column, `first` that column in C
+// `at`: TMEM address of this warp's rows and first column, `first` that column in C; `side`: of two parking places (without
+// pre-activations they take turns, from tile to tile) the next
 template <int BN, typename Release>
 __device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMap& tmC, TailRow<EPI_TAIL>& tr, uint8_t* stage_at, uint32_t at,
-                                           int first, int row_base, int lane, Release release) {
+                                           int first, int row_base, int lane, uint32_t& side, Release release) {
   const TailParams& q = p.tail;
-  const uint32_t sy = smem_u32(stage_at);
   PhiloxKey key{0u, 0u};
   if (q.drop.t) key = dropout_key(q.drop);
   bool held = true;
 #pragma unroll 1
-  for (int c = 0; c < BN / 2; c += 64) {
+  for (int c = 0; c < BN / 2; c += 32) {
     const int col0 = first + c;
     if (col0 >= p.N || row_base >= p.M) break;      // uniform across the warp
-    if (lane == 0) bulk_wait_read_all();            // the copy engine has read what was parked before
-    __syncwarp();
-    const int next_col = c + 64 < BN / 2 ? col0 + 64 : -1;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    float f[32];
+    {
       uint32_t v[32];
-      tmem_ld_32x32b_x32(at + c + 32 * h, v);
+      tmem_ld_32x32b_x32(at + c, v);
       tmem_ld_wait();
-      if (h == 1 && c + 64 >= BN / 2) {
-        release();
-        held = false;
-      }
-      if (q.act == 1) tail_chunk<1>(p, tr, 4 * h, v, sy, col0, next_col, key, lane);
-      else if (q.act == 2) tail_chunk<2>(p, tr, 4 * h, v, sy, col0, next_col, key, lane);
-      else tail_chunk<0>(p, tr, 4 * h, v, sy, col0, next_col, key, lane);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
     }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      if (q.has_pre) tma_store_3d(&tmC, stage_at + 4096, col0, row_base, q.pre_z);
-      tma_store_3d(&tmC, stage_at, col0, row_base, q.has_pre ? 1 - q.pre_z : 0);
-      bulk_commit_group();
+    const bool last = c + 32 >= BN / 2;
+    if (last) {
+      release();
+      held = false;
+    }
+    const int half = (c >> 5) & 1;                  // of the 64 columns that are parked together
+    if (half == 0) {
+      // the copy engine has read what was parked there before
+      if (lane == 0) {
+        if (q.has_pre) bulk_wait_read_all();
+        else bulk_wait_read_but_one();
+      }
+      __syncwarp();
+    }
+    const uint32_t sy = smem_u32(stage_at) + (q.has_pre ? 0u : side);
+    if (q.bias) add32(f, tr.bias);
+    if (q.has_pre) park32(sy + 4096, lane, 4 * half, f);
+    if (q.act == 1) act32<1>(f);
+    else if (q.act == 2) act32<2>(f);
+    if (q.drop.t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        dropout8(f + 8 * i, dropout_draws(q.drop.first_row + tr.row, (col0 >> 3) + i, key), q.drop.t, q.drop.scale);
+    }
+    if (p.residual) add32(f, tr.res);
+    if (!last) tr.fetch32(p, col0 + 32);
+    park32(sy, lane, 4 * half, f);
+    if (half == 1 || last || col0 + 32 >= p.N) {
+      const int x = col0 - 32 * half;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (q.has_pre) tma_store_3d(&tmC, stage_at + 4096, x, row_base, q.pre_z);
+        tma_store_3d(&tmC, stage_at + (q.has_pre ? 0u : side), x, row_base, q.has_pre ? 1 - q.pre_z : 0);
+        bulk_commit_group();
+      }
+      side ^= 4096u;
     }
   }
   if (held) release();

@@ -44,7 +44,7 @@ __device__ __forceinline__ uint4 dropout_draws(long long row, uint32_t g, Philox
   return philox(g, 0u, static_cast<uint32_t>(row), static_cast<uint32_t>(static_cast<uint64_t>(row) >> 32), k);
 }
 // eight values: what stays times the factor, the rest zero (whatever it was)
-__device__ __forceinline__ void dropout8(float (&f)[8], const uint4& u, uint32_t t, float scale) {
+__device__ __forceinline__ void dropout8(float* f, const uint4& u, uint32_t t, float scale) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
