@@ -378,8 +378,17 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         krange(x, k0, nkb);
         if (!mbar_wait(&tempty[acc], acc_phase ^ 1, KID_GEMM, 2)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t d_tmem = tmem_base + acc * BN;
+        uint32_t d_tmem = tmem_base + acc * BN;
         for (int kb = 0; kb < nkb; ++kb) {
+          if (EPI == EPI_LSE && kb > 0 && kb % LSE_RUN == 0) {
+            // this run of the sum goes to the epilogue, the next one into the other accumulator
+            if (PAIR) umma_commit_pair_w(leader, &tfull[acc]);
+            else umma_commit_w(leader, &tfull[acc]);
+            if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+            if (!mbar_wait(&tempty[acc], acc_phase ^ 1, KID_GEMM, 2)) { ok = false; break; }
+            tc_fence_after();
+            d_tmem = tmem_base + acc * BN;
+          }
           if (!mbar_wait(&full[stage], phase, KID_GEMM, 3, consumer_budget)) {
             if (p.ep.status && leader) atomicCAS(p.ep.status, 0, 0x10000 | (11 << 8));
             ok = false;
@@ -390,8 +399,9 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk) {
             const SmemDesc ak = desc_at(a, kk * (A_MN ? 2048 : 32)), bk = desc_at(b, kk * (B_MN ? 2048 : 32));
-            if (PAIR) umma_ss_pair_w(leader, d_tmem, ak, bk, idesc, (kb | kk) != 0);
-            else umma_ss_w(leader, d_tmem, ak, bk, idesc, (kb | kk) != 0);
+            const uint32_t more = EPI == EPI_LSE ? (kb % LSE_RUN | kk) != 0 : (kb | kk) != 0;
+            if (PAIR) umma_ss_pair_w(leader, d_tmem, ak, bk, idesc, more);
+            else umma_ss_w(leader, d_tmem, ak, bk, idesc, more);
           }
           if (PAIR) umma_commit_pair_w(leader, &empty[stage]);
           else umma_commit_w(leader, &empty[stage]);
@@ -425,6 +435,29 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       const long long gbase = static_cast<long long>(g) * p.c_group_stride;
       TailRow<EPI> tail;      // what the tail reads of this row, asked for ahead of the wait for the products
       if constexpr (EPI >= EPI_TAIL) tail.fetch(p, row, nt * BN + col_half * (BN / 2));
+      if constexpr (EPI == EPI_TAIL)
+        if (t + walkers < total_tiles) tail.ahead(p, next.mt * BM + lane_group * 32 + lane, next.nt * BN + col_half * (BN / 2), BN / 2);
+      if constexpr (EPI == EPI_LSE) {
+        float sum[BN / 2];
+#pragma unroll
+        for (int i = 0; i < BN / 2; ++i) sum[i] = 0.f;
+#pragma unroll 1
+        for (int kb = 0; kb < nkb && ok; kb += LSE_RUN) {
+          ok = mbar_wait(&tfull[acc], acc_phase, KID_GEMM, 4, consumer_budget);
+          if (!ok) break;
+          tc_fence_after();
+          tail_add<BN>(sum, tmem_base + acc * BN + (static_cast<uint32_t>(lane_group * 32) << 16) + col_half * (BN / 2));
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (PAIR) mbar_arrive_cluster(leader_addr(&tempty[acc]));
+            else mbar_arrive(&tempty[acc]);
+          }
+          if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+        }
+        if (ok) tail_stats<BN>(p, tail, sum, nt * BN + col_half * (BN / 2), 2 * nt + col_half, row);
+        continue;
+      }
       if (!mbar_wait(&tfull[acc], acc_phase, KID_GEMM, 4, consumer_budget)) { ok = false; break; }
       tc_fence_after();
       auto release = [&]() {      // the accumulator has been read
@@ -442,8 +475,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         const uint32_t at = t_row + col_half * (BN / 2);
         const int first = nt * BN + col_half * (BN / 2);
         if constexpr (EPI == EPI_TAIL) tail_store<BN>(p, tmC, tail, stage_at, at, first, row_base, lane, tail_side, release);
-        else if constexpr (EPI == EPI_LSE) tail_stats<BN>(p, tail, at, first, 2 * nt + col_half, row, release);
-        else tail_dlogits<BN>(p, tmC, tail, stage_at, at, first, row_base, lane, release);
+        else if constexpr (EPI == EPI_DLOGITS) tail_dlogits<BN>(p, tmC, tail, stage_at, at, first, row_base, lane, release);
         continue;
       }
       if (EPI == EPI_STORE && p.tma_out) {

@@ -54,6 +54,12 @@ struct TailRow<EPI_TAIL> {
       if (p.tail.bias && in) bias[i] = load16_here(p.tail.bias + col + 8 * i);
     }
   }
+  // `cols` columns of a row of the next tile into the L2: an epilogue of short sums is over before they would come from memory
+  __device__ __forceinline__ void ahead(const GemmParams& p, int r, int col, int cols) {
+    if (!p.residual || r >= p.M) return;
+    for (int c = col; c < col + cols && c < p.N; c += 64)
+      asm volatile("prefetch.global.L2 [%0];" ::"l"(p.residual + static_cast<long long>(r) * p.ldr + c));
+  }
   __device__ __forceinline__ void fetch(const GemmParams& p, int r, int col) {
     row = r;
     src = p.residual && r < p.M ? p.residual + static_cast<long long>(r) * p.ldr : nullptr;
@@ -178,59 +184,65 @@ __device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMa
   if (held) release();
 }
 
-template <int BN, typename Release>
-__device__ __forceinline__ void tail_stats(const GemmParams& p, const TailRow<EPI_LSE>& tr, uint32_t at, int first, int slot, int row,
-                                           Release release) {
-  const TailParams& q = p.tail;
-  float m = -1e30f, s = 0.f, w = 0.f;      // of no column at all: a weight of zero
-#pragma unroll 1
-  for (int c = 0; c < BN / 2; c += 32) {
-    const int col0 = first + c;
-    if (col0 >= p.N) break;                         // uniform across the warp
-    uint32_t v[32];
-    tmem_ld_32x32b_x32(at + c, v);
+// The tensor cores' fp32 sums are cut off, not rounded, at every addition: after 2048 products of random signs they are 1.4e-6 of their
+// size too near to zero, all of them to the same side, and the bias grows with the length (512: 3.1e-7).  Log-probabilities
+// leave in fp32, so their sums are run over LSE_RUN k-blocks at a time and the runs are added up in registers, rounded.
+constexpr int LSE_RUN = 8;
+
+template <int BN>
+__device__ __forceinline__ void tail_add(float (&sum)[BN / 2], uint32_t at) {
+#pragma unroll
+  for (int c = 0; c < BN / 2; c += 16) {
+    uint32_t v[16];
+    tmem_ld_32x32b_x16(at + c, v);
     tmem_ld_wait();
-    if (col0 + 32 > p.N) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (col0 + i >= p.N) v[i] = __float_as_uint(-1e30f);
-    }
-    const long long hit = tr.target - col0;
-    if (hit >= 0 && hit < 32) {
-      float l = 0.f;
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (hit == i) l = __uint_as_float(v[i]);
-      q.target_logit[row] = l;
-    }
-    float top = m;
-    float big = __uint_as_float(v[0]);
-#pragma unroll
-    for (int i = 1; i < 31; i += 2) big = fmax3(big, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-    big = fmaxf(big, __uint_as_float(v[31]));
-    top = fmaxf(m, big * LOG2E);
-    const float down = exp2_approx(m - top);
-    if (q.entropy) w = down * fmaf(s, m - top, w);
-    s *= down;
-    m = top;
-    float a0 = 0.f, a1 = 0.f, b0 = 0.f, b1 = 0.f;
-#pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-      const float d0 = fmaf(__uint_as_float(v[i]), LOG2E, -m), d1 = fmaf(__uint_as_float(v[i + 1]), LOG2E, -m);
-      const float e0 = exp2_approx(d0), e1 = exp2_approx(d1);
-      a0 += e0; a1 += e1;
-      if (q.entropy) { b0 = fmaf(e0, d0, b0); b1 = fmaf(e1, d1, b1); }
-    }
-    s += a0 + a1;
-    w += b0 + b1;
+    for (int i = 0; i < 16; i += 2)
+      f2_unpack(f2_add(f2_pack(sum[c + i], sum[c + i + 1]), f2_pack(__uint_as_float(v[i]), __uint_as_float(v[i + 1]))), sum[c + i], sum[c + i + 1]);
   }
-  release();
+}
+
+template <int BN>
+__device__ __forceinline__ void tail_stats(const GemmParams& p, const TailRow<EPI_LSE>& tr, float (&l)[BN / 2], int first, int slot, int row) {
+  const TailParams& q = p.tail;
+  if (first + BN / 2 > p.N) {
+#pragma unroll
+    for (int i = 0; i < BN / 2; ++i)
+      if (first + i >= p.N) l[i] = -1e30f;
+  }
+  const long long hit = tr.target - first;
+  if (hit >= 0 && hit < BN / 2) {
+    float at = 0.f;
+#pragma unroll
+    for (int i = 0; i < BN / 2; ++i)
+      if (hit == i) at = l[i];
+    q.target_logit[row] = at;
+  }
+  float big = fmaxf(l[0], l[1]);
+#pragma unroll
+  for (int i = 2; i < BN / 2; i += 2) big = fmax3(big, l[i], l[i + 1]);
+  const bool any = first < p.N;                 // of nothing: a weight of zero
+  const float m = any ? big * LOG2E : -1e30f;
+  float s0 = 0.f, s1 = 0.f, w0 = 0.f, w1 = 0.f;
+  const uint64_t log2e = f2_pack(LOG2E, LOG2E), down = f2_pack(-m, -m);
+  auto pass = [&](bool entropy) {
+#pragma unroll
+    for (int i = 0; i < BN / 2; i += 2) {
+      float d0, d1;
+      f2_unpack(f2_fma(f2_pack(l[i], l[i + 1]), log2e, down), d0, d1);
+      const float e0 = exp2_approx(d0), e1 = exp2_approx(d1);
+      s0 += e0; s1 += e1;
+      if (entropy) { w0 = fmaf(e0, d0, w0); w1 = fmaf(e1, d1, w1); }
+    }
+  };
+  if (q.entropy) pass(true);
+  else pass(false);
   if (row < p.M) {
     const long long slots = 2ll * p.n_tiles, plane = slots * p.M;
     float* dst = q.part + slot * static_cast<long long>(p.M) + row;
     dst[0] = m;
-    dst[plane] = s;
-    if (q.entropy) dst[2 * plane] = w;
+    dst[plane] = any ? s0 + s1 : 0.f;
+    if (q.entropy) dst[2 * plane] = any ? w0 + w1 : 0.f;
   }
 }
 

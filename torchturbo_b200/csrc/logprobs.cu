@@ -8,15 +8,15 @@
 
 namespace ttb {
 
-// 32 rows a block (neighbouring lanes, neighbouring rows), the pieces dealt out to its warps; joined in a fixed order.
-constexpr int JOIN_WARPS = 16;
+// Eight rows a block (a sector of neighbouring rows), the pieces dealt out to its 64 groups of eight lanes and joined in a fixed order.
+constexpr int JOIN_ROWS = 8, JOIN_GROUPS = 64;
 
-__global__ void __launch_bounds__(32 * JOIN_WARPS)
+__global__ void __launch_bounds__(JOIN_ROWS * JOIN_GROUPS)
 logprobs_join_kernel(const float* __restrict__ part, const float* __restrict__ target_logit, const long long* __restrict__ targets, int slots,
                      long long M, long long V, float* __restrict__ logp, float* __restrict__ lse, float* __restrict__ ent) {
-  __shared__ float sm[3][JOIN_WARPS][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long row = static_cast<long long>(blockIdx.x) * 32 + lane;
+  __shared__ float sm[3][JOIN_GROUPS][JOIN_ROWS];
+  const int lane = threadIdx.x % JOIN_ROWS, group = threadIdx.x / JOIN_ROWS;
+  const long long row = static_cast<long long>(blockIdx.x) * JOIN_ROWS + lane;
   const long long plane = static_cast<long long>(slots) * M;
   float m = -1e30f, s = 0.f, w = 0.f;
   auto join = [&](float m2, float s2, float w2) {
@@ -26,16 +26,30 @@ logprobs_join_kernel(const float* __restrict__ part, const float* __restrict__ t
     m = top;
   };
   if (row < M) {
-#pragma unroll 4
-    for (int i = warp; i < slots; i += JOIN_WARPS) {
-      const float* src = part + i * M + row;
-      join(src[0], src[plane], ent ? src[2 * plane] : 0.f);
+    constexpr int U = 8;      // loads under way
+    for (int i = group; i < slots; i += JOIN_GROUPS * U) {
+      float x[U], y[U], z[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int slot = i + u * JOIN_GROUPS;
+        const float* src = part + slot * M + row;
+        x[u] = slot < slots ? src[0] : -1e30f;
+        y[u] = slot < slots ? src[plane] : 0.f;
+        z[u] = ent && slot < slots ? src[2 * plane] : 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) join(x[u], y[u], z[u]);
     }
   }
-  sm[0][warp][lane] = m; sm[1][warp][lane] = s; sm[2][warp][lane] = w;
-  __syncthreads();
-  if (warp != 0 || row >= M) return;
-  for (int i = 1; i < JOIN_WARPS; ++i) join(sm[0][i][lane], sm[1][i][lane], sm[2][i][lane]);
+  sm[0][group][lane] = m; sm[1][group][lane] = s; sm[2][group][lane] = w;
+  for (int half = JOIN_GROUPS / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (group < half) {
+      join(sm[0][group + half][lane], sm[1][group + half][lane], sm[2][group + half][lane]);
+      sm[0][group][lane] = m; sm[1][group][lane] = s; sm[2][group][lane] = w;
+    }
+  }
+  if (group != 0 || row >= M) return;
   const float ln2 = 0.6931471805599453f, l2 = log2f(s), all = (m + l2) * ln2;
   const long long t = targets[row];
   logp[row] = t >= 0 && t < V ? target_logit[row] - all : 0.f;
@@ -53,7 +67,7 @@ TTB_EXPORT int ttb_logprobs_join(const float* part, const float* target_logit, c
                                  float* logp, float* lse, float* ent, void* stream) {
   using namespace ttb;
   if (M == 0) return 0;
-  logprobs_join_kernel<<<static_cast<unsigned>((M + 31) / 32), 32 * JOIN_WARPS, 0, static_cast<cudaStream_t>(stream)>>>(
+  logprobs_join_kernel<<<static_cast<unsigned>((M + JOIN_ROWS - 1) / JOIN_ROWS), JOIN_ROWS * JOIN_GROUPS, 0, static_cast<cudaStream_t>(stream)>>>(
       part, target_logit, targets, slots, M, V, logp, lse, ent);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 400 + static_cast<int>(e);
