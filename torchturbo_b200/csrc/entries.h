@@ -26,7 +26,7 @@ struct TailArgs {
   // 3: for every tile and half of its columns, of each row's logits: largest, sum of exponentials, sum of exponentials times distances
   float* part;                         // [3 or 2][slots][M], see logprobs.cu
   float* target_logit;                 // [M]
-  int entropy;
+  int entropy, tile_cols;              // ttb_logprobs_slots
   // 4: C = gradient of the logits of columns first_col .. first_col + N - 1
   const float *lse, *ent, *dlogp, *dent;   // [M]; `ent` and `dent` may be null
   long long first_col;
@@ -79,7 +79,7 @@ struct DeltaChunkIn {
 }  // namespace ttb
 
 TTB_EXPORT int ttb_gemm_bf16(const ttb::GemmArgs*, void*);
-TTB_EXPORT int ttb_logprobs_slots(int);
+TTB_EXPORT int ttb_logprobs_slots(int, int, int, int, int*);
 TTB_EXPORT int ttb_logprobs_join(const float*, const float*, const long long*, int, long long, long long, float*, float*, float*, void*);
 TTB_EXPORT int ttb_dropout(const void*, const void*, void*, int, long long, int, unsigned, float, unsigned long long, const unsigned long long*,
                             long long, int, void*);

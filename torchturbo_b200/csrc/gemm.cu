@@ -105,6 +105,7 @@ struct GemmParams {
   FastDiv by_group, by_band, by_rest;   // tile counts: of a group, of a whole band, rows of the last band
   int k_splits, kb_per_split;  // > 1: "group" g covers k-blocks [g, g + 1) * kb_per_split of one product, stored at C[g]
   TailParams tail;
+  int tile_cols;   // columns of a tile whose results are not stored (EPI_LSE)
 };
 
 template <int BN, bool PAIR, int EPI>
@@ -260,7 +261,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       int k0, nkb;
       krange(x, k0, nkb);
       const int m0 = x.mt * BM;
-      const int n0 = x.nt * (EPI == EPI_SWIGLU ? BN / 2 : BN);
+      const int bn = EPI == EPI_LSE ? p.tile_cols : BN;
+      const int n0 = x.nt * (EPI == EPI_SWIGLU ? BN / 2 : bn);
       const int bgroup = p.tile_group ? x.a : 0;
       for (int kb = 0; kb < nkb; ++kb) {
         if (!mbar_wait(&empty[stage], phase ^ 1, KID_GEMM, 1)) return false;
@@ -268,7 +270,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         uint8_t* sb = sa + L::A_BYTES;
         // a pair's loads all complete on the leading CTA's barrier, which expects both shares
         const uint32_t bar = PAIR ? leader_addr(&full[stage]) : 0u;
-        if (rank == 0) mbar_expect_tx(&full[stage], (PAIR ? 2 : 1) * L::STAGE_BYTES);
+        if (rank == 0)
+          mbar_expect_tx(&full[stage], EPI == EPI_LSE ? (PAIR ? 2 : 1) * L::A_BYTES + bn * BK * 2 : (PAIR ? 2 : 1) * L::STAGE_BYTES);
         auto load_a = [&](void* dst, int x, int y) {
           if (PAIR) tma_load_2d_pair(dst, &tmA, bar, x, y);
           else tma_load_2d(dst, &tmA, &full[stage], x, y);
@@ -286,7 +289,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         }
         if (!B_MN) {
           if (PAIR) {
-            load_b(sb, kc, EPI == EPI_SWIGLU ? rank * p.F + n0 : n0 + rank * (BN / 2));
+            load_b(sb, kc, EPI == EPI_SWIGLU ? rank * p.F + n0 : n0 + rank * (bn / 2));
           } else if (EPI == EPI_SWIGLU) {
             load_b(sb, kc, n0);
             load_b(sb + (BN / 2) * 128, kc, p.F + n0);
@@ -361,7 +364,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (the whole warp, see umma_ss_w)
     if (rank == 0) {
-      constexpr uint32_t idesc = make_idesc_bf16(PAIR ? 2 * BM : BM, BN, A_MN, B_MN);
+      constexpr uint32_t whole = make_idesc_bf16(PAIR ? 2 * BM : BM, BN, A_MN, B_MN);
+      const uint32_t idesc = EPI == EPI_LSE ? make_idesc_bf16(PAIR ? 2 * BM : BM, p.tile_cols, A_MN, B_MN) : whole;
       const uint32_t leader = elect_one() ? 1u : 0u;
       const SmemDesc dA = make_smem_desc2(smem_u32(smem), A_MN ? 8192 : 16, 1024);
       const SmemDesc dB = make_smem_desc2(smem_u32(smem) + L::A_BYTES, B_MN ? 8192 : 16, 1024);
@@ -438,6 +442,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       if constexpr (EPI == EPI_TAIL)
         if (t + walkers < total_tiles) tail.ahead(p, next.mt * BM + lane_group * 32 + lane, next.nt * BN + col_half * (BN / 2), BN / 2);
       if constexpr (EPI == EPI_LSE) {
+        const int mine = p.tile_cols / 2, first = nt * p.tile_cols + col_half * mine;      // of this warp's columns
         float sum[BN / 2];
 #pragma unroll
         for (int i = 0; i < BN / 2; ++i) sum[i] = 0.f;
@@ -446,7 +451,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
           ok = mbar_wait(&tfull[acc], acc_phase, KID_GEMM, 4, consumer_budget);
           if (!ok) break;
           tc_fence_after();
-          tail_add<BN>(sum, tmem_base + acc * BN + (static_cast<uint32_t>(lane_group * 32) << 16) + col_half * (BN / 2));
+          tail_add<BN>(sum, tmem_base + acc * BN + (static_cast<uint32_t>(lane_group * 32) << 16) + col_half * mine, mine);
           tc_fence_before();
           __syncwarp();
           if (lane == 0) {
@@ -455,7 +460,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
           }
           if (++acc == 2) { acc = 0; acc_phase ^= 1; }
         }
-        if (ok) tail_stats<BN>(p, tail, sum, nt * BN + col_half * (BN / 2), 2 * nt + col_half, row);
+        if (ok) tail_stats<BN>(p, tail, sum, first, max(0, min(mine, p.N - first)), 2 * nt + col_half, row);
         continue;
       }
       if (!mbar_wait(&tfull[acc], acc_phase, KID_GEMM, 4, consumer_budget)) { ok = false; break; }
@@ -1029,7 +1034,7 @@ static int launch(const GemmArgs& a, cudaStream_t stream) {
       dims[0] = static_cast<uint64_t>(a.K);
       dims[1] = rows_b;
       box[0] = BK;
-      box[1] = (EPI == EPI_SWIGLU || PAIR) ? BN / 2 : BN;
+      box[1] = EPI == EPI_LSE ? (PAIR ? a.tail->tile_cols / 2 : a.tail->tile_cols) : (EPI == EPI_SWIGLU || PAIR) ? BN / 2 : BN;
     } else {
       // memory [K rows][N contiguous]
       dims[0] = static_cast<uint64_t>(n_mem);
@@ -1061,7 +1066,7 @@ static int launch(const GemmArgs& a, cudaStream_t stream) {
     p.ep.ret_rows = e.ret_rows;
   }
   p.M = a.M; p.N = a.N; p.K = a.K;
-  constexpr int TN = (EPI == EPI_SWIGLU) ? BN / 2 : BN;
+  const int TN = EPI == EPI_LSE ? a.tail->tile_cols : EPI == EPI_SWIGLU ? BN / 2 : BN;
   constexpr int TM = PAIR ? 2 * BM : BM;
   p.m_tiles = a.tile_group ? a.m_tiles_cap : (a.M + TM - 1) / TM;
   p.n_tiles = (a.N + TN - 1) / TN;
@@ -1072,13 +1077,14 @@ static int launch(const GemmArgs& a, cudaStream_t stream) {
   p.tile_group = a.tile_group; p.group_rows = a.group_rows;
   p.F = a.F; p.row_scale = a.row_scale; p.alpha = a.alpha;
   p.preact = reinterpret_cast<__nv_bfloat16*>(a.preact); p.ld_preact = a.ld_preact;
-  p.k_splits = 1; p.kb_per_split = 0;
+  p.k_splits = 1; p.kb_per_split = 0; p.tile_cols = BN;
   memset(&p.tail, 0, sizeof(p.tail));
   if (a.tail) {
     const TailArgs& t = *a.tail;
     p.tail.bias = reinterpret_cast<const __nv_bfloat16*>(t.bias); p.tail.act = t.act;
     p.tail.drop = DropoutParams{t.drop_t, t.drop_scale, t.seed, t.seed_dev, t.first_row};
     p.tail.targets = t.targets; p.tail.vocab = t.vocab; p.tail.part = t.part; p.tail.target_logit = t.target_logit; p.tail.entropy = t.entropy;
+    if (EPI == EPI_LSE) p.tile_cols = t.tile_cols;
     p.tail.lse = t.lse; p.tail.ent = t.ent; p.tail.dlogp = t.dlogp; p.tail.dent = t.dent; p.tail.first_col = t.first_col;
   }
   const bool split = a.split_ws != nullptr && a.k_splits > 1;
@@ -1182,7 +1188,27 @@ static bool pays_in_pairs(const GemmArgs& a) {
   return 19 * two <= 20 * one && one * kb >= 48;
 }
 
+// Width of the column tiles of a product whose results are not stored, which no edge of a stored box ties to 64: the waves that tiles of
+// 256 columns would take, with equal work for all of them.  One wave more or less is most where rows are few and the weight streams by
+// (61 x 2048 x 151936: 594 tiles of 256 on 148 SMs are four waves and two tiles, 731 of 208 are five of nearly the same size).
+static int stats_tile_cols(const GemmArgs& a, bool pair) {
+  const long long walkers = pair ? a.num_sms / 2 : a.num_sms, mt = (a.M + (pair ? 2 * BM : BM) - 1) / (pair ? 2 * BM : BM);
+  const long long waves = (mt * ((a.N + 255) / 256) + walkers - 1) / walkers;
+  const long long across = waves * walkers / mt;            // tiles that a band of rows may have
+  const long long cols = (a.N + across - 1) / across;
+  return static_cast<int>((cols + 31) / 32 * 32);
+}
+
 }  // namespace ttb
+
+// Pieces that the statistics of N columns come in for each row (two for every tile of columns), and the width of a tile
+TTB_EXPORT int ttb_logprobs_slots(int M, int N, int K, int num_sms, int* tile_cols) {
+  using namespace ttb;
+  GemmArgs a{};
+  a.M = M; a.N = N; a.K = K; a.num_sms = num_sms; a.epi = EPI_LSE;
+  *tile_cols = stats_tile_cols(a, pays_in_pairs(a));
+  return 2 * ((N + *tile_cols - 1) / *tile_cols);
+}
 
 // Returns 0 on success; non-zero codes: 10000+r / 20000+r tensor-map encode failure of A / B (r = CUresult),
 // 300+e shared-memory opt-in, 400+e launch (e = cudaError_t), 9xx bad arguments.
@@ -1223,8 +1249,12 @@ TTB_EXPORT int ttb_gemm_bf16(const ttb::GemmArgs* args, void* stream_ptr) {
   if (a.epi == E) \
     return wide ? (pair ? launch<256, false, false, E, true>(a, stream) : launch<256, false, false, E, false>(a, stream)) \
                 : launch<128, false, false, E, false>(a, stream);
+    if (a.epi == EPI_LSE) {
+      // both sides of the call agree on the tiles by asking the same function (ttb_logprobs_slots)
+      if (a.tail->tile_cols != stats_tile_cols(a, pays_in_pairs(a))) return 913;
+      return pays_in_pairs(a) ? launch<256, false, false, EPI_LSE, true>(a, stream) : launch<256, false, false, EPI_LSE, false>(a, stream);
+    }
     TTB_TAIL(EPI_TAIL)
-    TTB_TAIL(EPI_LSE)
     TTB_TAIL(EPI_DLOGITS)
 #undef TTB_TAIL
   }

@@ -185,14 +185,16 @@ __device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMa
 }
 
 // The tensor cores' fp32 sums are cut off, not rounded, at every addition: after 2048 products of random signs they are 1.4e-6 of their
-// size too near to zero, all of them to the same side, and the bias grows with the length (512: 3.1e-7).  Log-probabilities
-// leave in fp32, so their sums are run over LSE_RUN k-blocks at a time and the runs are added up in registers, rounded.
-constexpr int LSE_RUN = 8;
+// size too near to zero, all of them to the same side, and the bias grows with the length (1024: 6.6e-7, 512: 3.1e-7).
+// Log-probabilities leave in fp32, so their sums are run over LSE_RUN k-blocks at a time and the runs are added up in registers, rounded.
+// 4096 x 2048 x 151936 under the power cap: one run 1815 us, runs of 16 blocks 1816, of 8 blocks 1877.
+constexpr int LSE_RUN = 16;
 
 template <int BN>
-__device__ __forceinline__ void tail_add(float (&sum)[BN / 2], uint32_t at) {
+__device__ __forceinline__ void tail_add(float (&sum)[BN / 2], uint32_t at, int cols) {
 #pragma unroll
   for (int c = 0; c < BN / 2; c += 16) {
+    if (c >= cols) break;
     uint32_t v[16];
     tmem_ld_32x32b_x16(at + c, v);
     tmem_ld_wait();
@@ -203,15 +205,16 @@ __device__ __forceinline__ void tail_add(float (&sum)[BN / 2], uint32_t at) {
 }
 
 template <int BN>
-__device__ __forceinline__ void tail_stats(const GemmParams& p, const TailRow<EPI_LSE>& tr, float (&l)[BN / 2], int first, int slot, int row) {
+__device__ __forceinline__ void tail_stats(const GemmParams& p, const TailRow<EPI_LSE>& tr, float (&l)[BN / 2], int first, int cols, int slot,
+                                           int row) {
   const TailParams& q = p.tail;
-  if (first + BN / 2 > p.N) {
+  if (cols < BN / 2) {
 #pragma unroll
     for (int i = 0; i < BN / 2; ++i)
-      if (first + i >= p.N) l[i] = -1e30f;
+      if (i >= cols) l[i] = -1e30f;
   }
   const long long hit = tr.target - first;
-  if (hit >= 0 && hit < BN / 2) {
+  if (hit >= 0 && hit < cols) {
     float at = 0.f;
 #pragma unroll
     for (int i = 0; i < BN / 2; ++i)
@@ -221,7 +224,7 @@ __device__ __forceinline__ void tail_stats(const GemmParams& p, const TailRow<EP
   float big = fmaxf(l[0], l[1]);
 #pragma unroll
   for (int i = 2; i < BN / 2; i += 2) big = fmax3(big, l[i], l[i + 1]);
-  const bool any = first < p.N;                 // of nothing: a weight of zero
+  const bool any = cols > 0;                    // of nothing: a weight of zero
   const float m = any ? big * LOG2E : -1e30f;
   float s0 = 0.f, s1 = 0.f, w0 = 0.f, w1 = 0.f;
   const uint64_t log2e = f2_pack(LOG2E, LOG2E), down = f2_pack(-m, -m);

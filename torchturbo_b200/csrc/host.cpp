@@ -146,7 +146,7 @@ PyObject* wrap_all(const Ts&... ts) {
 // rows x last dimension
 Tensor rows2d(const Tensor& t) { return t.dim() == 2 ? t.contiguous() : t.reshape({-1, t.size(-1)}).contiguous(); }
 Tensor like_shape(const Tensor& t2, const Tensor& x) { return x.dim() == 2 ? t2 : t2.view(x.sizes()); }
-int logprobs_slots(int columns) { return ttb_logprobs_slots(columns); }
+int logprobs_slots(const GemmArgs& g, int* tile_cols) { return ttb_logprobs_slots(g.M, g.N, g.K, g.num_sms, tile_cols); }
 int kda_gate_row_blocks(long long rows, int heads) { return ttb_kda_gate_row_blocks(rows, heads); }
 int row_blocks(long long rows, const Tensor& t) { return static_cast<int>(std::max<long long>(1, std::min<long long>(rows, 2 * sms(t)))); }
 at::ScalarType out_type(bool f32out) { return f32out ? at::kFloat : at::kBFloat16; }
@@ -393,9 +393,9 @@ PyObject* logprobs_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     need(g.N > 0 && g.K > 0, "a vocabulary and hidden states of at least one value");
     const Tensor logp = empty({M}, at::kFloat, h), lse = empty({M}, at::kFloat, h), ent = want_ent ? empty({M}, at::kFloat, h) : Tensor();
     if (M == 0) return wrap_all(logp, lse, ent);
-    const int slots = logprobs_slots(g.N);
-    const Tensor part = empty({want_ent ? 3 : 2, slots, M}, at::kFloat, h), hit = empty({M}, at::kFloat, h);
     ttb::TailArgs t{};
+    const int slots = logprobs_slots(g, &t.tile_cols);
+    const Tensor part = empty({want_ent ? 3 : 2, slots, M}, at::kFloat, h), hit = empty({M}, at::kFloat, h);
     t.targets = static_cast<const long long*>(at_(targets)); t.vocab = g.N;
     t.part = f32w(part); t.target_logit = f32w(hit); t.entropy = want_ent;
     g.epi = 3; g.tail = &t;

@@ -59,9 +59,6 @@ logprobs_join_kernel(const float* __restrict__ part, const float* __restrict__ t
 
 }  // namespace ttb
 
-// pieces that the product of N columns leaves for each row: two for every tile of its columns (gemm.cu)
-TTB_EXPORT int ttb_logprobs_slots(int N) { return N > 128 ? 2 * ((N + 255) / 256) : 2 * ((N + 127) / 128); }
-
 // part: fp32 [3 with `ent`, else 2][slots][M]
 TTB_EXPORT int ttb_logprobs_join(const float* part, const float* target_logit, const long long* targets, int slots, long long M, long long V,
                                  float* logp, float* lse, float* ent, void* stream) {
