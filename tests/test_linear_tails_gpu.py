@@ -122,6 +122,15 @@ def test_long_sums_in_pieces(M, N, K, act, p):
     assert Kn.status() == (0, 0)
 
 
+@pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 6, 7, 8])
+@pytest.mark.parametrize("N, K", [(8, 8), (24, 264), (2376, 520), (1200, 1032), (4744, 256), (72, 4104)])
+def test_few_rows(M, N, K):
+    """Rows that the weight streams past: every share of K among warps, one and two columns a warp, ends inside a step."""
+    gen = torch.Generator().manual_seed(M + N + K)
+    for act, p in (("gelu", 0.3), (None, 0.0), ("gelu_tanh", 0.0)):
+        _check(_rand(gen, M, K, std=0.2), _rand(gen, N, K, std=0.2), _rand(gen, N), _rand(gen, M, N), act, p, 5, _rand(gen, M, N))
+
+
 def test_pairs_of_CTAs():
     """Tiles of 256 rows, the last of them with one half empty, and a last tile of columns that is cut."""
     gen = torch.Generator().manual_seed(4)

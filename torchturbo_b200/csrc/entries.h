@@ -85,6 +85,7 @@ TTB_EXPORT int ttb_dropout(const void*, const void*, void*, int, long long, int,
                             long long, int, void*);
 TTB_EXPORT int ttb_tail_bwd(const void*, const void*, void*, float*, void*, int, long long, int, int, unsigned, float, unsigned long long,
                             const unsigned long long*, long long, int, void*);
+TTB_EXPORT int ttb_linear_rows(const ttb::GemmArgs*, void*);
 TTB_EXPORT int ttb_rmsnorm_fwd(const void*, const void*, const void*, void*, void*, float*, long long, int, float, int, void*);
 TTB_EXPORT int ttb_rmsnorm_bwd(const void*, const void*, const void*, const float*, const void*, void*, float*, void*, int, long
                             long, int, int, int, void*);

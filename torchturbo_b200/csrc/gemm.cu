@@ -106,6 +106,7 @@ struct GemmParams {
   int k_splits, kb_per_split;  // > 1: "group" g covers k-blocks [g, g + 1) * kb_per_split of one product, stored at C[g]
   TailParams tail;
   int tile_cols;   // columns of a tile whose results are not stored (EPI_LSE)
+  int a_bytes, stage_bytes, stages;   // of a product with a tail: A in a stage, a stage, how many there are
 };
 
 template <int BN, bool PAIR, int EPI>
@@ -117,6 +118,9 @@ struct SmemLayout {
   static constexpr int STAGES = ((BN == 256 && !PAIR) ? 4 : 6) - (EPI == EPI_TAIL ? 1 : 0);
   static constexpr int EPI_STAGE_BYTES = 32 * 32 * 4 * (EPI == EPI_TAIL ? 2 : 1);   // one 32-row x 32-column fp32 chunk per epilogue warp
   static constexpr int EPI_BYTES = 8 * EPI_STAGE_BYTES;
+  // A product with a tail cuts the room for its stages (statistics park nothing, so theirs is more) by what a stage really takes
+  static constexpr int ROOM = STAGES * STAGE_BYTES + (EPI == EPI_LSE ? EPI_BYTES : 0);
+  static constexpr int MOST = EPI >= EPI_TAIL ? 8 : STAGES;      // stages
   static constexpr int TOTAL = STAGES * STAGE_BYTES + EPI_BYTES + 1024 /*align*/ + 256 /*barriers*/;
 };
 
@@ -148,16 +152,17 @@ __global__ void __launch_bounds__(EPI < EPI_TAIL ? GEMM_THREADS_PUSH : GEMM_THRE
 gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
             const GemmParams p) {
   using L = SmemLayout<BN, PAIR, EPI>;
-  constexpr int STAGES = L::STAGES;
+  const int STAGES = EPI >= EPI_TAIL ? p.stages : L::STAGES;
+  const int stage_bytes = EPI >= EPI_TAIL ? p.stage_bytes : L::STAGE_BYTES, a_bytes = EPI >= EPI_TAIL ? p.a_bytes : L::A_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* epi_stage = smem + STAGES * L::STAGE_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * L::STAGE_BYTES + L::EPI_BYTES);
+  uint8_t* epi_stage = smem + L::STAGES * L::STAGE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::STAGES * L::STAGE_BYTES + L::EPI_BYTES);
   uint64_t* full = bars;
-  uint64_t* empty = bars + STAGES;
-  uint64_t* tfull = bars + 2 * STAGES;
-  uint64_t* tempty = bars + 2 * STAGES + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
+  uint64_t* empty = bars + L::MOST;
+  uint64_t* tfull = bars + 2 * L::MOST;
+  uint64_t* tempty = bars + 2 * L::MOST + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * L::MOST + 4);
 
   __shared__ uint32_t s_landed[32];   // push prologue: experts (up to 1024) whose rows are known to have landed
   __shared__ int s_last_cta;
@@ -266,12 +271,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       const int bgroup = p.tile_group ? x.a : 0;
       for (int kb = 0; kb < nkb; ++kb) {
         if (!mbar_wait(&empty[stage], phase ^ 1, KID_GEMM, 1)) return false;
-        uint8_t* sa = smem + stage * L::STAGE_BYTES;
-        uint8_t* sb = sa + L::A_BYTES;
+        uint8_t* sa = smem + stage * stage_bytes;
+        uint8_t* sb = sa + a_bytes;
         // a pair's loads all complete on the leading CTA's barrier, which expects both shares
         const uint32_t bar = PAIR ? leader_addr(&full[stage]) : 0u;
-        if (rank == 0)
-          mbar_expect_tx(&full[stage], EPI == EPI_LSE ? (PAIR ? 2 : 1) * L::A_BYTES + bn * BK * 2 : (PAIR ? 2 : 1) * L::STAGE_BYTES);
+        if (rank == 0) mbar_expect_tx(&full[stage], (PAIR ? 2 : 1) * stage_bytes);
         auto load_a = [&](void* dst, int x, int y) {
           if (PAIR) tma_load_2d_pair(dst, &tmA, bar, x, y);
           else tma_load_2d(dst, &tmA, &full[stage], x, y);
@@ -368,7 +372,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       const uint32_t idesc = EPI == EPI_LSE ? make_idesc_bf16(PAIR ? 2 * BM : BM, p.tile_cols, A_MN, B_MN) : whole;
       const uint32_t leader = elect_one() ? 1u : 0u;
       const SmemDesc dA = make_smem_desc2(smem_u32(smem), A_MN ? 8192 : 16, 1024);
-      const SmemDesc dB = make_smem_desc2(smem_u32(smem) + L::A_BYTES, B_MN ? 8192 : 16, 1024);
+      const SmemDesc dB = make_smem_desc2(smem_u32(smem) + a_bytes, B_MN ? 8192 : 16, 1024);
       int stage = 0;
       uint32_t phase = 0;
       int acc = 0;
@@ -399,7 +403,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
             break;
           }
           tc_fence_after();
-          const SmemDesc a = desc_at(dA, stage * L::STAGE_BYTES), b = desc_at(dB, stage * L::STAGE_BYTES);
+          const SmemDesc a = desc_at(dA, stage * stage_bytes), b = desc_at(dB, stage * stage_bytes);
 #pragma unroll
           for (int kk = 0; kk < BK / 16; ++kk) {
             const SmemDesc ak = desc_at(a, kk * (A_MN ? 2048 : 32)), bk = desc_at(b, kk * (B_MN ? 2048 : 32));
@@ -993,6 +997,10 @@ split_tail_kernel(const float* __restrict__ ws, int splits, int M, int N, __nv_b
   *reinterpret_cast<uint4*>(C + r * ldc + 8 * g) = pack8(f);
 }
 
+// Rows of A that a tile of a product with a tail loads: where one tile has them all, those that there are, in whole groups of eight (as
+// shared memory is laid out).  What the rest of the tile's rows hold stays in them, and nobody reads it.
+static int tail_rows(int M) { return M < BM ? (M + 7) / 8 * 8 : BM; }
+
 template <int BN, bool A_MN, bool B_MN, int EPI, bool PAIR>
 static int launch(const GemmArgs& a, cudaStream_t stream) {
   using L = SmemLayout<BN, PAIR, EPI>;
@@ -1007,7 +1015,7 @@ static int launch(const GemmArgs& a, cudaStream_t stream) {
       dims[0] = static_cast<uint64_t>(a.K);
       dims[1] = static_cast<uint64_t>(a.M);
       box[0] = BK;
-      box[1] = BM;
+      box[1] = EPI >= EPI_TAIL ? tail_rows(a.M) : BM;
     } else {
       // memory [K rows][M contiguous]
       dims[0] = static_cast<uint64_t>(a.M);
@@ -1077,7 +1085,7 @@ static int launch(const GemmArgs& a, cudaStream_t stream) {
   p.tile_group = a.tile_group; p.group_rows = a.group_rows;
   p.F = a.F; p.row_scale = a.row_scale; p.alpha = a.alpha;
   p.preact = reinterpret_cast<__nv_bfloat16*>(a.preact); p.ld_preact = a.ld_preact;
-  p.k_splits = 1; p.kb_per_split = 0; p.tile_cols = BN;
+  p.k_splits = 1; p.kb_per_split = 0; p.tile_cols = BN; p.a_bytes = tail_rows(a.M) * BK * 2;
   memset(&p.tail, 0, sizeof(p.tail));
   if (a.tail) {
     const TailArgs& t = *a.tail;
@@ -1096,6 +1104,8 @@ static int launch(const GemmArgs& a, cudaStream_t stream) {
     p.c_fp32 = 1; p.accumulate = 0; p.residual = nullptr; p.alpha = nullptr;
   }
 
+  p.stage_bytes = p.a_bytes + (PAIR ? p.tile_cols / 2 : p.tile_cols) * BK * 2;
+  p.stages = L::ROOM / p.stage_bytes < L::MOST ? L::ROOM / p.stage_bytes : L::MOST;
   const long long total = static_cast<long long>(p.m_tiles) * p.n_tiles * (p.groups_k > 0 ? p.groups_k : p.k_splits);
   if (total <= 0) return 0;
   if (total >= (1ll << 31) - 65536) return 910;
@@ -1241,7 +1251,9 @@ TTB_EXPORT int ttb_gemm_bf16(const ttb::GemmArgs* args, void* stream_ptr) {
     if (!a.tail || a.epi > EPI_DLOGITS || a.a_mn || a.b_mn || a.tile_group || a.groups_k > 0 || a.ep || a.alpha || a.accumulate || a.c_fp32) return 911;
     if (a.epi == EPI_TAIL && ((a.N % 8) || (reinterpret_cast<uintptr_t>(a.tail->pre) & 15) || (reinterpret_cast<uintptr_t>(a.tail->bias) & 15))) return 912;
     if (a.epi != EPI_TAIL && (a.split_ws || a.residual || !a.tail->targets)) return 912;
-    const bool wide = a.N > 128, pair = wide && pays_in_pairs(a);
+    // a product that leaves SMs without a tile of 128 columns has its tail done sooner on more of them
+    const bool wide = a.N > 128 && (a.epi != EPI_TAIL || static_cast<long long>((a.M + BM - 1) / BM) * ((a.N + 127) / 128) > a.num_sms);
+    const bool pair = wide && pays_in_pairs(a);
     if (a.epi == EPI_TAIL && a.split_ws && a.k_splits > 1)
       return wide ? (pair ? launch<256, false, false, EPI_STORE, true>(a, stream) : launch<256, false, false, EPI_STORE, false>(a, stream))
                   : launch<128, false, false, EPI_STORE, false>(a, stream);

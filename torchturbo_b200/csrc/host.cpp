@@ -295,6 +295,11 @@ GemmArgs product(const Tensor& a, const Tensor& b) {
   return g;
 }
 
+// Whether a linear layer's rows are so few that streaming the weight past them beats tiles of 128 rows, most of them empty.  Times in us,
+// rows kernel and tiles, weights from memory: 1 row 1152 x 1152 3.5 and 8.6, 4096 x 4096 8.0 and 22, 4096 -> 12288 20 and 38; 4 rows 3.9
+// and 8.7, 12 and 19, 28 and 34; 8 rows 6.4 and 8.6, 19 and 18, 46 and 34.
+bool few_rows(const GemmArgs& g) { return g.M <= 4 || (g.M <= 8 && static_cast<long long>(g.N) * g.K <= (1 << 23)); }
+
 PyObject* linear_tail(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Args in(args, n, 11);
@@ -322,6 +327,10 @@ PyObject* linear_tail(PyObject*, PyObject* const* args, Py_ssize_t n) {
     g.C = y.data_ptr(); g.ldc = N;
     g.epi = 2; g.tail = &t;
     Tensor ws;
+    if (few_rows(g)) {
+      launch("ttb_linear_rows", 1, [&](void* st) { return ttb_linear_rows(&g, st); });
+      return wrap_all(y, pre);
+    }
     const long long s = g.K >= 4096 ? k_splits(M, N, g.K, g.num_sms) : 1;
     if (s > 1) {
       ws = empty({s, M, N}, at::kFloat, x);

@@ -8,8 +8,9 @@
 
 namespace ttb {
 
-// Eight rows a block (a sector of neighbouring rows), the pieces dealt out to its 64 groups of eight lanes and joined in a fixed order.
-constexpr int JOIN_ROWS = 8, JOIN_GROUPS = 64;
+// Eight rows a block (a sector of neighbouring rows), the pieces dealt out to its 128 groups of eight lanes and joined in a fixed order,
+// four at a time under one largest: 1462 pieces are three rounds of loads.
+constexpr int JOIN_ROWS = 8, JOIN_GROUPS = 128;
 
 __global__ void __launch_bounds__(JOIN_ROWS * JOIN_GROUPS)
 logprobs_join_kernel(const float* __restrict__ part, const float* __restrict__ target_logit, const long long* __restrict__ targets, int slots,
@@ -26,7 +27,7 @@ logprobs_join_kernel(const float* __restrict__ part, const float* __restrict__ t
     m = top;
   };
   if (row < M) {
-    constexpr int U = 8;      // loads under way
+    constexpr int U = 4;
     for (int i = group; i < slots; i += JOIN_GROUPS * U) {
       float x[U], y[U], z[U];
 #pragma unroll
@@ -37,8 +38,16 @@ logprobs_join_kernel(const float* __restrict__ part, const float* __restrict__ t
         y[u] = slot < slots ? src[plane] : 0.f;
         z[u] = ent && slot < slots ? src[2 * plane] : 0.f;
       }
+      float top = x[0], sum = 0.f, dist = 0.f;
 #pragma unroll
-      for (int u = 0; u < U; ++u) join(x[u], y[u], z[u]);
+      for (int u = 1; u < U; ++u) top = fmaxf(top, x[u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float d = x[u] - top, e = exp2f(d);
+        sum += e * y[u];
+        if (ent) dist += e * (z[u] + y[u] * d);
+      }
+      join(top, sum, dist);
     }
   }
   sm[0][group][lane] = m; sm[1][group][lane] = s; sm[2][group][lane] = w;
