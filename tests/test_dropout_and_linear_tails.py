@@ -86,7 +86,7 @@ def test_seed_from_the_generator_of_the_host():
     assert torch.equal(a, ops.dropout(x, 0.5)) and not torch.equal(a, b)
 
 
-@pytest.mark.parametrize("bad", [dict(p=-0.1), dict(p=1.5), dict(p=float("nan")), dict(p=0.1, seed=-1), dict(p=0.1, seed=2 ** 63), dict(p=0.1, seed=1.0),
+@pytest.mark.parametrize("bad", [dict(p=-0.1), dict(p=1.5), dict(p=float("nan")), dict(p=float("inf")), dict(p=0.1, seed=-1), dict(p=0.1, seed=2 ** 63), dict(p=0.1, seed=1.0),
                                  dict(p=0.1, seed=True), dict(p=0.1, seed=torch.tensor([1, 2])), dict(p=0.1, seed=torch.tensor(1.0)),
                                  dict(p=0.1, seed=1, first_row=-1)])
 def test_refused_dropout_arguments(bad):

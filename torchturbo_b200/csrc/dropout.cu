@@ -16,26 +16,100 @@ __device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
   *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
   *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
 }
+// a load that stays where it is written: the compiler otherwise moves the unpacking of a row up to its load, and the thread waits there
+__device__ __forceinline__ uint4 load16_here(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-// y = residual + dropout(x), rows of whole groups of eight columns, a group a thread.
+// A block's threads lie over groups of eight columns, and over rows where a row has fewer groups than a block threads; a thread keeps its
+// column group and walks rows.
+struct Walk {
+  int across, per_block, down;      // groups of a row, groups that a block covers, rows that it covers at a time
+};
+static Walk walk_of(int groups) {
+  Walk w{groups, groups < 256 ? groups : 256, 1};
+  w.down = 256 / w.per_block;
+  return w;
+}
+
+// Eight values as they lie in memory
 template <typename T>
-__global__ void __launch_bounds__(256)
-dropout_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* __restrict__ y, int groups, FastDiv by_row, int per_row, DropoutParams d) {
-  const PhiloxKey key = dropout_key(d);
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < groups; i += gridDim.x * 256) {
-    const int row = by_row(i), g = i - row * per_row;
-    float f[8];
-    load8(x + 8ll * i, f);
-    dropout8(f, dropout_draws(d.first_row + row, g, key), d.t, d.scale);
-    if (residual) {
-      float r[8];
-      load8(residual + 8ll * i, r);
+struct Raw {
+  uint4 u[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] += r[j];
+    for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) u[i] = load16_here(reinterpret_cast<const uint4*>(p) + i);
+  }
+  __device__ __forceinline__ void values(float (&f)[8]) const {
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t w[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[2 * j] = __uint_as_float(w[j] << 16);
+        f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    } else {
+      const uint32_t w[8] = {u[0].x, u[0].y, u[0].z, u[0].w, u[1].x, u[1].y, u[1].z, u[1].w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = __uint_as_float(w[j]);
     }
-    store8(y + 8ll * i, f);
+  }
+};
+
+// y = residual + dropout(x), rows of whole groups of eight columns; two rows at a time, the next two's loads ahead of their arithmetic.
+template <typename T, typename Keys, bool RES>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 || !RES ? 3 : 2)
+dropout_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* __restrict__ y, long long R, Walk w, const DropoutParams d) {
+  const int at = threadIdx.x % w.per_block, g = blockIdx.x * w.per_block + at;
+  if (g >= w.across || static_cast<int>(threadIdx.x) >= w.down * w.per_block) return;
+  const Keys key(d);
+  const uint32_t top = d.t << 16;
+  const long long step = static_cast<long long>(gridDim.y) * w.down, stride = static_cast<long long>(w.across) * 8;
+  long long row = static_cast<long long>(blockIdx.y) * w.down + threadIdx.x / w.per_block;
+  uint32_t high = static_cast<uint32_t>(static_cast<uint64_t>(d.first_row + row) >> 32);
+  PhiloxColumn col = philox_column(g, high, key);
+  constexpr int U = 2;
+  Raw<T> xn[U], rn[U];
+  auto load = [&](long long first) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (first + u * step >= R) return;
+      xn[u].load(x + (first + u * step) * stride + 8 * g);
+      if (RES) rn[u].load(residual + (first + u * step) * stride + 8 * g);
+    }
+  };
+  load(row);
+  for (; row < R; row += U * step) {
+    Raw<T> xs[U], rs[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      xs[u] = xn[u];
+      if (RES) rs[u] = rn[u];
+    }
+    load(row + U * step);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (row + u * step >= R) break;
+      const uint64_t i = static_cast<uint64_t>(d.first_row + row + u * step);
+      if (static_cast<uint32_t>(i >> 32) != high) {
+        high = static_cast<uint32_t>(i >> 32);
+        col = philox_column(g, high, key);
+      }
+      float f[8];
+      xs[u].values(f);
+      dropout8(f, philox(col, philox_row(static_cast<uint32_t>(i), key), key), top, d.scale);
+      if (RES) {
+        float r[8];
+        rs[u].values(r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] += r[j];
+      }
+      store8(y + (row + u * step) * stride + 8 * g, f);
+    }
   }
 }
 
@@ -45,9 +119,9 @@ constexpr int FLAT = 2048;
 template <typename T>
 __global__ void __launch_bounds__(256)
 dropout_flat_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* __restrict__ y, long long n, int C, FastDiv by_c, int G,
-                    FastDiv by_g, DropoutParams d) {
+                    FastDiv by_g, const DropoutParams d) {
   extern __shared__ uint4 draws[];
-  const PhiloxKey key = dropout_key(d);
+  const KeysOfSeed key(d);
   const long long e0 = static_cast<long long>(blockIdx.x) * FLAT;
   const int cnt = static_cast<int>(n - e0 < FLAT ? n - e0 : FLAT);
   const long long r0 = e0 / C;
@@ -107,53 +181,100 @@ dropout_flat_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* 
   }
 }
 
-// Backward of C = residual + dropout(act(z)):  dz = dropout(dy) act'(z), and its column sums.  Blocks walk rows of up to 8192 columns
-// (blockIdx.y: which), eight columns a thread, the next row's loads ahead of this one's arithmetic, as the backward of the separate
-// bias and activation does; `dz` is null where it is dy itself, `part` where no sums are wanted.
-template <int ACT, bool DROP>
-__global__ void __launch_bounds__(1024)
+// Backward of C = residual + dropout(act(z)):  dz = dropout(dy) act'(z), and its column sums (partial ones per block of rows, reduced by
+// colsum_kernel).  `dz` is null where it is dy itself.  Two rows at a time, the next two's loads ahead of their arithmetic.
+template <int ACT, bool DROP, bool SUM, typename Keys>
+__global__ void __launch_bounds__(256, 3)
 tail_bwd_kernel(const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ z, __nv_bfloat16* __restrict__ dz,
-                float* __restrict__ part, long long R, int C, DropoutParams d) {
-  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * 8;
-  if (c >= C) return;
-  PhiloxKey key{0u, 0u};
-  if (DROP) key = dropout_key(d);
+                float* __restrict__ part, int R, Walk w, const DropoutParams d) {
+  __shared__ float sums[SUM ? 256 * 8 : 1];
+  const int at = threadIdx.x % w.per_block, down = threadIdx.x / w.per_block, g = blockIdx.x * w.per_block + at;
+  const bool live = g < w.across && down < w.down;
   float acc[8] = {};
-  uint4 du = make_uint4(0, 0, 0, 0), zu = du;
-  auto load = [&](long long row) {
-    if (row >= R) return;
-    du = *reinterpret_cast<const uint4*>(dy + row * C + c);
-    if (ACT) zu = *reinterpret_cast<const uint4*>(z + row * C + c);
-  };
-  load(blockIdx.x);
-  for (long long row = blockIdx.x; row < R; row += gridDim.x) {
-    const uint32_t ds[4] = {du.x, du.y, du.z, du.w}, zs[4] = {zu.x, zu.y, zu.z, zu.w};
-    load(row + gridDim.x);
-    float f[8];
+  if (live) {
+    const Keys key(d);
+    const uint32_t top = d.t << 16;
+    const long long stride = static_cast<long long>(w.across) * 8;
+    const int step = gridDim.y * w.down;
+    int row = blockIdx.y * w.down + down;
+    uint32_t high = static_cast<uint32_t>(static_cast<uint64_t>(d.first_row + row) >> 32);
+    PhiloxColumn col;
+    if (DROP) col = philox_column(g, high, key);
+    constexpr int U = 2;
+    uint4 du[U], zu[U];
+    auto load = [&](int first) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 g = unpack_bf16(ds[j]);
-      f[2 * j] = g.x; f[2 * j + 1] = g.y;
-    }
-    if (DROP) dropout8(f, dropout_draws(d.first_row + row, c >> 3, key), d.t, d.scale);
-    if (ACT) {
+      for (int u = 0; u < U; ++u) {
+        const long long i = static_cast<long long>(first) + static_cast<long long>(u) * step;
+        if (i >= R) return;
+        du[u] = load16_here(dy + i * stride + 8 * g);
+        if (ACT) zu[u] = load16_here(z + i * stride + 8 * g);
+      }
+    };
+    load(row);
+    for (long long at_row = row; at_row < R; at_row += U * step) {
+      uint4 ds[U], zs[U];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float2 v = unpack_bf16(zs[j]);
-        f[2 * j] *= act_slope<ACT>(v.x);
-        f[2 * j + 1] *= act_slope<ACT>(v.y);
+      for (int u = 0; u < U; ++u) {
+        ds[u] = du[u];
+        if (ACT) zs[u] = zu[u];
+      }
+      if (at_row + U * step < R) load(static_cast<int>(at_row) + U * step);
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long i = at_row + static_cast<long long>(u) * step;
+        if (i >= R) break;
+        float f[8];
+        const uint32_t dw[4] = {ds[u].x, ds[u].y, ds[u].z, ds[u].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[2 * j] = __uint_as_float(dw[j] << 16);
+          f[2 * j + 1] = __uint_as_float(dw[j] & 0xffff0000u);
+        }
+        if (DROP) {
+          const uint64_t whole = static_cast<uint64_t>(d.first_row + i);
+          if (static_cast<uint32_t>(whole >> 32) != high) {
+            high = static_cast<uint32_t>(whole >> 32);
+            col = philox_column(g, high, key);
+          }
+          dropout8(f, philox(col, philox_row(static_cast<uint32_t>(whole), key), key), top, d.scale);
+        }
+        if (ACT) {
+          const uint32_t zw[4] = {zs[u].x, zs[u].y, zs[u].z, zs[u].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float a = __uint_as_float(zw[j] << 16), b = __uint_as_float(zw[j] & 0xffff0000u);
+            act_slope_pair<ACT>(a, b);
+            f[2 * j] *= a;
+            f[2 * j + 1] *= b;
+          }
+        }
+        if (SUM) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) acc[j] += f[j];
+        }
+        if (DROP || ACT) store8(dz + i * stride + 8 * g, f);
       }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j] += f[j];
-    if (dz) store8(dz + row * C + c, f);
   }
-  if (!part) return;
-  store8(part + static_cast<long long>(blockIdx.x) * C + c, acc);
+  if (!SUM) return;
+  // the rows of the block that share a column, in a fixed order
+  if (w.down > 1) {
+    if (live) store8(sums + (down * w.per_block + at) * 8, acc);
+    __syncthreads();
+    if (!live || down != 0) return;
+    for (int i = 1; i < w.down; ++i) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] += sums[(i * w.per_block + at) * 8 + j];
+    }
+  } else if (!live) {
+    return;
+  }
+  store8(part + (static_cast<long long>(blockIdx.y) * w.across + g) * 8, acc);
 }
 
 template <typename T>
-static void dropout_rows(const void* x, const void* residual, void* y, long long R, int C, DropoutParams d, int sms, cudaStream_t st) {
+static void dropout_rows(const void* x, const void* residual, void* y, long long R, int C, const DropoutParams& d, int sms, cudaStream_t st) {
   const T *xs = static_cast<const T*>(x), *rs = static_cast<const T*>(residual);
   T* ys = static_cast<T*>(y);
   if (C % 8) {
@@ -165,13 +286,14 @@ static void dropout_rows(const void* x, const void* residual, void* y, long long
                                                                                                              fast_div(G), d);
     return;
   }
-  const int per_row = C / 8;
-  const long long most = std::max<long long>(1, ((1ll << 31) - (1 << 24)) / per_row);
-  for (long long a = 0; a < R; a += most, d.first_row += most) {
-    const int groups = static_cast<int>(std::min(most, R - a) * per_row);
-    const int blocks = std::min((groups + 255) / 256, sms * 8);
-    dropout_kernel<T><<<blocks, 256, 0, st>>>(xs + a * C, rs ? rs + a * C : nullptr, ys + a * C, groups, fast_div(per_row), per_row, d);
-  }
+  const Walk w = walk_of(C / 8);
+  const int bx = (w.across + w.per_block - 1) / w.per_block;
+  // three blocks an SM, which is what it holds
+  const long long rows = (R + w.down - 1) / w.down;
+  const unsigned by = static_cast<unsigned>(std::max<long long>(1, std::min<long long>({rows, 65535, (3ll * sms + bx - 1) / bx})));
+  auto go = [&](auto kernel) { kernel<<<dim3(bx, by), 256, 0, st>>>(xs, rs, ys, R, w, d); };
+  if (d.seed_dev) rs ? go(dropout_kernel<T, KeysOfSeed, true>) : go(dropout_kernel<T, KeysOfSeed, false>);
+  else rs ? go(dropout_kernel<T, KeysOfLaunch, true>) : go(dropout_kernel<T, KeysOfLaunch, false>);
 }
 
 }  // namespace ttb
@@ -183,37 +305,48 @@ TTB_EXPORT int ttb_dropout(const void* x, const void* residual, void* y, int fp3
                            unsigned long long seed, const unsigned long long* seed_dev, long long first_row, int sms, void* stream) {
   using namespace ttb;
   if (R == 0 || C == 0) return 0;
-  const DropoutParams d{t, scale, seed, seed_dev, first_row};
+  if (t > 65535) return 903;
+  const DropoutParams d = dropout_params(t, scale, seed, seed_dev, first_row);
   if (fp32) dropout_rows<float>(x, residual, y, R, C, d, sms, STREAM(stream));
   else dropout_rows<__nv_bfloat16>(x, residual, y, R, C, d, sms, STREAM(stream));
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 400 + static_cast<int>(e);
 }
 
-// part: grid * C floats, with `dbias` null it is not used.  dy, z, dz: [R, C] bf16 without gaps on 16-byte boundaries, C % 8 == 0, C <= 16384
+// Row blocks of ttb_tail_bwd, each of which leaves a row of `part`: three blocks an SM
+TTB_EXPORT int ttb_tail_row_blocks(long long R, int C, int sms) {
+  using namespace ttb;
+  const Walk w = walk_of(C / 8);
+  const int bx = (w.across + w.per_block - 1) / w.per_block;
+  return static_cast<int>(std::max<long long>(1, std::min<long long>((R + w.down - 1) / w.down, (3ll * sms + bx - 1) / bx)));
+}
+
+// part: [row blocks, C] floats, used with `dbias` alone.  dy, z, dz: [R, C] bf16 without gaps on 16-byte boundaries, C % 8 == 0
 TTB_EXPORT int ttb_tail_bwd(const void* dy, const void* z, void* dz, float* part, void* dbias, int out_bf16, long long R, int C, int act,
                             unsigned t, float scale, unsigned long long seed, const unsigned long long* seed_dev, long long first_row, int grid,
                             void* stream) {
   using namespace ttb;
   if (C % 8 || act < 0 || act > 2 || (act && !z)) return 901;
-  if (C > 16384) return 902;
+  if (t > 65535 || R >= (1ll << 30)) return 903;
   if (R == 0) return 0;
-  if (grid > R) grid = static_cast<int>(R);
-  const DropoutParams d{t, scale, seed, seed_dev, first_row};
-  const int width = C > 8192 ? (C + 15) / 16 * 8 : C, threads = (width / 8 + 31) / 32 * 32;
+  const DropoutParams d = dropout_params(t, scale, seed, seed_dev, first_row);
+  const Walk w = walk_of(C / 8);
   auto go = [&](auto kernel) {
-    kernel<<<dim3(grid, C > 8192 ? 2 : 1), threads, 0, STREAM(stream)>>>(
-        static_cast<const __nv_bfloat16*>(dy), static_cast<const __nv_bfloat16*>(z), static_cast<__nv_bfloat16*>(dz), dbias ? part : nullptr, R, C, d);
+    kernel<<<dim3((w.across + w.per_block - 1) / w.per_block, grid), 256, 0, STREAM(stream)>>>(
+        static_cast<const __nv_bfloat16*>(dy), static_cast<const __nv_bfloat16*>(z), static_cast<__nv_bfloat16*>(dz), part, static_cast<int>(R), w, d);
   };
-  if (t) {
-    if (act == 1) go(tail_bwd_kernel<1, true>);
-    else if (act == 2) go(tail_bwd_kernel<2, true>);
-    else go(tail_bwd_kernel<0, true>);
+#define TTB_ACT(DROP, SUM, KEYS)                              \
+  if (act == 1) go(tail_bwd_kernel<1, DROP, SUM, KEYS>);      \
+  else if (act == 2) go(tail_bwd_kernel<2, DROP, SUM, KEYS>); \
+  else go(tail_bwd_kernel<0, DROP, SUM, KEYS>);
+  if (t && seed_dev) {
+    if (dbias) { TTB_ACT(true, true, KeysOfSeed) } else { TTB_ACT(true, false, KeysOfSeed) }
+  } else if (t) {
+    if (dbias) { TTB_ACT(true, true, KeysOfLaunch) } else { TTB_ACT(true, false, KeysOfLaunch) }
   } else {
-    if (act == 1) go(tail_bwd_kernel<1, false>);
-    else if (act == 2) go(tail_bwd_kernel<2, false>);
-    else go(tail_bwd_kernel<0, false>);
+    if (dbias) { TTB_ACT(false, true, KeysOfLaunch) } else { TTB_ACT(false, false, KeysOfLaunch) }
   }
+#undef TTB_ACT
   if (dbias) colsum(part, dbias, out_bf16, grid, C, STREAM(stream));
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 400 + static_cast<int>(e);

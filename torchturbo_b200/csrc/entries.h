@@ -83,6 +83,7 @@ TTB_EXPORT int ttb_logprobs_slots(int, int, int, int, int*);
 TTB_EXPORT int ttb_logprobs_join(const float*, const float*, const long long*, int, long long, long long, float*, float*, float*, void*);
 TTB_EXPORT int ttb_dropout(const void*, const void*, void*, int, long long, int, unsigned, float, unsigned long long, const unsigned long long*,
                             long long, int, void*);
+TTB_EXPORT int ttb_tail_row_blocks(long long, int, int);
 TTB_EXPORT int ttb_tail_bwd(const void*, const void*, void*, float*, void*, int, long long, int, int, unsigned, float, unsigned long long,
                             const unsigned long long*, long long, int, void*);
 TTB_EXPORT int ttb_linear_rows(const ttb::GemmArgs*, void*);

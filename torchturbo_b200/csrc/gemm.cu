@@ -992,7 +992,7 @@ split_tail_kernel(const float* __restrict__ ws, int splits, int M, int N, __nv_b
     if (q.act == 1) act_pair<1>(f[j], f[j + 1]);
     else if (q.act == 2) act_pair<2>(f[j], f[j + 1]);
   }
-  if (q.drop.t) dropout8(f, dropout_draws(q.drop.first_row + r, g, dropout_key(q.drop)), q.drop.t, q.drop.scale);
+  if (q.drop.t) dropout8(f, dropout_draws(q.drop.first_row + r, g, KeysOfSeed(q.drop)), q.drop.t << 16, q.drop.scale);
   if (residual) add8(f, *reinterpret_cast<const uint4*>(residual + r * ldr + 8 * g));
   *reinterpret_cast<uint4*>(C + r * ldc + 8 * g) = pack8(f);
 }
@@ -1090,7 +1090,7 @@ static int launch(const GemmArgs& a, cudaStream_t stream) {
   if (a.tail) {
     const TailArgs& t = *a.tail;
     p.tail.bias = reinterpret_cast<const __nv_bfloat16*>(t.bias); p.tail.act = t.act;
-    p.tail.drop = DropoutParams{t.drop_t, t.drop_scale, t.seed, t.seed_dev, t.first_row};
+    p.tail.drop = dropout_params(t.drop_t, t.drop_scale, t.seed, t.seed_dev, t.first_row);
     p.tail.targets = t.targets; p.tail.vocab = t.vocab; p.tail.part = t.part; p.tail.target_logit = t.target_logit; p.tail.entropy = t.entropy;
     if (EPI == EPI_LSE) p.tile_cols = t.tile_cols;
     p.tail.lse = t.lse; p.tail.ent = t.ent; p.tail.dlogp = t.dlogp; p.tail.dent = t.dent; p.tail.first_col = t.first_col;
@@ -1249,7 +1249,7 @@ TTB_EXPORT int ttb_gemm_bf16(const ttb::GemmArgs* args, void* stream_ptr) {
   }
   if (a.epi >= EPI_TAIL) {
     if (!a.tail || a.epi > EPI_DLOGITS || a.a_mn || a.b_mn || a.tile_group || a.groups_k > 0 || a.ep || a.alpha || a.accumulate || a.c_fp32) return 911;
-    if (a.epi == EPI_TAIL && ((a.N % 8) || (reinterpret_cast<uintptr_t>(a.tail->pre) & 15) || (reinterpret_cast<uintptr_t>(a.tail->bias) & 15))) return 912;
+    if (a.epi == EPI_TAIL && ((a.N % 8) || a.tail->drop_t > 65535 || (reinterpret_cast<uintptr_t>(a.tail->pre) & 15) || (reinterpret_cast<uintptr_t>(a.tail->bias) & 15))) return 912;
     if (a.epi != EPI_TAIL && (a.split_ws || a.residual || !a.tail->targets)) return 912;
     // a product that leaves SMs without a tile of 128 columns has its tail done sooner on more of them
     const bool wide = a.N > 128 && (a.epi != EPI_TAIL || static_cast<long long>((a.M + BM - 1) / BM) * ((a.N + 127) / 128) > a.num_sms);

@@ -30,12 +30,6 @@ __device__ __forceinline__ uint4 load16_here(const void* p) {
   asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return v;
 }
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // What an epilogue thread reads of its row (one row a thread) before the accumulator is there
 template <int EPI>
 struct TailRow {
@@ -127,8 +121,10 @@ template <int BN, typename Release>
 __device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMap& tmC, TailRow<EPI_TAIL>& tr, uint8_t* stage_at, uint32_t at,
                                            int first, int row_base, int lane, uint32_t& side, Release release) {
   const TailParams& q = p.tail;
-  PhiloxKey key{0u, 0u};
-  if (q.drop.t) key = dropout_key(q.drop);
+  const KeysOfSeed key(q.drop);
+  const uint64_t place = static_cast<uint64_t>(q.drop.first_row + tr.row);
+  PhiloxRow mine{};
+  if (q.drop.t) mine = philox_row(static_cast<uint32_t>(place), key);
   bool held = true;
 #pragma unroll 1
   for (int c = 0; c < BN / 2; c += 32) {
@@ -164,7 +160,7 @@ __device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMa
     if (q.drop.t) {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        dropout8(f + 8 * i, dropout_draws(q.drop.first_row + tr.row, (col0 >> 3) + i, key), q.drop.t, q.drop.scale);
+        dropout8(f + 8 * i, philox(philox_column((col0 >> 3) + i, static_cast<uint32_t>(place >> 32), key), mine, key), q.drop.t << 16, q.drop.scale);
     }
     if (p.residual) add32(f, tr.res);
     if (!last) tr.fetch32(p, col0 + 32);

@@ -146,6 +146,7 @@ PyObject* wrap_all(const Ts&... ts) {
 // rows x last dimension
 Tensor rows2d(const Tensor& t) { return t.dim() == 2 ? t.contiguous() : t.reshape({-1, t.size(-1)}).contiguous(); }
 Tensor like_shape(const Tensor& t2, const Tensor& x) { return x.dim() == 2 ? t2 : t2.view(x.sizes()); }
+int tail_row_blocks(long long rows, long long cols, int num_sms) { return ttb_tail_row_blocks(rows, static_cast<int>(cols), num_sms); }
 int logprobs_slots(const GemmArgs& g, int* tile_cols) { return ttb_logprobs_slots(g.M, g.N, g.K, g.num_sms, tile_cols); }
 int kda_gate_row_blocks(long long rows, int heads) { return ttb_kda_gate_row_blocks(rows, heads); }
 int row_blocks(long long rows, const Tensor& t) { return static_cast<int>(std::max<long long>(1, std::min<long long>(rows, 2 * sms(t)))); }
@@ -355,7 +356,7 @@ PyObject* tail_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const long long R = dy.size(0), C = dy.size(1);
     const bool own = act != 0 || d.t != 0;
     const Tensor dz = own ? empty_rows(dy) : dy;
-    const int grid = row_blocks(R, dy);
+    const int grid = tail_row_blocks(R, C, sms(dy));
     const Tensor part = want_db ? empty({grid, C}, at::kFloat, dy) : Tensor();
     const Tensor db = !want_db ? Tensor() : R ? empty({C}, out_type(f32out), dy) : at::zeros({C}, plain(dy).dtype(out_type(f32out)));
     if (R && (own || want_db))

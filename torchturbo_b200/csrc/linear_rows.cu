@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(256) linear_rows_kernel(const RowsParams p) {
   if (p.act == 1) act_pair<1>(z, unused);
   else if (p.act == 2) act_pair<2>(z, unused);
   if (p.drop.t) {
-    const uint4 u = dropout_draws(p.drop.first_row + m, n >> 3, dropout_key(p.drop));
+    const uint4 u = dropout_draws(p.drop.first_row + m, n >> 3, KeysOfSeed(p.drop));
     const uint32_t pair = (n & 4) ? ((n & 2) ? u.w : u.z) : ((n & 2) ? u.y : u.x);
     const uint32_t draw = (n & 1) ? pair >> 16 : pair & 0xffffu;
     z = draw >= p.drop.t ? z * p.drop.scale : 0.f;
@@ -125,12 +125,12 @@ static void rows_launch(const RowsParams& p, int sms, cudaStream_t st) {
 TTB_EXPORT int ttb_linear_rows(const ttb::GemmArgs* args, void* stream) {
   using namespace ttb;
   const GemmArgs& a = *args;
-  if (a.M < 1 || a.M > 8 || (a.K % 8) || (a.N % 8) || (a.lda % 8) || (a.ldb % 8) || a.ldc != a.N || !a.tail) return 901;
+  if (a.M < 1 || a.M > 8 || (a.K % 8) || (a.N % 8) || (a.lda % 8) || (a.ldb % 8) || a.ldc != a.N || !a.tail || a.tail->drop_t > 65535) return 901;
   if ((reinterpret_cast<uintptr_t>(a.A) | reinterpret_cast<uintptr_t>(a.B)) & 15) return 902;
   const TailArgs& t = *a.tail;
   const RowsParams p{static_cast<const __nv_bfloat16*>(a.A), static_cast<const __nv_bfloat16*>(a.B), static_cast<const __nv_bfloat16*>(t.bias),
                      static_cast<const __nv_bfloat16*>(a.residual), static_cast<__nv_bfloat16*>(a.C), static_cast<__nv_bfloat16*>(t.pre),
-                     a.lda, a.ldb, a.ldr, a.N, a.K, t.act, DropoutParams{t.drop_t, t.drop_scale, t.seed, t.seed_dev, t.first_row}};
+                     a.lda, a.ldb, a.ldr, a.N, a.K, t.act, dropout_params(t.drop_t, t.drop_scale, t.seed, t.seed_dev, t.first_row)};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (a.M) {
     case 1: rows_launch<1>(p, a.num_sms, st); break;

@@ -17,7 +17,7 @@ from torch.autograd import forward_ad
 from ... import kernels as K
 from ...runtime import TurboDevice
 from ..base import OpImpl, OpImplKind
-from ..dropout import dropout_args
+from ..dropout import dropout_args, dropout_ref
 from ..moe import MoEPermutation
 from ..registry import register_op
 from . import native as N
@@ -408,10 +408,11 @@ class B200LinearBiasAct(_B200Op):
 
     def __call__(self, x, weight, bias=None, act=None, *, residual=None, dropout_p=0.0, seed=None, first_row=0):
         N.check_linear_bias_act(x, weight, bias, act, residual)
-        if not _ok(x, weight, bias, residual) or x.shape[-1] % 8 or weight.shape[0] % 8 or not weight.numel() or weight.shape[0] > 16384:
-            return N.TorchLinearBiasAct()(x, weight, bias, act, residual=residual, dropout_p=dropout_p, seed=seed, first_row=first_row)
+        drop = dropout_args(dropout_p, seed, first_row)
+        if not _ok(x, weight, bias, residual) or x.shape[-1] % 8 or weight.shape[0] % 8 or not weight.numel() or drop.t > 65535:
+            return N.linear_bias_act_ref(x, weight, bias, act, residual, drop)
         shape = x.shape[:-1] + weight.shape[:1]
-        y = LinearBiasActFn.apply(_matrix(x), weight, bias, _matrix(residual), act, dropout_args(dropout_p, seed, first_row))
+        y = LinearBiasActFn.apply(_matrix(x), weight, bias, _matrix(residual), act, drop)
         return y if y.shape == shape else y.view(shape)
 
 
@@ -437,9 +438,10 @@ class B200Dropout(_B200Op):
 
     def __call__(self, x, p, seed=None, *, residual=None, scale=1.0, first_row=0):
         N.check_dropout(x, residual)
-        if not x.is_cuda or x.dtype not in (BF16, torch.float32) or not x.numel():
-            return N.TorchDropout()(x, p, seed, residual=residual, scale=scale, first_row=first_row)
-        y = DropoutFn.apply(_matrix(x), _matrix(residual), dropout_args(p, seed, first_row, scale))
+        drop = dropout_args(p, seed, first_row, scale)
+        if not x.is_cuda or x.dtype not in (BF16, torch.float32) or not x.numel() or drop.t > 65535:
+            return dropout_ref(x, drop, residual)
+        y = DropoutFn.apply(_matrix(x), _matrix(residual), drop)
         return y if y.shape == x.shape else y.view(x.shape)
 
 
