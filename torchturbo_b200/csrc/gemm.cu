@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(EPI < EPI_TAIL ? GEMM_THREADS_PUSH : GEMM_THRE
 gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
             const GemmParams p) {
   using L = SmemLayout<BN, PAIR, EPI>;
+  constexpr bool FREE = EPI == EPI_TAIL || EPI == EPI_LSE;      // tiles of p.tile_cols columns, at most BN
   const int STAGES = EPI >= EPI_TAIL ? p.stages : L::STAGES;
   const int stage_bytes = EPI >= EPI_TAIL ? p.stage_bytes : L::STAGE_BYTES, a_bytes = EPI >= EPI_TAIL ? p.a_bytes : L::A_BYTES;
   extern __shared__ uint8_t smem_raw[];
@@ -266,7 +267,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       int k0, nkb;
       krange(x, k0, nkb);
       const int m0 = x.mt * BM;
-      const int bn = EPI == EPI_LSE ? p.tile_cols : BN;
+      const int bn = FREE ? p.tile_cols : BN;
       const int n0 = x.nt * (EPI == EPI_SWIGLU ? BN / 2 : bn);
       const int bgroup = p.tile_group ? x.a : 0;
       for (int kb = 0; kb < nkb; ++kb) {
@@ -369,7 +370,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     // ------------------------------------------------------------ MMA issuer (the whole warp, see umma_ss_w)
     if (rank == 0) {
       constexpr uint32_t whole = make_idesc_bf16(PAIR ? 2 * BM : BM, BN, A_MN, B_MN);
-      const uint32_t idesc = EPI == EPI_LSE ? make_idesc_bf16(PAIR ? 2 * BM : BM, p.tile_cols, A_MN, B_MN) : whole;
+      const uint32_t idesc = FREE ? make_idesc_bf16(PAIR ? 2 * BM : BM, p.tile_cols, A_MN, B_MN) : whole;
       const uint32_t leader = elect_one() ? 1u : 0u;
       const SmemDesc dA = make_smem_desc2(smem_u32(smem), A_MN ? 8192 : 16, 1024);
       const SmemDesc dB = make_smem_desc2(smem_u32(smem) + a_bytes, B_MN ? 8192 : 16, 1024);
@@ -442,9 +443,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       const uint32_t t_row = tmem_base + acc * BN + (static_cast<uint32_t>(lane_group * 32) << 16);
       const long long gbase = static_cast<long long>(g) * p.c_group_stride;
       TailRow<EPI> tail;      // what the tail reads of this row, asked for ahead of the wait for the products
-      if constexpr (EPI >= EPI_TAIL) tail.fetch(p, row, nt * BN + col_half * (BN / 2));
-      if constexpr (EPI == EPI_TAIL)
-        if (t + walkers < total_tiles) tail.ahead(p, next.mt * BM + lane_group * 32 + lane, next.nt * BN + col_half * (BN / 2), BN / 2);
+      // a tail's columns are dealt out 64 at a time, as they are stored: of 192 the first warps take 128
+      const int split = p.tile_cols > 128 ? 128 : 64, tail_at = col_half * split, tail_cols = col_half ? p.tile_cols - split : split;
+      if constexpr (EPI == EPI_LSE || EPI == EPI_DLOGITS) tail.fetch(p, row);
+      if constexpr (EPI == EPI_TAIL) {
+        tail.fetch(p, row, nt * p.tile_cols + tail_at, tail_cols);
+        if (t + walkers < total_tiles) tail.ahead(p, next.mt * BM + lane_group * 32 + lane, next.nt * p.tile_cols + tail_at, tail_cols);
+      }
       if constexpr (EPI == EPI_LSE) {
         const int mine = p.tile_cols / 2, first = nt * p.tile_cols + col_half * mine;      // of this warp's columns
         float sum[BN / 2];
@@ -481,10 +486,10 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
 
       if constexpr (EPI >= EPI_TAIL) {
         uint8_t* stage_at = epi_stage + (warp - 2) * L::EPI_STAGE_BYTES;
-        const uint32_t at = t_row + col_half * (BN / 2);
-        const int first = nt * BN + col_half * (BN / 2);
-        if constexpr (EPI == EPI_TAIL) tail_store<BN>(p, tmC, tail, stage_at, at, first, row_base, lane, tail_side, release);
-        else if constexpr (EPI == EPI_DLOGITS) tail_dlogits<BN>(p, tmC, tail, stage_at, at, first, row_base, lane, release);
+        if constexpr (EPI == EPI_TAIL)
+          tail_store(p, tmC, tail, stage_at, t_row + tail_at, nt * p.tile_cols + tail_at, tail_cols, row_base, lane, tail_side, release);
+        else if constexpr (EPI == EPI_DLOGITS)
+          tail_dlogits<BN>(p, tmC, tail, stage_at, t_row + col_half * (BN / 2), nt * BN + col_half * (BN / 2), row_base, lane, release);
         continue;
       }
       if (EPI == EPI_STORE && p.tma_out) {
@@ -1002,7 +1007,7 @@ split_tail_kernel(const float* __restrict__ ws, int splits, int M, int N, __nv_b
 static int tail_rows(int M) { return M < BM ? (M + 7) / 8 * 8 : BM; }
 
 template <int BN, bool A_MN, bool B_MN, int EPI, bool PAIR>
-static int launch(const GemmArgs& a, cudaStream_t stream) {
+static int launch(const GemmArgs& a, cudaStream_t stream, int tile_cols = BN) {
   using L = SmemLayout<BN, PAIR, EPI>;
   CUtensorMap tmA, tmB, tmC;
   // ---- A map (2D)
@@ -1042,7 +1047,7 @@ static int launch(const GemmArgs& a, cudaStream_t stream) {
       dims[0] = static_cast<uint64_t>(a.K);
       dims[1] = rows_b;
       box[0] = BK;
-      box[1] = EPI == EPI_LSE ? (PAIR ? a.tail->tile_cols / 2 : a.tail->tile_cols) : (EPI == EPI_SWIGLU || PAIR) ? BN / 2 : BN;
+      box[1] = EPI == EPI_SWIGLU ? BN / 2 : PAIR ? tile_cols / 2 : tile_cols;
     } else {
       // memory [K rows][N contiguous]
       dims[0] = static_cast<uint64_t>(n_mem);
@@ -1074,7 +1079,7 @@ static int launch(const GemmArgs& a, cudaStream_t stream) {
     p.ep.ret_rows = e.ret_rows;
   }
   p.M = a.M; p.N = a.N; p.K = a.K;
-  const int TN = EPI == EPI_LSE ? a.tail->tile_cols : EPI == EPI_SWIGLU ? BN / 2 : BN;
+  const int TN = EPI == EPI_SWIGLU ? BN / 2 : tile_cols;
   constexpr int TM = PAIR ? 2 * BM : BM;
   p.m_tiles = a.tile_group ? a.m_tiles_cap : (a.M + TM - 1) / TM;
   p.n_tiles = (a.N + TN - 1) / TN;
@@ -1085,14 +1090,13 @@ static int launch(const GemmArgs& a, cudaStream_t stream) {
   p.tile_group = a.tile_group; p.group_rows = a.group_rows;
   p.F = a.F; p.row_scale = a.row_scale; p.alpha = a.alpha;
   p.preact = reinterpret_cast<__nv_bfloat16*>(a.preact); p.ld_preact = a.ld_preact;
-  p.k_splits = 1; p.kb_per_split = 0; p.tile_cols = BN; p.a_bytes = tail_rows(a.M) * BK * 2;
+  p.k_splits = 1; p.kb_per_split = 0; p.tile_cols = tile_cols; p.a_bytes = tail_rows(a.M) * BK * 2;
   memset(&p.tail, 0, sizeof(p.tail));
   if (a.tail) {
     const TailArgs& t = *a.tail;
     p.tail.bias = reinterpret_cast<const __nv_bfloat16*>(t.bias); p.tail.act = t.act;
     p.tail.drop = dropout_params(t.drop_t, t.drop_scale, t.seed, t.seed_dev, t.first_row);
     p.tail.targets = t.targets; p.tail.vocab = t.vocab; p.tail.part = t.part; p.tail.target_logit = t.target_logit; p.tail.entropy = t.entropy;
-    if (EPI == EPI_LSE) p.tile_cols = t.tile_cols;
     p.tail.lse = t.lse; p.tail.ent = t.ent; p.tail.dlogp = t.dlogp; p.tail.dent = t.dent; p.tail.first_col = t.first_col;
   }
   const bool split = a.split_ws != nullptr && a.k_splits > 1;
@@ -1198,6 +1202,23 @@ static bool pays_in_pairs(const GemmArgs& a) {
   return 19 * two <= 20 * one && one * kb >= 48;
 }
 
+// Width of the column tiles of a product with a tail: the waves that tiles of 256, 192, 128 or 64 columns take, each as long as its width
+// and the handing over of a tile (about 32 columns' worth).  Narrow tiles where there is one wave or less, 192 columns where that fills
+// a wave that 256 leave partly empty (3001 x 4304 -> 1152: 60 pairs of 74 and 72).
+static int tail_tile_cols(const GemmArgs& a, bool pair) {
+  const long long walkers = pair ? a.num_sms / 2 : a.num_sms, mt = (a.M + (pair ? 2 * BM : BM) - 1) / (pair ? 2 * BM : BM);
+  int best = 256;
+  long long least = 0;
+  for (const int cols : {256, 192, 128, 64}) {
+    const long long cost = (mt * ((a.N + cols - 1) / cols) + walkers - 1) / walkers * (cols + 32);
+    if (!least || cost < least) {
+      least = cost;
+      best = cols;
+    }
+  }
+  return best;
+}
+
 // Width of the column tiles of a product whose results are not stored, which no edge of a stored box ties to 64: the waves that tiles of
 // 256 columns would take, with equal work for all of them.  One wave more or less is most where rows are few and the weight streams by
 // (61 x 2048 x 151936: 594 tiles of 256 on 148 SMs are four waves and two tiles, 731 of 208 are five of nearly the same size).
@@ -1251,24 +1272,25 @@ TTB_EXPORT int ttb_gemm_bf16(const ttb::GemmArgs* args, void* stream_ptr) {
     if (!a.tail || a.epi > EPI_DLOGITS || a.a_mn || a.b_mn || a.tile_group || a.groups_k > 0 || a.ep || a.alpha || a.accumulate || a.c_fp32) return 911;
     if (a.epi == EPI_TAIL && ((a.N % 8) || a.tail->drop_t > 65535 || (reinterpret_cast<uintptr_t>(a.tail->pre) & 15) || (reinterpret_cast<uintptr_t>(a.tail->bias) & 15))) return 912;
     if (a.epi != EPI_TAIL && (a.split_ws || a.residual || !a.tail->targets)) return 912;
-    // a product that leaves SMs without a tile of 128 columns has its tail done sooner on more of them
-    const bool wide = a.N > 128 && (a.epi != EPI_TAIL || static_cast<long long>((a.M + BM - 1) / BM) * ((a.N + 127) / 128) > a.num_sms);
-    const bool pair = wide && pays_in_pairs(a);
-    if (a.epi == EPI_TAIL && a.split_ws && a.k_splits > 1)
+    const bool split = a.epi == EPI_TAIL && a.split_ws && a.k_splits > 1;
+    // pieces of sums that leave SMs without a tile of 128 columns (9 x 4096 -> 4096 in two pieces: 20 us in tiles of 256, 16 so)
+    const bool few = split && static_cast<long long>((a.M + BM - 1) / BM) * ((a.N + 127) / 128) * a.k_splits <= a.num_sms;
+    const bool wide = a.N > 128 && !few, pair = wide && pays_in_pairs(a);
+    if (split)
       return wide ? (pair ? launch<256, false, false, EPI_STORE, true>(a, stream) : launch<256, false, false, EPI_STORE, false>(a, stream))
                   : launch<128, false, false, EPI_STORE, false>(a, stream);
-#define TTB_TAIL(E) \
-  if (a.epi == E) \
-    return wide ? (pair ? launch<256, false, false, E, true>(a, stream) : launch<256, false, false, E, false>(a, stream)) \
-                : launch<128, false, false, E, false>(a, stream);
+    if (a.epi == EPI_TAIL) {
+      const int cols = tail_tile_cols(a, pair);
+      return pair ? launch<256, false, false, EPI_TAIL, true>(a, stream, cols) : launch<256, false, false, EPI_TAIL, false>(a, stream, cols);
+    }
     if (a.epi == EPI_LSE) {
       // both sides of the call agree on the tiles by asking the same function (ttb_logprobs_slots)
       if (a.tail->tile_cols != stats_tile_cols(a, pays_in_pairs(a))) return 913;
-      return pays_in_pairs(a) ? launch<256, false, false, EPI_LSE, true>(a, stream) : launch<256, false, false, EPI_LSE, false>(a, stream);
+      return pays_in_pairs(a) ? launch<256, false, false, EPI_LSE, true>(a, stream, a.tail->tile_cols)
+                              : launch<256, false, false, EPI_LSE, false>(a, stream, a.tail->tile_cols);
     }
-    TTB_TAIL(EPI_TAIL)
-    TTB_TAIL(EPI_DLOGITS)
-#undef TTB_TAIL
+    return wide ? (pair ? launch<256, false, false, EPI_DLOGITS, true>(a, stream) : launch<256, false, false, EPI_DLOGITS, false>(a, stream))
+                : launch<128, false, false, EPI_DLOGITS, false>(a, stream);
   }
   const bool wide = (a.epi == EPI_SWIGLU) ? true : (a.N > 128);
   const bool pair = wide && pays_in_pairs(a);

@@ -33,7 +33,7 @@ __device__ __forceinline__ uint4 load16_here(const void* p) {
 // What an epilogue thread reads of its row (one row a thread) before the accumulator is there
 template <int EPI>
 struct TailRow {
-  __device__ __forceinline__ void fetch(const GemmParams&, int, int) {}
+  __device__ __forceinline__ void fetch(const GemmParams&, int) {}
 };
 template <>
 struct TailRow<EPI_TAIL> {
@@ -54,24 +54,24 @@ struct TailRow<EPI_TAIL> {
     for (int c = col; c < col + cols && c < p.N; c += 64)
       asm volatile("prefetch.global.L2 [%0];" ::"l"(p.residual + static_cast<long long>(r) * p.ldr + c));
   }
-  __device__ __forceinline__ void fetch(const GemmParams& p, int r, int col) {
+  __device__ __forceinline__ void fetch(const GemmParams& p, int r, int col, int cols) {
     row = r;
     src = p.residual && r < p.M ? p.residual + static_cast<long long>(r) * p.ldr : nullptr;
 #pragma unroll
     for (int i = 0; i < 4; ++i) res[i] = bias[i] = make_uint4(0u, 0u, 0u, 0u);
-    fetch32(p, col);
+    if (cols > 0) fetch32(p, col);
   }
 };
 template <>
 struct TailRow<EPI_LSE> {
   long long target;
-  __device__ __forceinline__ void fetch(const GemmParams& p, int r, int) { target = r < p.M ? __ldg(p.tail.targets + r) : -1; }
+  __device__ __forceinline__ void fetch(const GemmParams& p, int r) { target = r < p.M ? __ldg(p.tail.targets + r) : -1; }
 };
 template <>
 struct TailRow<EPI_DLOGITS> {
   long long target;      // column of this product, or one that it does not have
   float lse2, g, e, shift;
-  __device__ __forceinline__ void fetch(const GemmParams& p, int r, int) {
+  __device__ __forceinline__ void fetch(const GemmParams& p, int r) {
     const TailParams& q = p.tail;
     target = -1;
     lse2 = g = e = shift = 0.f;
@@ -115,11 +115,11 @@ __device__ __forceinline__ void act32(float (&f)[32]) {
   for (int i = 0; i < 32; i += 2) act_pair<ACT>(f[i], f[i + 1]);
 }
 
-// `at`: TMEM address of this warp's rows and first column, `first` that column in C; `side`: of two parking places (without
-// pre-activations they take turns, from tile to tile) the next
-template <int BN, typename Release>
+// `at`: TMEM address of this warp's rows and first column, `first` that column in C, `cols` how many it has; `side`: of two parking places
+// (without pre-activations they take turns, from tile to tile) the next
+template <typename Release>
 __device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMap& tmC, TailRow<EPI_TAIL>& tr, uint8_t* stage_at, uint32_t at,
-                                           int first, int row_base, int lane, uint32_t& side, Release release) {
+                                           int first, int cols, int row_base, int lane, uint32_t& side, Release release) {
   const TailParams& q = p.tail;
   const KeysOfSeed key(q.drop);
   const uint64_t place = static_cast<uint64_t>(q.drop.first_row + tr.row);
@@ -127,7 +127,7 @@ __device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMa
   if (q.drop.t) mine = philox_row(static_cast<uint32_t>(place), key);
   bool held = true;
 #pragma unroll 1
-  for (int c = 0; c < BN / 2; c += 32) {
+  for (int c = 0; c < cols; c += 32) {
     const int col0 = first + c;
     if (col0 >= p.N || row_base >= p.M) break;      // uniform across the warp
     float f[32];
@@ -138,7 +138,7 @@ __device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMa
 #pragma unroll
       for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
     }
-    const bool last = c + 32 >= BN / 2;
+    const bool last = c + 32 >= cols;
     if (last) {
       release();
       held = false;

@@ -32,6 +32,8 @@ def dropout_args(p: float, seed, first_row: int = 0, scale: float = 1.0) -> Drop
     """Checks a dropout's arguments.  `seed`: an integer in [0, 2^63), an int64 tensor of one value (read when the kernel runs: a captured
     step draws new masks when the tensor is moved on), or None for one drawn from torch's CPU generator (so that `torch.manual_seed`
     and the restored generator state of activation checkpointing apply)."""
+    if p == 0.0 and scale == 1.0 and first_row == 0:
+        return NONE
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability must lie in [0, 1], got {p}")
     if first_row < 0:

@@ -369,13 +369,22 @@ def _graph_of_gradients(y, inputs, needs, dys):
     return tuple(next(grads) if n else None for n in needs)
 
 
+def _differentiated(*tensors) -> bool:
+    """Whether autograd, or a transform, has to see a call.  A Function that nothing is recorded for costs 6 us of a 9 us call."""
+    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or not _eager(*(t for t in tensors if t is not None))
+
+
+def _linear_tail(x, w, bias, residual, act, drop, want_pre):
+    return K.linear_tail(_operand(x), _operand(w), _aligned(bias) if bias is not None else None, act,
+                         _operand(residual) if residual is not None else None, drop, want_pre)
+
+
 class LinearBiasActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, act, drop):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         back = need_x or need_w or need_b
-        y, z = K.linear_tail(_operand(x), _operand(w), _aligned(bias) if bias is not None else None, act,
-                             _operand(residual) if residual is not None else None, drop, back and K.ACT[act] != 0)
+        y, z = _linear_tail(x, w, bias, residual, act, drop, back and K.ACT[act] != 0)
         if back:
             # the seed is saved like an operand: moving it on before the backward is an error and not another mask
             ctx.save_for_backward(x, w, bias, z, drop.seed_tensor)
@@ -412,7 +421,10 @@ class B200LinearBiasAct(_B200Op):
         if not _ok(x, weight, bias, residual) or x.shape[-1] % 8 or weight.shape[0] % 8 or not weight.numel() or drop.t > 65535:
             return N.linear_bias_act_ref(x, weight, bias, act, residual, drop)
         shape = x.shape[:-1] + weight.shape[:1]
-        y = LinearBiasActFn.apply(_matrix(x), weight, bias, _matrix(residual), act, drop)
+        if _differentiated(x, weight, bias, residual):
+            y = LinearBiasActFn.apply(_matrix(x), weight, bias, _matrix(residual), act, drop)
+        else:
+            y = _linear_tail(_matrix(x), weight, bias, _matrix(residual), act, drop, False)[0]
         return y if y.shape == shape else y.view(shape)
 
 
@@ -441,7 +453,10 @@ class B200Dropout(_B200Op):
         drop = dropout_args(p, seed, first_row, scale)
         if not x.is_cuda or x.dtype not in (BF16, torch.float32) or not x.numel() or drop.t > 65535:
             return dropout_ref(x, drop, residual)
-        y = DropoutFn.apply(_matrix(x), _matrix(residual), drop)
+        if _differentiated(x, residual):
+            y = DropoutFn.apply(_matrix(x), _matrix(residual), drop)
+        else:
+            y = K.dropout(_aligned(_matrix(x)), _aligned(_matrix(residual)) if residual is not None else None, drop)
         return y if y.shape == x.shape else y.view(x.shape)
 
 
@@ -1007,8 +1022,12 @@ class B200LinearLogprobs(_B200Op):
         if not _ok(hidden, weight) or hidden.shape[-1] % 8:
             return N.TorchLinearLogprobs()(hidden, weight, targets, want_entropy=want_entropy)
         flat = targets if targets.dim() == 1 else targets.reshape(-1)
-        out = LinearLogprobsFn.apply(_matrix(hidden), weight, flat.long().contiguous(), want_entropy)
-        logp, ent = out if want_entropy else (out, None)
+        flat = flat.long().contiguous()
+        if _differentiated(hidden, weight):
+            out = LinearLogprobsFn.apply(_matrix(hidden), weight, flat, want_entropy)
+            logp, ent = out if want_entropy else (out, None)
+        else:
+            logp, _, ent = K.logprobs_fwd(_operand(_matrix(hidden)), _operand(weight), flat, want_entropy)
         if targets.dim() == 1:
             return logp, ent
         return logp.view(targets.shape), ent.view(targets.shape) if want_entropy else None
