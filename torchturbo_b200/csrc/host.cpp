@@ -167,7 +167,7 @@ long long k_splits(long long M, long long N, long long K, int num_sms) {
 // ---------------------------------------------------------------------------------------------
 PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    Args in(args, n, 15);
+    Args in(args, n, 16);
     const Tensor &a = in.tensor(), &b = in.tensor();
     const bool a_mn = in.flag(), b_mn = in.flag();
     Tensor out = in.optional();
@@ -177,6 +177,7 @@ PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const Tensor row_scale = in.optional(), preact = in.optional();
     const long long ep = in.integer();
     const Tensor alpha = in.optional();
+    const long long splits = in.integer();
     need(is_bf16(a) && is_bf16(b), "operands must be bf16");
     need(a.stride(-1) == 1 && b.stride(-1) == 1, "operands must be contiguous along their last dimension");
     check_device(a);
@@ -244,7 +245,7 @@ PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Tensor ws;
     int kernels = 1;
     if (K >= 4096 && !swiglu && !tile_group.defined() && !ep) {
-      const long long s = k_splits(M, N, K, g.num_sms);
+      const long long s = splits ? splits : k_splits(M, N, K, g.num_sms);
       if (s > 1) {
         ws = empty({s, M, N}, at::kFloat, a);
         g.split_ws = f32w(ws); g.k_splits = static_cast<int>(s);

@@ -163,6 +163,20 @@ def gemm_splits(M: int, N: int, K: int, sms: int) -> int:
     return max(1, min(sms // tiles, (K + 63) // 64 // 32))
 
 
+def wave_splits(M: int, N: int, K: int, sms: int) -> int:
+    """Pieces along K for a product of many k-blocks whose tiles of 256 x 256 (pairs of CTAs) leave a wave partly empty: ``s`` pieces take
+    ``ceil(tiles s / pairs) / s`` whole waves, of 0.37 us a k-block, but ``s`` fp32 results are written at 2.5 TB/s, read at 6 and their
+    sum written once more.  1501 x 4096 x 32003 (96 tiles on 74 pairs) 349 -> 306 us in three pieces; 4096 x 2048 x 50688 would go from
+    602 to 611 in four."""
+    tiles, pairs, blocks = ((M + 255) // 256) * ((N + 255) // 256), sms // 2, (K + 63) // 64
+    if M <= 128 or N <= 128 or N % 8 or 2 * tiles < pairs:
+        return gemm_splits(M, N, K, sms)
+    size = M * N * 1e-6
+    cost = {s: -(-tiles * s // pairs) / s * blocks * 0.37 + (s > 1) * (s * size * (4 / 2.5 + 4 / 6) + size * 2 / 3 + 5)
+            for s in range(1, 9) if s == 1 or blocks // s >= 32}
+    return min(cost, key=cost.get)
+
+
 def _is_f32(dtype: torch.dtype) -> bool:
     assert dtype in (torch.bfloat16, torch.float32), dtype
     return dtype == torch.float32
@@ -185,6 +199,7 @@ def gemm(
     preact: torch.Tensor | None = None,
     ep: "EpFuseArgs | None" = None,
     alpha: torch.Tensor | None = None,
+    splits: int = 0,
 ) -> torch.Tensor:
     """tcgen05 GEMM ``C = op(A) @ op(B)`` on bf16 operands with fp32 accumulation.
 
@@ -198,9 +213,10 @@ def gemm(
       * ``swiglu=True``: ``b`` holds ``[gate | up]`` output columns (``2F``); the result is
         ``silu(gate) * up * row_scale`` of width ``F``; ``preact`` (``[M, 2F]``) optionally keeps gate|up.
       * ``alpha`` (one fp32 value on the device) is multiplied into the fp32 product before it is rounded or added.
+      * ``splits`` pieces along K (from 4096 on) in place of `gemm_splits`'s.
     """
     return host().gemm(a, b, a_mn, b_mn, out, _is_f32(out_dtype), accumulate, residual, tile_group, group_rows, swiglu, row_scale, preact,
-                       C.addressof(ep) if ep is not None else 0, alpha)
+                       C.addressof(ep) if ep is not None else 0, alpha, splits)
 
 
 # --------------------------------------------------------------------------------------

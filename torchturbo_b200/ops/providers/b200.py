@@ -371,7 +371,14 @@ def _graph_of_gradients(y, inputs, needs, dys):
 
 def _differentiated(*tensors) -> bool:
     """Whether autograd, or a transform, has to see a call.  A Function that nothing is recorded for costs 6 us of a 9 us call."""
-    return (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)) or not _eager(*(t for t in tensors if t is not None))
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level >= 0 or torch.compiler.is_compiling() or torch.jit.is_tracing() or torch._C._are_functorch_transforms_active() \
+            or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        return True
+    return not all(t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors)
 
 
 def _linear_tail(x, w, bias, residual, act, drop, want_pre):
@@ -420,12 +427,11 @@ class B200LinearBiasAct(_B200Op):
         drop = dropout_args(dropout_p, seed, first_row)
         if not _ok(x, weight, bias, residual) or x.shape[-1] % 8 or weight.shape[0] % 8 or not weight.numel() or drop.t > 65535:
             return N.linear_bias_act_ref(x, weight, bias, act, residual, drop)
-        shape = x.shape[:-1] + weight.shape[:1]
         if _differentiated(x, weight, bias, residual):
             y = LinearBiasActFn.apply(_matrix(x), weight, bias, _matrix(residual), act, drop)
         else:
             y = _linear_tail(_matrix(x), weight, bias, _matrix(residual), act, drop, False)[0]
-        return y if y.shape == shape else y.view(shape)
+        return y if x.dim() == 2 else y.view(x.shape[:-1] + weight.shape[:1])
 
 
 class DropoutFn(torch.autograd.Function):
@@ -457,7 +463,7 @@ class B200Dropout(_B200Op):
             y = DropoutFn.apply(_matrix(x), _matrix(residual), drop)
         else:
             y = K.dropout(_aligned(_matrix(x)), _aligned(_matrix(residual)) if residual is not None else None, drop)
-        return y if y.shape == x.shape else y.view(x.shape)
+        return y if x.dim() == 2 else y.view(x.shape)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -994,7 +1000,7 @@ class LinearLogprobsFn(torch.autograd.Function):
         dw = torch.empty(V, H, dtype=BF16, device=h2.device) if need_w and mg is None else None
         if not T:
             return torch.zeros_like(hidden) if need_h else None, dw.zero_() if dw is not None else None, None, None
-        step = LinearLogprobsFn.pieces(T, V)
+        step, sms = LinearLogprobsFn.pieces(T, V), K.num_sms(h2.device.index)
         buf = torch.empty(T * min(step, -(-V // 8) * 8), dtype=BF16, device=h2.device)
         dh = None
         for s in range(0, V, step):
@@ -1003,10 +1009,11 @@ class LinearLogprobsFn(torch.autograd.Function):
             dl = buf[:T * (-(-n // 8) * 8)].view(T, -1)[:, :n]
             K.logprobs_dlogits(h2, piece, targets, lse, ent if dent is not None else None, *gs, s, V, dl)
             if need_h:
+                splits = K.wave_splits(T, H, n, sms)
                 if step >= V:
-                    dh = K.gemm(dl, piece, b_mn=True)
+                    dh = K.gemm(dl, piece, b_mn=True, splits=splits)
                 else:
-                    dh = K.gemm(dl, piece, b_mn=True, out=dh, out_dtype=torch.float32, accumulate=dh is not None)
+                    dh = K.gemm(dl, piece, b_mn=True, out=dh, out_dtype=torch.float32, accumulate=dh is not None, splits=splits)
             if need_w:
                 if mg is not None:
                     K.gemm(dl, h2, a_mn=True, b_mn=True, out=mg[s:s + n], accumulate=True)
