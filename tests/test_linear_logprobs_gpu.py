@@ -209,7 +209,7 @@ def test_loss_in_pieces_by_name():
     lq = torch.log_softmax(h.detach().double() @ w.detach().double().t(), -1)
     ok = t >= 0
     want = -lq[ok, t[ok]].sum()
-    assert abs(float(loss) - float(want)) <= 1e-5 * float(want)
+    assert abs(float(loss.detach()) - float(want)) <= 1e-5 * float(want)
     dh, dw = torch.autograd.grad(loss * 0.5, (h, w))
     d = torch.zeros_like(lq)
     d[ok] = lq[ok].exp()

@@ -25,6 +25,8 @@ class LoraConfig:
     r: int = 8
     lora_alpha: float = 16.0
     lora_dropout: float = 0.0
+    # masks by `ops.dropout` (drawn by place, never stored, the same in a recomputed forward) instead of `nn.Dropout`'s
+    counter_dropout: bool = False
     target_modules: list[str] | str = field(default_factory=lambda: ["all-linear"])
     use_dora: bool = False
     use_rslora: bool = False
@@ -117,6 +119,12 @@ class LoRALinear(nn.Module):
     def forward(self, x):
         if self.dropout is not None and self.training:
             n = self.cfg.adapter_name
+            if self.cfg.counter_dropout:
+                from ...ops import ops
+
+                low = ops.linear(ops.dropout(x, self.cfg.lora_dropout, scale=self.cfg.scaling), self.lora_A[n].weight)
+                base = ops.linear_bias_act(x, self.base_layer.weight, self.base_layer.bias)
+                return ops.linear_bias_act(low, self.lora_B[n].weight, residual=base)
             base = nn.functional.linear(x, self.base_layer.weight, self.base_layer.bias)
             return base + self.lora_B[n](self.lora_A[n](self.dropout(x))) * self.cfg.scaling
         return nn.functional.linear(x, self.weight, self.bias)

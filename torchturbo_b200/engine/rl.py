@@ -29,32 +29,36 @@ class RLMixin:
             mb[k] = flat.unsqueeze(0)
         return mb
 
-    def _forward_microbatch(self, model, inputs: dict[str, Any]):
+    def _forward_microbatch(self, model, inputs: dict[str, Any], **options):
         keys = ("input_ids", "position_ids", "cu_seq_lens_q", "cu_seq_lens_k", "max_length_q", "max_length_k",
                 "pixel_values", "image_grid_thw")
         model_in = {k: inputs[k] for k in keys if k in inputs}
         model_in = self.backend.prepare_inputs(model, model.on_prepare_inputs(model_in, source_inputs=inputs))
         self.backend._prepare_moe_runtime(model, model_in, 1.0)
-        return model(**model_in)
+        return model(**model_in, **options)
 
-    def _logprobs_and_entropy(self, model, mb: dict[str, Any], want_entropy: bool):
+    def _logprobs_and_entropy(self, model, mb: dict[str, Any], want_entropy: bool, fused: bool = False):
         be = self.backend
-        out = self._forward_microbatch(model, mb)
-        logits = out["logits"].reshape(-1, out["logits"].shape[-1])
+        out = self._forward_microbatch(model, mb, **({"skip_lm_head": True} if fused else {}))
         ids = mb["input_ids"].to(be.device)
         targets = shifted_packed_tensor(ids, mb["cu_seq_lens_q"], fill=-100).reshape(-1)
         T = targets.numel()
         lo, hi = (be.sp_rank * (T // be.sp_size), (be.sp_rank + 1) * (T // be.sp_size)) if be.sp_size > 1 else (0, T)
-        lp, ent = gather_logprobs_entropy(logits, targets[lo:hi], want_entropy=want_entropy)
+        if fused:
+            lp, ent = model.get_lm_head()(out["hidden_states"], targets=targets[lo:hi], want_entropy=want_entropy)
+        else:
+            logits = out["logits"].reshape(-1, out["logits"].shape[-1])
+            lp, ent = gather_logprobs_entropy(logits, targets[lo:hi], want_entropy=want_entropy)
         return lp, ent, (targets != -100)
 
     @torch.no_grad()
-    def compute_logprobs(self, model, micro_batches: Sequence[dict[str, Any]], want_entropy: bool = False):
-        """Per-token log-prob of the next token for every micro-batch, gathered over the SP group: list of [T]."""
+    def compute_logprobs(self, model, micro_batches: Sequence[dict[str, Any]], want_entropy: bool = False, *, fused: bool = False):
+        """Per-token log-prob of the next token for every micro-batch, gathered over the SP group: list of [T].  `fused`: from the output
+        head without its logits (`ops.linear_logprobs`)."""
         model.eval()
         outs = []
         for mb in micro_batches:
-            lp, ent, valid = self._logprobs_and_entropy(model, mb, want_entropy)
+            lp, ent, valid = self._logprobs_and_entropy(model, mb, want_entropy, fused)
             lp = gather_logprobs_and_shift(lp, self.backend.sp_group, self.backend.sp_size)
             if want_entropy:
                 ent = gather_logprobs_and_shift(ent, self.backend.sp_group, self.backend.sp_size)
@@ -64,10 +68,11 @@ class RLMixin:
 
     def forward_backward_batch(self, model, micro_batches: Sequence[dict[str, Any]],
                                loss_fn: Callable[[torch.Tensor, torch.Tensor | None, dict[str, Any]], torch.Tensor],
-                               *, want_entropy: bool = False, loss_weight_key: str | None = "loss_mask"):
+                               *, want_entropy: bool = False, loss_weight_key: str | None = "loss_mask", fused: bool = False):
         """Forward + backward over the micro-batches of one optimizer step.  `loss_fn(logp, entropy, mb)` returns
         per-token losses on this rank's shard; they are normalised by the total loss weight of the global batch
-        (all micro-batches, all DP ranks), so gradients do not depend on how the batch was split."""
+        (all micro-batches, all DP ranks), so gradients do not depend on how the batch was split.  `fused` as in
+        `compute_logprobs`; the logits are formed again for the gradient."""
         be = self.backend
         total_w = torch.zeros((), dtype=torch.float32, device=be.device)
         for mb in micro_batches:
@@ -80,7 +85,7 @@ class RLMixin:
         mult = self._get_loss_multiplier()
         total = torch.zeros((), dtype=torch.float32, device=be.device)
         for mb in micro_batches:
-            lp, ent, _ = self._logprobs_and_entropy(model, mb, want_entropy)
+            lp, ent, _ = self._logprobs_and_entropy(model, mb, want_entropy, fused)
             per_tok = loss_fn(lp, ent, mb)
             T = mb["input_ids"].shape[-1]
             lo, hi = (be.sp_rank * (T // be.sp_size), (be.sp_rank + 1) * (T // be.sp_size)) if be.sp_size > 1 else (0, T)

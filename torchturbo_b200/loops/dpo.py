@@ -2,7 +2,7 @@
 
 One packed row holds `2N` segments: the N chosen answers followed by the N rejected ones (each with its prompt).
 Policy and frozen reference model run the same row; per-token log-probabilities come from a full-vocabulary
-log-softmax in fp32, are summed per segment, and feed the sigmoid / IPO / hinge preference losses.  Token weights
+log-softmax in fp32 (or, with `DPOConfig.fused_logps`, from the output head without its logits), are summed per segment, and feed the sigmoid / IPO / hinge preference losses.  Token weights
 (IPO length normalisation, LD-DPO down-weighting of the tail beyond the shorter answer) are computed on the
 global row *before* it is sharded for sequence parallelism, and the per-segment statistics of all SP ranks are
 combined with a single all-reduce (adapters/msswift/trainer.py:479-668 and adapters/llamafactory_v0/trainer.py:590-797
@@ -28,6 +28,7 @@ class DPOConfig:
     label_smoothing: float = 0.0
     ld_alpha: float | None = None    # LD-DPO: weight of the tokens beyond min(len_chosen, len_rejected)
     sft_alpha: float = 0.0           # optional NLL regulariser on the chosen answers
+    fused_logps: bool = False        # log-probabilities by the head's `linear_logprobs`: no logits are kept, fp32 sums are not rounded to bf16
 
 
 def segment_token_weights(labels_shifted: torch.Tensor, cu: torch.Tensor, cfg: DPOConfig) -> torch.Tensor:
@@ -76,11 +77,15 @@ def sequence_logps(engine, model, batch: dict, cfg: DPOConfig, *, grad: bool):
         inputs["position_ids"] = torch.arange(T, device=be.device).unsqueeze(0)
     be._prepare_moe_runtime(model, inputs, 1.0)
     with torch.set_grad_enabled(grad):
-        out = model(**inputs)
-        logits = out["logits"].reshape(-1, out["logits"].shape[-1])
         tgt = shifted.reshape(-1)[lo:hi]
-        lsm = F.log_softmax(logits.float(), dim=-1)
-        tok = lsm.gather(1, tgt.clamp(min=0).unsqueeze(1)).squeeze(1)
+        if cfg.fused_logps:
+            out = model(**inputs, skip_lm_head=True)
+            tok, _ = model.get_lm_head()(out["hidden_states"], targets=tgt)
+        else:
+            out = model(**inputs)
+            logits = out["logits"].reshape(-1, out["logits"].shape[-1])
+            lsm = F.log_softmax(logits.float(), dim=-1)
+            tok = lsm.gather(1, tgt.clamp(min=0).unsqueeze(1)).squeeze(1)
         tok = torch.where(tgt != IGNORE_INDEX, tok, torch.zeros_like(tok)) * weights[lo:hi]
     offs = cu.tolist()
     sums = segment_sums(tok, offs, lo, hi)
@@ -121,7 +126,7 @@ def dpo_step(engine, policy, reference, optimizer, batch: dict, cfg: DPOConfig, 
     is `None` the batch must carry precomputed `reference_logps` ([2N])."""
     if reference is not None:
         reference.eval()
-        ref, _ = sequence_logps(engine, reference, batch, DPOConfig(cfg.beta, cfg.loss_type, ld_alpha=None), grad=False)
+        ref, _ = sequence_logps(engine, reference, batch, DPOConfig(cfg.beta, cfg.loss_type, ld_alpha=None, fused_logps=cfg.fused_logps), grad=False)
     else:
         ref = batch["reference_logps"].to(engine.backend.device)
     pol, counts = sequence_logps(engine, policy, batch, cfg, grad=True)

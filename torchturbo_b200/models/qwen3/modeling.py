@@ -61,9 +61,13 @@ class Qwen3Model(nn.Module):
 
 class LMHead(nn.Linear):
     """Output projection.  Called as a module (never through `.weight`) so that FSDP's forward hooks gather
-    the sharded weight; with `labels` it runs the fused projection + cross entropy and returns the loss sum."""
+    the sharded weight; with `labels` it runs the fused projection + cross entropy and returns the loss sum, with
+    `targets` (one token id per hidden state, -100 for none) the log-probabilities of the targets and, if wanted, the
+    entropies, without logits (`ops.linear_logprobs`)."""
 
-    def forward(self, hidden, labels=None, chunk_size: int = 1024):
+    def forward(self, hidden, labels=None, chunk_size: int = 1024, targets=None, want_entropy: bool = False):
+        if targets is not None:
+            return ops.linear_logprobs(hidden.reshape(-1, hidden.shape[-1]), self.weight, targets.reshape(-1), want_entropy=want_entropy)
         if labels is None:
             return ops.linear(hidden, self.weight)
         return ops.linear_cross_entropy(hidden.reshape(-1, hidden.shape[-1]), self.weight, labels.reshape(-1),

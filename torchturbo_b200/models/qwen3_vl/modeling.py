@@ -97,6 +97,14 @@ class _VisionMLP(nn.Module):
         self.linear_fc2 = nn.Linear(hidden, H, dtype=dtype)
 
 
+def linear_tail(fused: bool, x, lin, act=None, residual=None):
+    """A biased layer with what follows it: one product whose epilogue does it all (`ops.linear_bias_act`: what the product adds up is not
+    rounded before the bias), or a pass of its own after the product."""
+    if fused:
+        return ops.linear_bias_act(x, lin.weight, lin.bias, act, residual=residual)
+    return ops.bias_act(ops.linear(x, lin.weight), lin.bias, act, residual=residual)
+
+
 _ACTS = {"gelu_pytorch_tanh": "gelu_tanh", "gelu_tanh": "gelu_tanh", "gelu": "gelu"}
 
 
@@ -111,9 +119,11 @@ class VisionBlock(nn.Module):
         self.attn = _VisionAttention(H, dtype)
         self.mlp = _VisionMLP(H, cfg.intermediate_size, dtype)
         self.act = _ACTS[getattr(cfg, "hidden_act", "gelu_pytorch_tanh")]
+        self.fused = bool(getattr(cfg, "fused_linear_tails", False))
 
     def forward(self, x, cos, sin, cu, max_len):
-        """Biases, GELU and residual adds ride on `ops.bias_act` (one pass after each GEMM) and, with the rotary embedding, on
+        """Biases, GELU and residual adds ride on `ops.bias_act` (one pass after each GEMM; with the configuration's `fused_linear_tails`
+        in the GEMM's epilogue, `ops.linear_bias_act`) and, with the rotary embedding, on
         `ops.qkv_bias_rope`, the norms on `ops.layer_norm`; attention is full (non-causal) over each frame's patches."""
         P = x.shape[0]
         a, m = self.attn, self.mlp
@@ -121,10 +131,10 @@ class VisionBlock(nn.Module):
         q, k, v = ops.qkv_bias_rope(ops.linear(h, a.qkv.weight), a.qkv.bias, self.n_heads, cos, sin)
         o = ops.attention(q.contiguous(), k.contiguous(), v.contiguous(), cu, max_len, causal=False,
                           scale=1.0 / math.sqrt(self.head_dim))
-        x = ops.bias_act(ops.linear(o.reshape(P, -1), a.proj.weight), a.proj.bias, residual=x)
+        x = linear_tail(self.fused, o.reshape(P, -1), a.proj, residual=x)
         h = ops.layer_norm(x, self.norm2.weight, self.norm2.bias, self.norm2.eps)
-        h = ops.bias_act(ops.linear(h, m.linear_fc1.weight), m.linear_fc1.bias, self.act)
-        return ops.bias_act(ops.linear(h, m.linear_fc2.weight), m.linear_fc2.bias, residual=x)
+        h = linear_tail(self.fused, h, m.linear_fc1, self.act)
+        return linear_tail(self.fused, h, m.linear_fc2, residual=x)
 
 
 class PatchMerger(nn.Module):
@@ -138,6 +148,7 @@ class PatchMerger(nn.Module):
         self.postshuffle = postshuffle
         self.norm = nn.LayerNorm(Hm if postshuffle else cfg.hidden_size, eps=1e-6, dtype=dtype)
         self.project = not getattr(cfg, "disable_merger_proj", False)
+        self.fused = bool(getattr(cfg, "fused_linear_tails", False))
         if self.project:
             self.linear_fc1 = nn.Linear(Hm, Hm, dtype=dtype)
             self.linear_fc2 = nn.Linear(Hm, cfg.out_hidden_size, dtype=dtype)
@@ -149,8 +160,7 @@ class PatchMerger(nn.Module):
                                                                                    else self.unit * x.shape[-1])
         if not self.project:
             return x
-        h = ops.bias_act(ops.linear(x, self.linear_fc1.weight), self.linear_fc1.bias, "gelu")
-        return ops.bias_act(ops.linear(h, self.linear_fc2.weight), self.linear_fc2.bias)
+        return linear_tail(self.fused, linear_tail(self.fused, x, self.linear_fc1, "gelu"), self.linear_fc2)
 
 
 def interpolated_positions(table: torch.Tensor, grid_thw: list[list[int]], merge: int) -> torch.Tensor:
