@@ -127,5 +127,5 @@ def test_refusals():
                  lambda: ops.dropout(x, 0.1, 1, residual=x.float())):
         with pytest.raises(ValueError):
             call()
-    with pytest.raises(AssertionError, match="seed tensor"):
+    with pytest.raises(AssertionError, match="seed tensor"):      # read by the kernel, so it has to be where the rows are
         ops.dropout(x, 0.1, torch.tensor([1]))

@@ -249,6 +249,20 @@ def test_result_may_be_changed_in_place():
     assert torch.equal(got, want)
 
 
+def test_refusals():
+    from torchturbo_b200.ops import ops
+
+    bf = dict(device="cuda", dtype=torch.bfloat16)
+    x, w = torch.ones(6, 16, **bf), torch.ones(24, 16, **bf)
+    for call in (lambda: ops.linear_bias_act(x, torch.ones(24, 8, **bf)), lambda: ops.linear_bias_act(x, w[0]), lambda: ops.linear_bias_act(x, w, torch.ones(1, **bf)),
+                 lambda: ops.linear_bias_act(x, w, torch.ones(24, 1, **bf)), lambda: ops.linear_bias_act(x, w, act="relu6"),
+                 lambda: ops.linear_bias_act(x, w, residual=torch.ones(24, **bf)), lambda: ops.linear_bias_act(x, w, residual=torch.ones(1, 24, **bf)),
+                 lambda: ops.linear_bias_act(x, w, residual=torch.ones(6, 16, **bf)), lambda: ops.linear_bias_act(x.view(2, 3, 16), w, residual=torch.ones(6, 24, **bf)),
+                 lambda: ops.linear_bias_act(x, w.cpu()), lambda: ops.linear_bias_act(x, w, dropout_p=1.5), lambda: ops.linear_bias_act(x, w, dropout_p=0.1, seed=-1)):
+        with pytest.raises(ValueError):
+            call()
+
+
 def test_types_and_widths_that_the_kernel_does_not_take():
     """fp32, and widths that are no multiple of eight, take the plain formulation."""
     from torchturbo_b200.ops import ops

@@ -3,6 +3,7 @@ blocks, preference and policy-gradient steps, and a run of them together."""
 import pytest
 import torch
 
+from dist_utils import run_distributed
 from test_dpo_loop import DENSE, _pair_row
 from torchturbo_b200.engine import EngineConfig, TorchTurboEngine
 from torchturbo_b200.engine.peft.lora import LoRALinear, LoraConfig
@@ -116,8 +117,22 @@ def test_vision_block_with_fused_tails(device):
         assert (a - c).norm() <= 1.25 * (b - c).norm() + 2.0 ** -8 * c.norm()
 
 
+def _on(device, worker):
+    """CPU engines set up a process group: in a process of their own."""
+    run_distributed(worker, 1, device) if device == "cpu" else worker(0, 1, device)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_preference_step_without_logits(device):
+    _on(device, _w_preference)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_policy_gradient_batch_without_logits(device):
+    _on(device, _w_policy)
+
+
+def _w_preference(rank, world, device):
     """Segment log-probabilities with and without logits agree, their gradients too, and a step runs."""
     engine = _engine(device)
     cfg = dict(DENSE) if device == "cpu" else dict(DENSE, head_dim=128, hidden_size=256, intermediate_size=512)
@@ -141,8 +156,7 @@ def test_preference_step_without_logits(device):
     assert torch.isfinite(loss) and torch.isfinite(gnorm) and abs(float(metrics["rewards/margins"])) < 1e-3
 
 
-@pytest.mark.parametrize("device", DEVICES)
-def test_policy_gradient_batch_without_logits(device):
+def _w_policy(rank, world, device):
     engine = _engine(device)
     cfg = dict(DENSE) if device == "cpu" else dict(DENSE, head_dim=128, hidden_size=256, intermediate_size=512)
     model = engine.build_model(None, load_weights=False, init_kwargs={"config": cfg})

@@ -132,6 +132,15 @@ dropout_flat_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* 
     c = c0 + k - row * C;
     return row * G + (c >> 3);
   };
+  // the values are asked for before the draws, which take as long as they do
+  const int k0 = threadIdx.x * 8;
+  const long long at = e0 + k0;
+  const bool whole = k0 + 8 <= cnt;
+  Raw<T> xs, rs;
+  if (whole) {
+    xs.load(x + at);
+    if (residual) rs.load(residual + at);
+  }
   int c;
   const int first = c0 >> 3, last = group_of(cnt - 1, c);
   for (int id = first + threadIdx.x; id <= last; id += 256) {
@@ -140,16 +149,13 @@ dropout_flat_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* 
   }
   __syncthreads();
   const uint16_t* half = reinterpret_cast<const uint16_t*>(draws);
-  const int k0 = threadIdx.x * 8;
   if (k0 >= cnt) return;
-  const long long at = e0 + k0;
   int g = group_of(k0, c);
   int row_end = C - c;         // values left in this row
   float f[8], r[8];
-  const bool whole = k0 + 8 <= cnt;
   if (whole) {
-    load8(x + at, f);
-    if (residual) load8(residual + at, r);
+    xs.values(f);
+    if (residual) rs.values(r);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {

@@ -73,7 +73,7 @@ struct EpFuse {
 // see TailArgs (entries.h)
 struct TailParams {
   const __nv_bfloat16* bias;
-  int act, has_pre, pre_z, entropy;   // pre_z: plane of the map of C that the pre-activations are stored in, C's own is the other
+  int act, has_pre, entropy;
   DropoutParams drop;
   const long long* targets;
   long long vocab;
@@ -150,7 +150,7 @@ namespace ttb {
 template <int BN, bool A_MN, bool B_MN, int EPI, bool PAIR>
 __global__ void __launch_bounds__(EPI < EPI_TAIL ? GEMM_THREADS_PUSH : GEMM_THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
-            const GemmParams p) {
+            const __grid_constant__ CUtensorMap tmZ, const GemmParams p) {
   using L = SmemLayout<BN, PAIR, EPI>;
   constexpr bool FREE = EPI == EPI_TAIL || EPI == EPI_LSE;      // tiles of p.tile_cols columns, at most BN
   const int STAGES = EPI >= EPI_TAIL ? p.stages : L::STAGES;
@@ -487,7 +487,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       if constexpr (EPI >= EPI_TAIL) {
         uint8_t* stage_at = epi_stage + (warp - 2) * L::EPI_STAGE_BYTES;
         if constexpr (EPI == EPI_TAIL)
-          tail_store(p, tmC, tail, stage_at, t_row + tail_at, nt * p.tile_cols + tail_at, tail_cols, row_base, lane, tail_side, release);
+          tail_store(p, tmC, tmZ, tail, stage_at, t_row + tail_at, nt * p.tile_cols + tail_at, tail_cols, row_base, lane, tail_side, release);
         else if constexpr (EPI == EPI_DLOGITS)
           tail_dlogits<BN>(p, tmC, tail, stage_at, t_row + col_half * (BN / 2), nt * BN + col_half * (BN / 2), row_base, lane, release);
         continue;
@@ -1009,7 +1009,7 @@ static int tail_rows(int M) { return M < BM ? (M + 7) / 8 * 8 : BM; }
 template <int BN, bool A_MN, bool B_MN, int EPI, bool PAIR>
 static int launch(const GemmArgs& a, cudaStream_t stream, int tile_cols = BN) {
   using L = SmemLayout<BN, PAIR, EPI>;
-  CUtensorMap tmA, tmB, tmC;
+  CUtensorMap tmA, tmB, tmC, tmZ;
   // ---- A map (2D)
   {
     uint64_t dims[2];
@@ -1114,7 +1114,7 @@ static int launch(const GemmArgs& a, cudaStream_t stream, int tile_cols = BN) {
   if (total <= 0) return 0;
   if (total >= (1ll << 31) - 65536) return 910;
   // ---- C map (3D, last dim = group)
-  tmC = tmA;       // placeholder where nothing is stored through it
+  tmC = tmZ = tmA;       // placeholders where nothing is stored through them
   p.tma_out = EPI == EPI_STORE && !split && !a.c_fp32 && !a.residual && !a.accumulate && !p.ep.scat_on && a.M > 0 && a.N > 0 &&
               (a.groups_k == 0 || a.c_group_stride % 8 == 0);
   if (p.tma_out) {
@@ -1125,15 +1125,16 @@ static int launch(const GemmArgs& a, cudaStream_t stream, int tile_cols = BN) {
     if (r) return 30000 + r;
   }
   if (EPI == EPI_TAIL || EPI == EPI_DLOGITS) {
-    // C and the pre-activations, equally wide and high, are two planes of one map: their distance is its outermost stride
-    const uintptr_t c = reinterpret_cast<uintptr_t>(a.C), pre = reinterpret_cast<uintptr_t>(a.tail->pre);
-    p.tail.has_pre = a.tail->pre != nullptr;
-    p.tail.pre_z = pre > c;
-    const uint64_t dims[3] = {static_cast<uint64_t>(a.N), static_cast<uint64_t>(a.M), pre ? 2ull : 1ull};
-    const uint64_t str[2] = {static_cast<uint64_t>(a.ldc) * 2, pre ? (pre > c ? pre - c : c - pre) : static_cast<uint64_t>(a.ldc) * a.M * 2};
+    const uint64_t dims[3] = {static_cast<uint64_t>(a.N), static_cast<uint64_t>(a.M), 1};
+    const uint64_t str[2] = {static_cast<uint64_t>(a.ldc) * 2, static_cast<uint64_t>(a.ldc) * a.M * 2};
     const uint32_t box[3] = {64, 32, 1};
-    int r = make_tmap_bf16(&tmC, reinterpret_cast<const void*>(pre && pre < c ? pre : c), 3, dims, str, box);
+    int r = make_tmap_bf16(&tmC, a.C, 3, dims, str, box);
     if (r) return 30000 + r;
+    p.tail.has_pre = EPI == EPI_TAIL && a.tail->pre != nullptr;
+    if (p.tail.has_pre) {
+      r = make_tmap_bf16(&tmZ, a.tail->pre, 3, dims, str, box);
+      if (r) return 30000 + r;
+    }
   }
   constexpr int RASTER_M = PAIR ? 8 : 16;
   p.by_group = fast_div(p.m_tiles * p.n_tiles);
@@ -1158,11 +1159,11 @@ static int launch(const GemmArgs& a, cudaStream_t stream, int tile_cols = BN) {
     attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kfn, tmA, tmB, tmC, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kfn, tmA, tmB, tmC, tmZ, p);
     if (e != cudaSuccess) return 400 + static_cast<int>(e);
   } else {
     const int grid = static_cast<int>(total < a.num_sms ? total : a.num_sms);
-    kfn<<<grid, p.ep.push_on ? GEMM_THREADS_PUSH : GEMM_THREADS, L::TOTAL, stream>>>(tmA, tmB, tmC, p);
+    kfn<<<grid, p.ep.push_on ? GEMM_THREADS_PUSH : GEMM_THREADS, L::TOTAL, stream>>>(tmA, tmB, tmC, tmZ, p);
   }
   if (split && a.tail) {
     const long long n = static_cast<long long>(a.M) * (a.N / 8);

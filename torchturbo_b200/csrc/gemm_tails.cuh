@@ -118,7 +118,7 @@ __device__ __forceinline__ void act32(float (&f)[32]) {
 // `at`: TMEM address of this warp's rows and first column, `first` that column in C, `cols` how many it has; `side`: of two parking places
 // (without pre-activations they take turns, from tile to tile) the next
 template <typename Release>
-__device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMap& tmC, TailRow<EPI_TAIL>& tr, uint8_t* stage_at, uint32_t at,
+__device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMap& tmC, const CUtensorMap& tmZ, TailRow<EPI_TAIL>& tr, uint8_t* stage_at, uint32_t at,
                                            int first, int cols, int row_base, int lane, uint32_t& side, Release release) {
   const TailParams& q = p.tail;
   const KeysOfSeed key(q.drop);
@@ -170,8 +170,8 @@ __device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMa
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) {
-        if (q.has_pre) tma_store_3d(&tmC, stage_at + 4096, x, row_base, q.pre_z);
-        tma_store_3d(&tmC, stage_at + (q.has_pre ? 0u : side), x, row_base, q.has_pre ? 1 - q.pre_z : 0);
+        if (q.has_pre) tma_store_3d(&tmZ, stage_at + 4096, x, row_base, 0);
+        tma_store_3d(&tmC, stage_at + (q.has_pre ? 0u : side), x, row_base, 0);
         bulk_commit_group();
       }
       side ^= 4096u;

@@ -280,6 +280,23 @@ Dropout dropout_args(Args& in, const Tensor& like) {
        "a seed tensor is one int64 value on the device of the rows");
   return d;
 }
+// A user's mistake in an operator's arguments
+void fits(bool ok, const char* what) {
+  if (!ok) fail(PyExc_ValueError, what);
+}
+bool on_16_bytes(const Tensor& t) { return reinterpret_cast<uintptr_t>(at_(t)) % 16 == 0; }
+Tensor aligned(const Tensor& t) {
+  if (!t.defined()) return t;
+  const Tensor c = t.contiguous();
+  return on_16_bytes(c) ? c : c.clone();
+}
+// A matrix as the copy engine can read it: values of a row side by side, rows apart by at least their length and by a multiple of 16
+// bytes, from a 16-byte boundary on
+Tensor operand(const Tensor& t) {
+  if (!t.defined()) return t;
+  if (t.dim() == 2 && t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && on_16_bytes(t)) return t;
+  return aligned(t);
+}
 void need_rows(const Tensor& t, long long rows, long long cols, const Tensor& like, const char* what) {
   need(is_bf16(t) && t.dim() == 2 && t.size(0) == rows && t.size(1) == cols && t.stride(1) == 1 && t.device() == like.device(), what);
 }
@@ -305,23 +322,30 @@ bool few_rows(const GemmArgs& g) { return g.M <= 4 || (g.M <= 8 && static_cast<l
 PyObject* linear_tail(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Args in(args, n, 11);
-    const Tensor &x = in.tensor(), &w = in.tensor();
-    const Tensor bias = in.optional();
+    const Tensor &x_ = in.tensor(), &w_ = in.tensor();
+    const Tensor bias = aligned(in.optional());
     ttb::TailArgs t{};
     t.act = static_cast<int>(in.integer());
-    const Tensor residual = in.optional();
-    const Dropout d = dropout_args(in, x);
+    const Tensor residual_ = in.optional();
+    const Dropout d = dropout_args(in, x_);
     const bool want_pre = in.flag();
+    fits(x_.dim() == 2 && w_.dim() == 2 && x_.size(1) == w_.size(1), "rows do not fit the weight");
+    fits(!bias.defined() || (bias.dim() == 1 && bias.size(0) == w_.size(0)), "the bias has one value a column of the result");
+    fits(!residual_.defined() || (residual_.dim() == 2 && residual_.size(0) == x_.size(0) && residual_.size(1) == w_.size(0)),
+         "the residual must have the shape of the result");
+    for (const Tensor& o : {w_, bias, residual_}) fits(!o.defined() || o.device() == x_.device(), "operands live on different devices");
+    const Tensor x = operand(x_), w = operand(w_), residual = operand(residual_);
     GemmArgs g = product(x, w);
     const long long M = g.M, N = g.N;
+    need(N % 8 == 0 && g.K % 8 == 0 && g.K > 0, "widths are multiples of eight");
     const Tensor y = empty({M, N}, at::kBFloat16, x), pre = want_pre ? empty({M, N}, at::kBFloat16, x) : Tensor();
     if (M == 0 || N == 0) return wrap_all(y, pre);
     if (bias.defined()) {
-      need(is_bf16(bias) && bias.numel() == N && bias.is_contiguous() && bias.device() == x.device(), "the bias is one bf16 value a column");
+      need(is_bf16(bias), "the bias is bf16");
       t.bias = bias.const_data_ptr();
     }
     if (residual.defined()) {
-      need_rows(residual, M, N, x, "the residual is bf16 and has the shape of the result");
+      need(is_bf16(residual), "the residual is bf16");
       g.residual = residual.const_data_ptr(); g.ldr = residual.stride(0);
     }
     t.pre = to_(pre);
@@ -343,43 +367,86 @@ PyObject* linear_tail(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
+// (dz, db): dz = dropout(dy) act'(z), its column sums
+void tail_gradient(const Tensor& dy, const Tensor& z, int act, const Dropout& d, bool want_db, bool f32out, Tensor& dz, Tensor& db) {
+  check_device(dy);
+  need(dy.dim() == 2 && is_bf16(dy) && dy.is_contiguous() && on_16_bytes(dy), "gradients: bf16 rows without gaps");
+  need(!z.defined() || (is_bf16(z) && z.is_contiguous() && z.sizes() == dy.sizes() && z.device() == dy.device()), "pre-activations: bf16 rows without gaps");
+  const long long R = dy.size(0), C = dy.size(1);
+  const bool own = act != 0 || d.t != 0;
+  dz = own ? empty_rows(dy) : dy;
+  const int grid = tail_row_blocks(R, C, sms(dy));
+  const Tensor part = want_db ? empty({grid, C}, at::kFloat, dy) : Tensor();
+  db = !want_db ? Tensor() : R ? empty({C}, out_type(f32out), dy) : at::zeros({C}, plain(dy).dtype(out_type(f32out)));
+  if (R && (own || want_db))
+    launch("ttb_tail_bwd", want_db ? 2 : 1, [&](void* st) {
+      return ttb_tail_bwd(at_(dy), at_(z), own ? to_(dz) : nullptr, f32w(part), to_(db), !f32out, R, static_cast<int>(C), act, d.t, d.scale, d.seed,
+                          d.dev(), d.first_row, grid, st);
+    });
+}
+
 PyObject* tail_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Args in(args, n, 10);
-    const Tensor& dy = in.tensor();
-    const Tensor z = in.optional();
+    const Tensor dy = aligned(in.tensor()), z = in.optional();
     const int act = static_cast<int>(in.integer());
     const Dropout d = dropout_args(in, dy);
     const bool want_db = in.flag(), f32out = in.flag();
-    check_device(dy);
-    need(dy.dim() == 2 && is_bf16(dy) && dy.is_contiguous(), "gradients: bf16 rows without gaps");
-    need(!z.defined() || (is_bf16(z) && z.is_contiguous() && z.sizes() == dy.sizes() && z.device() == dy.device()), "pre-activations: bf16 rows without gaps");
-    const long long R = dy.size(0), C = dy.size(1);
-    const bool own = act != 0 || d.t != 0;
-    const Tensor dz = own ? empty_rows(dy) : dy;
-    const int grid = tail_row_blocks(R, C, sms(dy));
-    const Tensor part = want_db ? empty({grid, C}, at::kFloat, dy) : Tensor();
-    const Tensor db = !want_db ? Tensor() : R ? empty({C}, out_type(f32out), dy) : at::zeros({C}, plain(dy).dtype(out_type(f32out)));
-    if (R && (own || want_db))
-      launch("ttb_tail_bwd", want_db ? 2 : 1, [&](void* st) {
-        return ttb_tail_bwd(at_(dy), at_(z), own ? to_(dz) : nullptr, f32w(part), to_(db), !f32out, R, static_cast<int>(C), act, d.t, d.scale, d.seed,
-                            d.dev(), d.first_row, grid, st);
-      });
+    Tensor dz, db;
+    tail_gradient(dy, z, act, d, want_db, f32out, dz, db);
     return wrap_all(dz, db);
+  });
+}
+
+// plain bf16 product of MN-major operands as the backward of a linear layer has them
+Tensor backward_product(const Tensor& a, const Tensor& b, bool a_mn) {
+  GemmArgs g{};
+  const long long M = a.size(a_mn ? 1 : 0), K = a.size(a_mn ? 0 : 1), N = b.size(1);
+  const Tensor out = K ? empty({M, N}, at::kBFloat16, a) : at::zeros({M, N}, plain(a));
+  if (M == 0 || N == 0 || K == 0) return out;
+  g.A = a.const_data_ptr(); g.lda = a.stride(0);
+  g.B = b.const_data_ptr(); g.ldb = b.stride(0); g.b_groups = 1;
+  g.C = out.data_ptr(); g.ldc = N;
+  g.M = static_cast<int>(M); g.N = static_cast<int>(N); g.K = static_cast<int>(K);
+  g.a_mn = a_mn; g.b_mn = 1;
+  g.num_sms = sms(a);
+  Tensor ws;
+  const long long s = K >= 4096 ? k_splits(M, N, K, g.num_sms) : 1;
+  if (s > 1) {
+    ws = empty({s, M, N}, at::kFloat, a);
+    g.split_ws = f32w(ws); g.k_splits = static_cast<int>(s);
+  }
+  launch("ttb_gemm_bf16", s > 1 ? 2 : 1, [&](void* st) { return ttb_gemm_bf16(&g, st); });
+  return out;
+}
+
+// (dx, dw, db) of linear_tail, in one call: the three are four launches
+PyObject* linear_tail_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args in(args, n, 14);
+    const Tensor dy = aligned(in.tensor()), x = operand(in.optional()), w = operand(in.optional()), z = in.optional();
+    const int act = static_cast<int>(in.integer());
+    const Dropout d = dropout_args(in, dy);
+    const bool need_x = in.flag(), need_w = in.flag(), want_db = in.flag(), f32out = in.flag();
+    need((!need_x || (w.defined() && is_bf16(w) && w.dim() == 2 && w.size(0) == dy.size(1) && w.device() == dy.device())) &&
+             (!need_w || (x.defined() && is_bf16(x) && x.dim() == 2 && x.size(0) == dy.size(0) && x.device() == dy.device())),
+         "operands of the backward: bf16 matrices that fit the gradient");
+    Tensor dz, db;
+    tail_gradient(dy, z, act, d, want_db, f32out, dz, db);
+    const Tensor dx = need_x ? backward_product(dz, w, false) : Tensor(), dw = need_w ? backward_product(dz, x, true) : Tensor();
+    return wrap_all(dx, dw, db);
   });
 }
 
 PyObject* dropout(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Args in(args, n, 7);
-    const Tensor& x = in.tensor();
-    const Tensor residual = in.optional();
+    const Tensor x = aligned(in.tensor()), residual = aligned(in.optional());
     const Dropout d = dropout_args(in, x);
     check_device(x);
-    auto fits = [&](const Tensor& t) { return t.is_contiguous() && reinterpret_cast<uintptr_t>(at_(t)) % 16 == 0; };
-    need(x.dim() == 2 && (is_bf16(x) || x.scalar_type() == at::kFloat) && fits(x), "bf16 or fp32 rows without gaps on a 16-byte boundary");
-    need(!residual.defined() || (residual.scalar_type() == x.scalar_type() && residual.sizes() == x.sizes() && fits(residual) && residual.device() == x.device()),
-         "the residual has the type, shape and layout of the rows");
+    need(x.dim() == 2 && (is_bf16(x) || x.scalar_type() == at::kFloat), "bf16 or fp32 rows");
+    need(!residual.defined() || (residual.scalar_type() == x.scalar_type() && residual.sizes() == x.sizes() && residual.device() == x.device()),
+         "the residual has the type and shape of the rows");
     need(x.size(1) < (1ll << 31) - 8, "rows of fewer than 2^31 values");
     const Tensor y = empty_rows(x);
     if (x.numel())
@@ -395,7 +462,8 @@ PyObject* dropout(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* logprobs_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Args in(args, n, 4);
-    const Tensor &h = in.tensor(), &w = in.tensor(), &targets = in.tensor();
+    const Tensor h = operand(in.tensor()), w = operand(in.tensor());
+    const Tensor& targets = in.tensor();
     const bool want_ent = in.flag();
     GemmArgs g = product(h, w);
     const long long M = g.M;
@@ -1022,7 +1090,7 @@ PyObject* setup(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* launches(PyObject*, PyObject* const*, Py_ssize_t) { return PyLong_FromLongLong(g_launches.load(std::memory_order_relaxed)); }
 
 #define ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {ENTRY(setup), ENTRY(launches), ENTRY(gemm), ENTRY(linear_tail), ENTRY(tail_bwd), ENTRY(dropout), ENTRY(logprobs_fwd),
+PyMethodDef methods[] = {ENTRY(setup), ENTRY(launches), ENTRY(gemm), ENTRY(linear_tail), ENTRY(tail_bwd), ENTRY(linear_tail_bwd), ENTRY(dropout), ENTRY(logprobs_fwd),
                          ENTRY(logprobs_dlogits), ENTRY(rmsnorm_fwd), ENTRY(rmsnorm_bwd), ENTRY(layernorm_fwd), ENTRY(layernorm_bwd),
                          ENTRY(bias_act_fwd), ENTRY(bias_act_bwd), ENTRY(qknorm_rope_fwd), ENTRY(qknorm_rope_bwd), ENTRY(qkv_rope_fwd), ENTRY(qkv_rope_bwd), ENTRY(gdn_gate_fwd),
                          ENTRY(gdn_gate_bwd), ENTRY(scale), ENTRY(copy_words), ENTRY(kda_gate_fwd), ENTRY(kda_gate_bwd), ENTRY(delta_prep), ENTRY(delta_out), ENTRY(delta_bwd_pre),

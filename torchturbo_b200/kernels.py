@@ -228,6 +228,12 @@ def linear_tail(x, weight, bias, act, residual, drop, want_pre):
     return host().linear_tail(x, weight, bias, ACT[act], residual, drop.t, drop.scale, drop.seed, drop.seed_tensor, drop.first_row, want_pre)
 
 
+def linear_tail_bwd(dy, x, weight, z, act, drop, want_dx, want_dw, want_db, db_dtype=torch.bfloat16):
+    """(dx, dw, db) of `linear_tail`, each None unless wanted."""
+    return host().linear_tail_bwd(dy, x, weight, z, ACT[act], drop.t, drop.scale, drop.seed, drop.seed_tensor, drop.first_row, want_dx, want_dw,
+                                  want_db, _is_f32(db_dtype))
+
+
 def tail_bwd(dy, z, act, drop, want_db, db_dtype=torch.float32):
     """(dz, db) of `linear_tail`: ``dz = dropout(dy) * act'(z)`` (``dy`` itself where nothing is applied), ``db`` its column sums or None."""
     return host().tail_bwd(dy, z, ACT[act], drop.t, drop.scale, drop.seed, drop.seed_tensor, drop.first_row, want_db, _is_f32(db_dtype))

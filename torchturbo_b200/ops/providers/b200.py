@@ -381,17 +381,12 @@ def _differentiated(*tensors) -> bool:
     return not all(t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors)
 
 
-def _linear_tail(x, w, bias, residual, act, drop, want_pre):
-    return K.linear_tail(_operand(x), _operand(w), _aligned(bias) if bias is not None else None, act,
-                         _operand(residual) if residual is not None else None, drop, want_pre)
-
-
 class LinearBiasActFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, act, drop):
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         back = need_x or need_w or need_b
-        y, z = _linear_tail(x, w, bias, residual, act, drop, back and K.ACT[act] != 0)
+        y, z = K.linear_tail(x, w, bias, act, residual, drop, back and K.ACT[act] != 0)
         if back:
             # the seed is saved like an operand: moving it on before the backward is an error and not another mask
             ctx.save_for_backward(x, w, bias, z, drop.seed_tensor)
@@ -409,11 +404,13 @@ class LinearBiasActFn(torch.autograd.Function):
                 y = N.linear_bias_act_ref(x, w, bias, ctx.act, None, drop)
                 dx, dw, db = _graph_of_gradients(y, (x, w, bias), (need_x, need_w, need_b), dy)
             else:
-                dz, db = K.tail_bwd(_aligned(dy), z, ctx.act, drop, need_b, bias.dtype if need_b else BF16)
-                if need_x:
-                    dx = K.gemm(dz, _operand(w), b_mn=True)
-                if need_w:
-                    dw = _weight_grad(w, dz, _operand(x))
+                db_dtype = bias.dtype if need_b else BF16
+                if need_w and getattr(w, "main_grad", None) is not None:
+                    dz, db = K.tail_bwd(dy, z, ctx.act, drop, need_b, db_dtype)
+                    dx = K.gemm(dz, _operand(w), b_mn=True) if need_x else None
+                    _weight_grad(w, dz, _operand(x))
+                else:
+                    dx, dw, db = K.linear_tail_bwd(dy, x, w, z, ctx.act, drop, need_x, need_w, need_b, db_dtype)
         return dx, dw, db, dy if need_r else None, None, None
 
 
@@ -423,14 +420,17 @@ class B200LinearBiasAct(_B200Op):
     backward is one pass over them and the incoming gradient, and the two products."""
 
     def __call__(self, x, weight, bias=None, act=None, *, residual=None, dropout_p=0.0, seed=None, first_row=0):
-        N.check_linear_bias_act(x, weight, bias, act, residual)
         drop = dropout_args(dropout_p, seed, first_row)
-        if not _ok(x, weight, bias, residual) or x.shape[-1] % 8 or weight.shape[0] % 8 or not weight.numel() or drop.t > 65535:
+        if not _ok(x, weight, bias, residual) or act not in K.ACT or weight.dim() != 2 or weight.shape[0] % 8 or weight.shape[1] % 8 or not weight.numel() \
+                or drop.t > 65535:
+            N.check_linear_bias_act(x, weight, bias, act, residual)
             return N.linear_bias_act_ref(x, weight, bias, act, residual, drop)
+        if residual is not None and residual.shape[:-1] != x.shape[:-1]:          # the rest of the shapes is checked where they are read
+            N.check_linear_bias_act(x, weight, bias, act, residual)
         if _differentiated(x, weight, bias, residual):
             y = LinearBiasActFn.apply(_matrix(x), weight, bias, _matrix(residual), act, drop)
         else:
-            y = _linear_tail(_matrix(x), weight, bias, _matrix(residual), act, drop, False)[0]
+            y = K.linear_tail(_matrix(x), weight, bias, act, _matrix(residual), drop, False)[0]
         return y if x.dim() == 2 else y.view(x.shape[:-1] + weight.shape[:1])
 
 
@@ -439,14 +439,14 @@ class DropoutFn(torch.autograd.Function):
     def forward(ctx, x, residual, drop):
         ctx.save_for_backward(drop.seed_tensor)
         ctx.drop = drop
-        return K.dropout(_aligned(x), _aligned(residual) if residual is not None else None, drop)
+        return K.dropout(x, residual, drop)
 
     @staticmethod
     def backward(ctx, dy):
         drop = _with_seed(ctx.drop, *ctx.saved_tensors)
         dx = None
         if ctx.needs_input_grad[0]:
-            dx = DropoutFn.apply(dy, None, drop) if torch.is_grad_enabled() else K.dropout(_aligned(dy), None, drop)
+            dx = DropoutFn.apply(dy, None, drop) if torch.is_grad_enabled() else K.dropout(dy, None, drop)
         return dx, dy if ctx.needs_input_grad[1] else None, None
 
 
@@ -462,7 +462,7 @@ class B200Dropout(_B200Op):
         if _differentiated(x, residual):
             y = DropoutFn.apply(_matrix(x), _matrix(residual), drop)
         else:
-            y = K.dropout(_aligned(_matrix(x)), _aligned(_matrix(residual)) if residual is not None else None, drop)
+            y = K.dropout(_matrix(x), _matrix(residual), drop)
         return y if x.dim() == 2 else y.view(x.shape)
 
 
@@ -978,7 +978,7 @@ class LinearLogprobsFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, hidden, weight, targets, want_entropy):
-        logp, lse, ent = K.logprobs_fwd(_operand(hidden), _operand(weight), targets, want_entropy)
+        logp, lse, ent = K.logprobs_fwd(hidden, weight, targets, want_entropy)
         ctx.save_for_backward(hidden, weight, targets, lse, ent)
         ctx.set_materialize_grads(False)
         return (logp, ent) if want_entropy else logp
@@ -1034,7 +1034,7 @@ class B200LinearLogprobs(_B200Op):
             out = LinearLogprobsFn.apply(_matrix(hidden), weight, flat, want_entropy)
             logp, ent = out if want_entropy else (out, None)
         else:
-            logp, _, ent = K.logprobs_fwd(_operand(_matrix(hidden)), _operand(weight), flat, want_entropy)
+            logp, _, ent = K.logprobs_fwd(_matrix(hidden), weight, flat, want_entropy)
         if targets.dim() == 1:
             return logp, ent
         return logp.view(targets.shape), ent.view(targets.shape) if want_entropy else None
