@@ -148,7 +148,6 @@ dropout_flat_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* 
     draws[id - first] = dropout_draws(d.first_row + r0 + row, id - row * G, key);
   }
   __syncthreads();
-  const uint16_t* half = reinterpret_cast<const uint16_t*>(draws);
   if (k0 >= cnt) return;
   int g = group_of(k0, c);
   int row_end = C - c;         // values left in this row
@@ -164,19 +163,35 @@ dropout_flat_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* 
       r[j] = in && residual ? as_float(residual[at + j]) : 0.f;
     }
   }
+  const int h0 = (g - first) * 8 + (c & 7);      // place of the first value's draw
+  if (row_end >= 8) {
+    // of one row: eight halves side by side, from an even one on or an odd one
+    const uint32_t* word = reinterpret_cast<const uint32_t*>(draws) + (h0 >> 1);
+    uint32_t w[5];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t u = half[(g - first) * 8 + (c & 7)];
-    f[j] = u >= d.t ? f[j] * d.scale : 0.f;
-    if (residual) f[j] += r[j];
-    if (k0 + j + 1 < cnt) {
-      ++c;
-      if (--row_end == 0) {
-        ++g; c = 0; row_end = C;
-      } else if ((c & 7) == 0) {
-        ++g;
+    for (int j = 0; j < 4; ++j) w[j] = word[j];
+    w[4] = (h0 & 1) ? word[4] : 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = (h0 & 1) ? __funnelshift_r(w[j], w[j + 1], 16) : w[j];
+    dropout8(f, make_uint4(w[0], w[1], w[2], w[3]), d.t << 16, d.scale);
+  } else {
+    const uint16_t* half = reinterpret_cast<const uint16_t*>(draws);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      f[j] = half[(g - first) * 8 + (c & 7)] >= d.t ? f[j] * d.scale : 0.f;
+      if (k0 + j + 1 < cnt) {
+        ++c;
+        if (--row_end == 0) {
+          ++g; c = 0; row_end = C;
+        } else if ((c & 7) == 0) {
+          ++g;
+        }
       }
     }
+  }
+  if (residual) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] += r[j];
   }
   if (whole) {
     store8(y + at, f);

@@ -30,6 +30,7 @@ struct TailArgs {
   // 4: C = gradient of the logits of columns first_col .. first_col + N - 1
   const float *lse, *ent, *dlogp, *dent;   // [M]; `ent` and `dent` may be null
   long long first_col;
+  int rest;                            // C has M more rows behind, for what the rounding to bf16 left out
 };
 
 struct GemmArgs {

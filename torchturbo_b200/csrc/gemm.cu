@@ -1125,13 +1125,14 @@ static int launch(const GemmArgs& a, cudaStream_t stream, int tile_cols = BN) {
     if (r) return 30000 + r;
   }
   if (EPI == EPI_TAIL || EPI == EPI_DLOGITS) {
-    const uint64_t dims[3] = {static_cast<uint64_t>(a.N), static_cast<uint64_t>(a.M), 1};
+    const bool rest = EPI == EPI_DLOGITS && a.tail->rest;
+    const uint64_t dims[3] = {static_cast<uint64_t>(a.N), static_cast<uint64_t>(a.M), rest ? 2ull : 1ull};
     const uint64_t str[2] = {static_cast<uint64_t>(a.ldc) * 2, static_cast<uint64_t>(a.ldc) * a.M * 2};
     const uint32_t box[3] = {64, 32, 1};
     int r = make_tmap_bf16(&tmC, a.C, 3, dims, str, box);
     if (r) return 30000 + r;
-    p.tail.has_pre = EPI == EPI_TAIL && a.tail->pre != nullptr;
-    if (p.tail.has_pre) {
+    p.tail.has_pre = rest || (EPI == EPI_TAIL && a.tail->pre != nullptr);
+    if (EPI == EPI_TAIL && p.tail.has_pre) {
       r = make_tmap_bf16(&tmZ, a.tail->pre, 3, dims, str, box);
       if (r) return 30000 + r;
     }

@@ -7,7 +7,9 @@
 //                 log2(e) as rounded to fp32, d = l log2(e) - m is one fma, 2^d one instruction, and log2 sum 2^(l log2 e) = m + log2 s is
 //                 exact in m whatever its rounding was.
 //   tail_dlogits  gradient of the logits, formed again from the same operands:  p = 2^(l log2 e - lse log2 e),
-//                 dl = g (1[target] - p) - e p (l - lse + H), one rounding to bf16 (the type in which the two products behind it take it).
+//                 dl = g (1[target] - p) - e p (l - lse + H), rounded to bf16, the type in which the two products behind it take it.  Of few
+//                 rows one value, the target's, is most of a row, and its rounding would not average out: what it left out goes to a
+//                 second plane, as further rows of those products.
 #pragma once
 
 namespace ttb {
@@ -264,34 +266,42 @@ __device__ __forceinline__ void tail_dlogits(const GemmParams& p, const CUtensor
       release();
       held = false;
     }
-    const long long hit = tr.target - col0;
-    const bool here = hit >= 0 && hit < 64;
-    if (lane == 0) bulk_wait_read_all();
-    __syncwarp();
-    if (silent) {
+    const int hit = tr.target >= col0 && tr.target < col0 + 64 ? static_cast<int>(tr.target - col0) : -1;
+    // (the rounded value, and with `rest` what its rounding left out)
+    auto park = [&](bool rest) {
+      if (lane == 0) bulk_wait_read_all();
+      __syncwarp();
+      if (silent) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) st_shared_v4(epi_piece_addr(sy, lane, i), 0u, 0u, 0u, 0u);
-    } else {
+        for (int i = 0; i < 8; ++i) st_shared_v4(epi_piece_addr(sy, lane, i), 0u, 0u, 0u, 0u);
+      } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float f[8];
+        for (int i = 0; i < 8; ++i) {
+          float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float d = fmaf(__uint_as_float(v[i >> 2][(8 * i + j) & 31]), LOG2E, -tr.lse2);
-          const float pr = exp2_approx(d);
-          f[j] = -pr * (p.tail.dent ? fmaf(tr.e, fmaf(d, ln2, tr.shift), tr.g) : tr.g);
-          if (here && hit == 8 * i + j) f[j] += tr.g;
+          for (int j = 0; j < 8; ++j) {
+            const float d = fmaf(__uint_as_float(v[i >> 2][(8 * i + j) & 31]), LOG2E, -tr.lse2);
+            const float pr = exp2_approx(d);
+            f[j] = -pr * (p.tail.dent ? fmaf(tr.e, fmaf(d, ln2, tr.shift), tr.g) : tr.g);
+            if (hit == 8 * i + j) f[j] += tr.g;
+          }
+          if (rest) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] -= __bfloat162float(__float2bfloat16(f[j]));
+          }
+          const uint4 y = pack8(f);
+          st_shared_v4(epi_piece_addr(sy, lane, i), y.x, y.y, y.z, y.w);
         }
-        const uint4 y = pack8(f);
-        st_shared_v4(epi_piece_addr(sy, lane, i), y.x, y.y, y.z, y.w);
       }
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) {
-      tma_store_3d(&tmC, stage_at, col0, row_base, 0);
-      bulk_commit_group();
-    }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        tma_store_3d(&tmC, stage_at, col0, row_base, rest ? 1 : 0);
+        bulk_commit_group();
+      }
+    };
+    park(false);
+    if (p.tail.has_pre) park(true);
   }
   if (held) release();
 }

@@ -501,7 +501,9 @@ PyObject* logprobs_dlogits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     for (const Tensor& r : {lse, ent, dlogp, dent})
       need(!r.defined() || (r.scalar_type() == at::kFloat && r.is_contiguous() && r.numel() == g.M && r.device() == h.device()), "statistics and gradients: one fp32 value a row");
     need(!dent.defined() || ent.defined(), "the entropy's gradient needs the entropy");
-    need_rows(out, g.M, g.N, h, "the gradient is bf16, a row for each of the hidden states");
+    t.rest = out.dim() == 2 && out.size(0) == 2ll * g.M;
+    need_rows(out, t.rest ? 2ll * g.M : g.M, g.N, h, "the gradient is bf16, a row or two for each of the hidden states");
+    need(out.stride(0) % 8 == 0 && on_16_bytes(out), "rows of the gradient start on 16-byte boundaries");
     if (g.M == 0 || g.N == 0) return wrap(out);
     t.targets = static_cast<const long long*>(at_(targets));
     t.lse = f32(lse); t.ent = f32(ent); t.dlogp = f32(dlogp); t.dent = f32(dent);

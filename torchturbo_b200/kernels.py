@@ -251,7 +251,8 @@ def logprobs_fwd(hidden, weight, targets, want_entropy: bool):
 
 
 def logprobs_dlogits(hidden, weight, targets, lse, entropy, dlogp, dent, first_col: int, vocab: int, out):
-    """Gradient of the logits of the columns that ``weight`` (rows ``first_col ..`` of the head's) covers, bf16, into ``out``."""
+    """Gradient of the logits of the columns that ``weight`` (rows ``first_col ..`` of the head's) covers, bf16, into ``out``; an
+    ``out`` of twice the rows takes what the rounding left out behind them."""
     return host().logprobs_dlogits(hidden, weight, targets, lse, entropy, dlogp, dent, first_col, vocab, out)
 
 
