@@ -84,6 +84,19 @@ def test_larger(T, H, V):
     _check(*_case(T, H, V), True, True)
 
 
+def test_rows_in_shares():
+    """Statistics of more rows than are held at a time (2^26 values of 1188 pieces and three planes: 18688 rows)."""
+    from torchturbo_b200.ops import ops
+
+    h, w, t = _case(19001, 8, 151936)
+    logp, ent = ops.linear_logprobs(h, w, t, want_entropy=True)
+    for a in (0, 18600, 18900):
+        parts = ops.linear_logprobs(h[a:a + 101], w, t[a:a + 101], want_entropy=True)
+        for x, y in zip((logp, ent), parts):
+            assert ((x[a:a + 101] - y).abs() <= 2.0 ** -18 * (1 + y.abs())).all()      # other tiles, other order of the same sums
+    _check(h[-64:].clone(), w, t[-64:].clone(), True, False)
+
+
 @pytest.mark.parametrize("V", [700, 1025])
 @pytest.mark.parametrize("want_entropy", [False, True])
 def test_several_pieces(monkeypatch, V, want_entropy):

@@ -472,16 +472,27 @@ PyObject* logprobs_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     need(g.N > 0 && g.K > 0, "a vocabulary and hidden states of at least one value");
     const Tensor logp = empty({M}, at::kFloat, h), lse = empty({M}, at::kFloat, h), ent = want_ent ? empty({M}, at::kFloat, h) : Tensor();
     if (M == 0) return wrap_all(logp, lse, ent);
+    const Tensor hit = empty({M}, at::kFloat, h);
     ttb::TailArgs t{};
-    const int slots = logprobs_slots(g, &t.tile_cols);
-    const Tensor part = empty({want_ent ? 3 : 2, slots, M}, at::kFloat, h), hit = empty({M}, at::kFloat, h);
-    t.targets = static_cast<const long long*>(at_(targets)); t.vocab = g.N;
-    t.part = f32w(part); t.target_logit = f32w(hit); t.entropy = want_ent;
+    t.vocab = g.N; t.entropy = want_ent;
     g.epi = 3; g.tail = &t;
-    launch("ttb_gemm_bf16", 1, [&](void* st) { return ttb_gemm_bf16(&g, st); });
-    launch("ttb_logprobs_join", 1, [&](void* st) {
-      return ttb_logprobs_join(f32(part), f32(hit), t.targets, slots, M, g.N, f32w(logp), f32w(lse), f32w(ent), st);
-    });
+    // The statistics of all pieces are 8 or 12 bytes for every 128 logits; rows are taken in shares that keep them below 256 MB
+    const int planes = want_ent ? 3 : 2;
+    const long long share = std::max<long long>(256, (1ll << 26) / (planes * (2ll * ((g.N + 255) / 256) + 2)) / 256 * 256);
+    Tensor part;
+    for (long long r = 0; r < M; r += share) {
+      const long long rows = std::min(share, M - r);
+      g.A = static_cast<const char*>(h.const_data_ptr()) + r * g.lda * 2;
+      g.M = static_cast<int>(rows);
+      const int slots = logprobs_slots(g, &t.tile_cols);
+      if (!part.defined() || part.numel() < planes * slots * rows) part = empty({planes * slots * rows}, at::kFloat, h);
+      t.targets = static_cast<const long long*>(at_(targets)) + r;
+      t.part = f32w(part); t.target_logit = f32w(hit) + r;
+      launch("ttb_gemm_bf16", 1, [&](void* st) { return ttb_gemm_bf16(&g, st); });
+      launch("ttb_logprobs_join", 1, [&](void* st) {
+        return ttb_logprobs_join(f32(part), t.target_logit, t.targets, slots, rows, g.N, f32w(logp) + r, f32w(lse) + r, ent.defined() ? f32w(ent) + r : nullptr, st);
+      });
+    }
     return wrap_all(logp, lse, ent);
   });
 }

@@ -44,6 +44,8 @@ class LoraConfig:
         d = asdict(self)
         if isinstance(d["target_modules"], (set, tuple)):
             d["target_modules"] = sorted(d["target_modules"])
+        if not self.counter_dropout:
+            d.pop("counter_dropout")
         return d
 
     @classmethod

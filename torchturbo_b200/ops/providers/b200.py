@@ -370,15 +370,24 @@ def _graph_of_gradients(y, inputs, needs, dys):
 
 
 def _differentiated(*tensors) -> bool:
-    """Whether autograd, or a transform, has to see a call.  A Function that nothing is recorded for costs 6 us of a 9 us call."""
+    """Whether autograd has to see a call.  A Function that nothing is recorded for costs 6 us of a 9 us call."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
+    return False
+
+
+def _traced(*tensors) -> bool:
+    """Tracers, function transforms, forward-mode differentiation and tensor subclasses: theirs is the plain formulation.  (`_eager` asks
+    every tensor more; this is for calls that a kernel has done in a few microseconds.)"""
     if forward_ad._current_level >= 0 or torch.compiler.is_compiling() or torch.jit.is_tracing() or torch._C._are_functorch_transforms_active() \
             or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
         return True
-    return not all(t is None or type(t) in (torch.Tensor, torch.nn.Parameter) for t in tensors)
+    for t in tensors:
+        if t is not None and type(t) is not torch.Tensor and type(t) is not torch.nn.Parameter:
+            return True
+    return False
 
 
 class LinearBiasActFn(torch.autograd.Function):
@@ -422,7 +431,7 @@ class B200LinearBiasAct(_B200Op):
     def __call__(self, x, weight, bias=None, act=None, *, residual=None, dropout_p=0.0, seed=None, first_row=0):
         drop = dropout_args(dropout_p, seed, first_row)
         if not _ok(x, weight, bias, residual) or act not in K.ACT or weight.dim() != 2 or weight.shape[0] % 8 or weight.shape[1] % 8 or not weight.numel() \
-                or drop.t > 65535:
+                or drop.t > 65535 or _traced(x, weight, bias, residual):
             N.check_linear_bias_act(x, weight, bias, act, residual)
             return N.linear_bias_act_ref(x, weight, bias, act, residual, drop)
         if residual is not None and residual.shape[:-1] != x.shape[:-1]:          # the rest of the shapes is checked where they are read
@@ -457,7 +466,7 @@ class B200Dropout(_B200Op):
     def __call__(self, x, p, seed=None, *, residual=None, scale=1.0, first_row=0):
         N.check_dropout(x, residual)
         drop = dropout_args(p, seed, first_row, scale)
-        if not x.is_cuda or x.dtype not in (BF16, torch.float32) or not x.numel() or drop.t > 65535:
+        if not x.is_cuda or x.dtype not in (BF16, torch.float32) or not x.numel() or drop.t > 65535 or _traced(x, residual):
             return dropout_ref(x, drop, residual)
         if _differentiated(x, residual):
             y = DropoutFn.apply(_matrix(x), _matrix(residual), drop)
@@ -1025,16 +1034,17 @@ class LinearLogprobsFn(torch.autograd.Function):
                     K.gemm(dl, h_rows, a_mn=True, b_mn=True, out=mg[s:s + n], accumulate=True)
                 else:
                     K.gemm(dl, h_rows, a_mn=True, b_mn=True, out=dw[s:s + n])
-        if need_h and rows > T:
-            dh = dh[:T] + dh[T:]
-        return dh.to(BF16) if need_h else None, dw, None, None
+        if not need_h or (step >= V and rows == T):
+            return dh, dw, None, None
+        dh16 = torch.empty(T, H, dtype=BF16, device=h2.device)
+        return torch.add(dh[:T], dh[T:], out=dh16) if rows > T else dh16.copy_(dh), dw, None, None
 
 
 @_custom("linear_logprobs", "tcgen05_linear_logprobs")
 class B200LinearLogprobs(_B200Op):
     def __call__(self, hidden, weight, targets, *, want_entropy: bool = False):
         N.check_linear_logprobs(hidden, weight, targets)
-        if not _ok(hidden, weight) or hidden.shape[-1] % 8:
+        if not _ok(hidden, weight) or hidden.shape[-1] % 8 or _traced(hidden, weight):
             return N.TorchLinearLogprobs()(hidden, weight, targets, want_entropy=want_entropy)
         flat = targets if targets.dim() == 1 else targets.reshape(-1)
         flat = flat.long().contiguous()
