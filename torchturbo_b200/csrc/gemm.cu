@@ -109,22 +109,25 @@ struct GemmParams {
   int a_bytes, stage_bytes, stages;   // of a product with a tail: A in a stage, a stage, how many there are
 };
 
+constexpr int EPI_WARPS = 8;                       // two warps per TMEM lane quarter, each takes half of the columns
+constexpr int TAIL_WARPS = 16;                     // four, 64 columns each: a tail is arithmetic that wants more warps to hide its latency
+
 template <int BN, bool PAIR, int EPI>
 struct SmemLayout {
   static constexpr int A_BYTES = BM * BK * 2;
   static constexpr int B_BYTES = (PAIR ? BN / 2 : BN) * BK * 2;   // a CTA of a pair holds half of the tile's columns
   static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
-  // results and pre-activations of a warp's 64 columns are parked side by side, which costs a stage
+  // what twice the epilogue warps park costs a stage
   static constexpr int STAGES = ((BN == 256 && !PAIR) ? 4 : 6) - (EPI == EPI_TAIL ? 1 : 0);
-  static constexpr int EPI_STAGE_BYTES = 32 * 32 * 4 * (EPI == EPI_TAIL ? 2 : 1);   // one 32-row x 32-column fp32 chunk per epilogue warp
-  static constexpr int EPI_BYTES = 8 * EPI_STAGE_BYTES;
+  static constexpr int EPI_STAGE_BYTES = 32 * 32 * 4;   // one 32-row x 32-column fp32 chunk per epilogue warp, or 64 columns of bf16
+  static constexpr int WARPS = EPI == EPI_TAIL ? TAIL_WARPS : EPI_WARPS, THREADS = 64 + 32 * WARPS;
+  static constexpr int EPI_BYTES = WARPS * EPI_STAGE_BYTES;
   // A product with a tail cuts the room for its stages (statistics park nothing, so theirs is more) by what a stage really takes
   static constexpr int ROOM = STAGES * STAGE_BYTES + (EPI == EPI_LSE ? EPI_BYTES : 0);
   static constexpr int MOST = EPI >= EPI_TAIL ? 8 : STAGES;      // stages
   static constexpr int TOTAL = STAGES * STAGE_BYTES + EPI_BYTES + 1024 /*align*/ + 256 /*barriers*/;
 };
 
-constexpr int EPI_WARPS = 8;                       // two warps per TMEM lane quarter, each takes half of the columns
 constexpr int GEMM_THREADS = 64 + 32 * EPI_WARPS;
 constexpr int PUSH_WARPS = 2;                      // extra warps of a launch with the push prologue
 constexpr int GEMM_THREADS_PUSH = GEMM_THREADS + 32 * PUSH_WARPS;
@@ -148,7 +151,7 @@ __device__ __forceinline__ uint32_t epi_piece_addr64(uint32_t base, int row, int
 namespace ttb {
 
 template <int BN, bool A_MN, bool B_MN, int EPI, bool PAIR>
-__global__ void __launch_bounds__(EPI < EPI_TAIL ? GEMM_THREADS_PUSH : GEMM_THREADS, 1)
+__global__ void __launch_bounds__(EPI < EPI_TAIL ? GEMM_THREADS_PUSH : SmemLayout<BN, PAIR, EPI>::THREADS, 1)
 gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
             const __grid_constant__ CUtensorMap tmZ, const GemmParams p) {
   using L = SmemLayout<BN, PAIR, EPI>;
@@ -188,7 +191,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], PAIR ? 2 * EPI_WARPS : EPI_WARPS);
+      mbar_init(&tempty[a], PAIR ? 2 * L::WARPS : L::WARPS);
     }
     mbar_fence_init();
   }
@@ -422,14 +425,13 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
       }
     }
-  } else if (warp < 2 + EPI_WARPS) {
+  } else if (warp < 2 + L::WARPS) {
     // ------------------------------------------------------------ epilogue (warps 2..9)
     const int lane_group = warp & 3;  // TMEM lanes [32*lane_group, +32) are the ones this warp may touch
     const int col_half = (warp - 2) >> 2;  // which half of the tile's column chunks this warp stores
     int acc = 0;
     uint32_t acc_phase = 0;
     bool ok = true;
-    [[maybe_unused]] uint32_t tail_side = 0;
     Tile x = fetch(walker), next;
     for (int t = walker; t < total_tiles && ok; t += walkers, x = next) {
       int k0, nkb;
@@ -443,8 +445,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       const uint32_t t_row = tmem_base + acc * BN + (static_cast<uint32_t>(lane_group * 32) << 16);
       const long long gbase = static_cast<long long>(g) * p.c_group_stride;
       TailRow<EPI> tail;      // what the tail reads of this row, asked for ahead of the wait for the products
-      // a tail's columns are dealt out 64 at a time, as they are stored: of 192 the first warps take 128
-      const int split = p.tile_cols > 128 ? 128 : 64, tail_at = col_half * split, tail_cols = col_half ? p.tile_cols - split : split;
+      const int tail_at = 64 * col_half, tail_cols = min(64, p.tile_cols - tail_at);      // `col_half`: which quarter
       if constexpr (EPI == EPI_LSE || EPI == EPI_DLOGITS) tail.fetch(p, row);
       if constexpr (EPI == EPI_TAIL) {
         tail.fetch(p, row, nt * p.tile_cols + tail_at, tail_cols);
@@ -487,7 +488,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       if constexpr (EPI >= EPI_TAIL) {
         uint8_t* stage_at = epi_stage + (warp - 2) * L::EPI_STAGE_BYTES;
         if constexpr (EPI == EPI_TAIL)
-          tail_store(p, tmC, tmZ, tail, stage_at, t_row + tail_at, nt * p.tile_cols + tail_at, tail_cols, row_base, lane, tail_side, release);
+          tail_store(p, tmC, tmZ, tail, stage_at, t_row + tail_at, nt * p.tile_cols + tail_at, tail_cols, row_base, lane, release);
         else if constexpr (EPI == EPI_DLOGITS)
           tail_dlogits<BN>(p, tmC, tail, stage_at, t_row + col_half * (BN / 2), nt * BN + col_half * (BN / 2), row_base, lane, release);
         continue;
@@ -1152,7 +1153,7 @@ static int launch(const GemmArgs& a, cudaStream_t stream, int tile_cols = BN) {
     const int pairs = static_cast<int>(total < a.num_sms / 2 ? total : a.num_sms / 2);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(2 * pairs);
-    cfg.blockDim = dim3(GEMM_THREADS);
+    cfg.blockDim = dim3(L::THREADS);
     cfg.dynamicSmemBytes = L::TOTAL;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -1164,7 +1165,7 @@ static int launch(const GemmArgs& a, cudaStream_t stream, int tile_cols = BN) {
     if (e != cudaSuccess) return 400 + static_cast<int>(e);
   } else {
     const int grid = static_cast<int>(total < a.num_sms ? total : a.num_sms);
-    kfn<<<grid, p.ep.push_on ? GEMM_THREADS_PUSH : GEMM_THREADS, L::TOTAL, stream>>>(tmA, tmB, tmC, tmZ, p);
+    kfn<<<grid, p.ep.push_on ? GEMM_THREADS_PUSH : L::THREADS, L::TOTAL, stream>>>(tmA, tmB, tmC, tmZ, p);
   }
   if (split && a.tail) {
     const long long n = static_cast<long long>(a.M) * (a.N / 8);

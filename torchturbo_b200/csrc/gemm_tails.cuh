@@ -39,16 +39,18 @@ struct TailRow {
 };
 template <>
 struct TailRow<EPI_TAIL> {
-  uint4 res[4], bias[4];      // of 32 columns
+  uint4 res[2], bias[2];      // of 16 columns
   const __nv_bfloat16* src;
   long long row;
-  __device__ __forceinline__ void fetch32(const GemmParams& p, int col) {
+  __device__ __forceinline__ void fetch_bias(const GemmParams& p, int col) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool in = col + 8 * i < p.N;
-      if (src && in) res[i] = load16_here(src + col + 8 * i);
-      if (p.tail.bias && in) bias[i] = load16_here(p.tail.bias + col + 8 * i);
-    }
+    for (int i = 0; i < 2; ++i)
+      if (p.tail.bias && col + 8 * i < p.N) bias[i] = load16_here(p.tail.bias + col + 8 * i);
+  }
+  __device__ __forceinline__ void fetch_residual(const GemmParams& p, int col) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (src && col + 8 * i < p.N) res[i] = load16_here(src + col + 8 * i);
   }
   // `cols` columns of a row of the next tile into the L2: an epilogue of short sums is over before they would come from memory
   __device__ __forceinline__ void ahead(const GemmParams& p, int r, int col, int cols) {
@@ -60,8 +62,11 @@ struct TailRow<EPI_TAIL> {
     row = r;
     src = p.residual && r < p.M ? p.residual + static_cast<long long>(r) * p.ldr : nullptr;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) res[i] = bias[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (cols > 0) fetch32(p, col);
+    for (int i = 0; i < 2; ++i) res[i] = bias[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (cols > 0) {
+      fetch_residual(p, col);
+      fetch_bias(p, col);
+    }
   }
 };
 template <>
@@ -92,10 +97,10 @@ struct TailRow<EPI_DLOGITS> {
   }
 };
 
-// 32 values plus 32 packed ones
-__device__ __forceinline__ void add32(float (&f)[32], const uint4 (&u)[4]) {
+// 16 values plus 16 packed ones
+__device__ __forceinline__ void add16(float (&f)[16], const uint4 (&u)[2]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2; ++i) {
     const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -105,81 +110,69 @@ __device__ __forceinline__ void add32(float (&f)[32], const uint4 (&u)[4]) {
     }
   }
 }
-__device__ __forceinline__ void park32(uint32_t at, int lane, int piece, const float (&f)[32]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    st_shared_v4(epi_piece_addr(at, lane, piece + i), pack_bf16(f[8 * i], f[8 * i + 1]), pack_bf16(f[8 * i + 2], f[8 * i + 3]),
-                 pack_bf16(f[8 * i + 4], f[8 * i + 5]), pack_bf16(f[8 * i + 6], f[8 * i + 7]));
-}
 template <int ACT>
-__device__ __forceinline__ void act32(float (&f)[32]) {
+__device__ __forceinline__ void act16(float (&f)[16]) {
 #pragma unroll
-  for (int i = 0; i < 32; i += 2) act_pair<ACT>(f[i], f[i + 1]);
+  for (int i = 0; i < 16; i += 2) act_pair<ACT>(f[i], f[i + 1]);
 }
 
-// `at`: TMEM address of this warp's rows and first column, `first` that column in C, `cols` how many it has; `side`: of two parking places
-// (without pre-activations they take turns, from tile to tile) the next
+// `at`: TMEM address of this warp's rows and first column, `first` that column in C, `cols` how many it has (64 or none).  Sixteen columns
+// at a time; pre-activations are parked and stored first, the result from the same accumulator after them.
 template <typename Release>
-__device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMap& tmC, const CUtensorMap& tmZ, TailRow<EPI_TAIL>& tr, uint8_t* stage_at, uint32_t at,
-                                           int first, int cols, int row_base, int lane, uint32_t& side, Release release) {
+__device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMap& tmC, const CUtensorMap& tmZ, TailRow<EPI_TAIL>& tr, uint8_t* stage_at,
+                                           uint32_t at, int first, int cols, int row_base, int lane, Release release) {
   const TailParams& q = p.tail;
+  if (cols <= 0 || first >= p.N || row_base >= p.M) {      // uniform across the warp
+    release();
+    return;
+  }
   const KeysOfSeed key(q.drop);
   const uint64_t place = static_cast<uint64_t>(q.drop.first_row + tr.row);
   PhiloxRow mine{};
   if (q.drop.t) mine = philox_row(static_cast<uint32_t>(place), key);
-  bool held = true;
+  const uint32_t st = smem_u32(stage_at);
 #pragma unroll 1
-  for (int c = 0; c < cols; c += 32) {
-    const int col0 = first + c;
-    if (col0 >= p.N || row_base >= p.M) break;      // uniform across the warp
-    float f[32];
-    {
-      uint32_t v[32];
-      tmem_ld_32x32b_x32(at + c, v);
-      tmem_ld_wait();
+  for (int pass = q.has_pre ? 0 : 1; pass < 2; ++pass) {
+    // the copy engine has read what was parked before
+    if (lane == 0) bulk_wait_read_all();
+    __syncwarp();
+#pragma unroll 1
+    for (int c = 0; c < 64; c += 16) {
+      const int col0 = first + c;
+      float f[16];
+      {
+        uint32_t v[16];
+        tmem_ld_32x32b_x16(at + c, v);
+        tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 32; ++i) f[i] = __uint_as_float(v[i]);
-    }
-    const bool last = c + 32 >= cols;
-    if (last) {
-      release();
-      held = false;
-    }
-    const int half = (c >> 5) & 1;                  // of the 64 columns that are parked together
-    if (half == 0) {
-      // the copy engine has read what was parked there before
-      if (lane == 0) {
-        if (q.has_pre) bulk_wait_read_all();
-        else bulk_wait_read_but_one();
+        for (int i = 0; i < 16; ++i) f[i] = __uint_as_float(v[i]);
       }
-      __syncwarp();
-    }
-    const uint32_t sy = smem_u32(stage_at) + (q.has_pre ? 0u : side);
-    if (q.bias) add32(f, tr.bias);
-    if (q.has_pre) park32(sy + 4096, lane, 4 * half, f);
-    if (q.act == 1) act32<1>(f);
-    else if (q.act == 2) act32<2>(f);
-    if (q.drop.t) {
+      if (pass == 1 && c == 48) release();
+      if (q.bias) add16(f, tr.bias);
+      if (pass == 1) {
+        if (q.act == 1) act16<1>(f);
+        else if (q.act == 2) act16<2>(f);
+        if (q.drop.t) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        dropout8(f + 8 * i, philox(philox_column((col0 >> 3) + i, static_cast<uint32_t>(place >> 32), key), mine, key), q.drop.t << 16, q.drop.scale);
-    }
-    if (p.residual) add32(f, tr.res);
-    if (!last) tr.fetch32(p, col0 + 32);
-    park32(sy, lane, 4 * half, f);
-    if (half == 1 || last || col0 + 32 >= p.N) {
-      const int x = col0 - 32 * half;
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) {
-        if (q.has_pre) tma_store_3d(&tmZ, stage_at + 4096, x, row_base, 0);
-        tma_store_3d(&tmC, stage_at + (q.has_pre ? 0u : side), x, row_base, 0);
-        bulk_commit_group();
+          for (int i = 0; i < 2; ++i)
+            dropout8(f + 8 * i, philox(philox_column((col0 >> 3) + i, static_cast<uint32_t>(place >> 32), key), mine, key), q.drop.t << 16, q.drop.scale);
+        }
+        if (p.residual) add16(f, tr.res);
       }
-      side ^= 4096u;
+      if (c < 48 || pass == 0) tr.fetch_bias(p, c < 48 ? col0 + 16 : first);
+      if (c < 48 && pass == 1) tr.fetch_residual(p, col0 + 16);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        st_shared_v4(epi_piece_addr(st, lane, (c >> 3) + i), pack_bf16(f[8 * i], f[8 * i + 1]), pack_bf16(f[8 * i + 2], f[8 * i + 3]),
+                     pack_bf16(f[8 * i + 4], f[8 * i + 5]), pack_bf16(f[8 * i + 6], f[8 * i + 7]));
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_3d(pass ? &tmC : &tmZ, stage_at, first, row_base, 0);
+      bulk_commit_group();
     }
   }
-  if (held) release();
 }
 
 // The tensor cores' fp32 sums are cut off, not rounded, at every addition: after 2048 products of random signs they are 1.4e-6 of their
