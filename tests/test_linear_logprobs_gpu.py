@@ -84,6 +84,65 @@ def test_larger(T, H, V):
     _check(*_case(T, H, V), True, True)
 
 
+@pytest.mark.parametrize("T, share", [(257, 0.0), (300, 0.4), (700, 0.97), (520, 1.0), (1100, 0.5)])
+@pytest.mark.parametrize("pieces", [1, 3])
+def test_rows_without_a_target_are_left_out(monkeypatch, T, share, pieces):
+    """Wide vocabularies: prompts and padding are not computed.  None, some, nearly all and all of the rows; not a number in them stays there."""
+    from torchturbo_b200 import kernels as Kn
+    from torchturbo_b200.ops import ops
+    from torchturbo_b200.ops.providers.b200 import LinearLogprobsFn as Fn
+
+    h, w, t = _case(T, 136, 33003, std=1.0)
+    gen = torch.Generator().manual_seed(T)
+    t = torch.where(t < 0, 5, t)
+    t[(torch.rand(T, generator=gen) < share).cuda()] = -100
+    if share == 1.0:
+        t[:] = -1
+    assert Fn.compact(h, w, False) and not Fn.compact(h, w, True)
+    if pieces > 1:
+        monkeypatch.setattr(Fn, "PIECE", T * 33003 // 3)
+    _check(h, w, t, False, True)
+    if 0 < share < 1:
+        with torch.no_grad():
+            want = ops.linear_logprobs(h, w, t)[0]
+            h[t < 0] = float("nan")
+        logp, _ = ops.linear_logprobs(h, w, t)
+        dh, dw = torch.autograd.grad(logp.sum(), (h, w))
+        assert torch.equal(logp, want) and torch.isfinite(dh).all() and torch.isfinite(dw).all() and (dh[t < 0] == 0).all()
+        v = w.detach().clone().requires_grad_()
+        v.main_grad = torch.ones(33003, 136, device="cuda")
+        ops.linear_logprobs(h, v, t)[0].sum().backward()
+        assert ((v.main_grad - 1) - dw.float()).abs().max() <= HALF * dw.float().abs().max() + 1e-5
+    assert Kn.status() == (0, 0)
+
+
+@pytest.mark.parametrize("there", [0, 1, 63, 64, 129, 300, 512])
+@pytest.mark.parametrize("splits", [0, 2])
+def test_products_of_rows_that_the_device_counts(there, splits):
+    from torchturbo_b200 import kernels as Kn
+
+    gen = torch.Generator().manual_seed(there)
+    K = 4160 if splits else 200
+    count = torch.tensor([there], dtype=torch.int32, device="cuda")
+    a, b = (torch.randn(*s, generator=gen).bfloat16().cuda() for s in ((512, K), (K, 264)))
+    out = torch.full((512, 264), 7.0, dtype=torch.bfloat16, device="cuda")
+    Kn.gemm(a, b, b_mn=True, out=out, rows=count, splits=splits)
+    assert torch.equal(out[:there], Kn.gemm(a, b, b_mn=True, splits=splits)[:there])
+    if not splits:
+        assert (out[(there + 255) // 256 * 256:] == 7).all()
+    # of the rows of both operands: zeros behind them to the next multiple of 64
+    R = 8192 if splits else 512
+    x, y = (torch.randn(R, n, generator=gen).bfloat16().cuda() for n in (136, 264))
+    x[there:(there + 63) // 64 * 64] = 0
+    count.fill_(there)
+    want = Kn.gemm(torch.where(torch.arange(R, device="cuda")[:, None] < there, x, 0), y, a_mn=True, b_mn=True, splits=splits)
+    assert torch.equal(Kn.gemm(x, y, a_mn=True, b_mn=True, rows=count, splits=splits), want)
+    acc = torch.ones(136, 264, device="cuda")
+    Kn.gemm(x, y, a_mn=True, b_mn=True, rows=count, out=acc, accumulate=True, splits=splits)
+    assert ((acc - 1) - want.float()).abs().max() <= HALF * want.float().abs().max() + 1e-4
+    assert Kn.status() == (0, 0)
+
+
 def test_rows_in_shares():
     """Statistics of more rows than are held at a time (2^26 values of 1188 pieces and three planes: 18688 rows)."""
     from torchturbo_b200.ops import ops

@@ -30,6 +30,7 @@ struct TailArgs {
   // 4: C = gradient of the logits of columns first_col .. first_col + N - 1
   const float *lse, *ent, *dlogp, *dent;   // [M]; `ent` and `dent` may be null
   long long first_col;
+  const int* rows;                     // [M] where a row's dlogp and dent are, or null: at its own place
   int rest;                            // C has M more rows behind, for what the rounding to bf16 left out
 };
 
@@ -64,6 +65,10 @@ struct GemmArgs {
   float* split_ws;               // optional fp32 [k_splits, M, N]: the product is formed in k_splits pieces, then added up
   int k_splits;
   const TailArgs* tail;
+  // Rows that are there, where the device alone knows: of A's and C's M rows (with part_k of the K rows of both operands) those from
+  // row0 on that lie below *part_rows; what lies behind is neither read nor written but to the end of a tile.
+  const int* part_rows;
+  int row0, part_k;
 };
 
 // inputs of the chunk-parallel delta-rule kernels (delta_chunk.cuh)
@@ -81,7 +86,11 @@ struct DeltaChunkIn {
 
 TTB_EXPORT int ttb_gemm_bf16(const ttb::GemmArgs*, void*);
 TTB_EXPORT int ttb_logprobs_slots(int, int, int, int, int*);
-TTB_EXPORT int ttb_logprobs_join(const float*, const float*, const long long*, int, long long, long long, float*, float*, float*, void*);
+TTB_EXPORT int ttb_logprobs_join(const float*, const float*, const long long*, const int*, const int*, int, int, long long, long long, float*,
+                            float*, float*, void*);
+TTB_EXPORT int ttb_rows_with_targets(const long long*, long long, long long, int*, int*, long long*, int*, float*, void*);
+TTB_EXPORT int ttb_gather_rows(const void*, long long, const int*, const int*, void*, long long, int, void*);
+TTB_EXPORT int ttb_scatter_rows(const void*, int, const int*, void*, long long, int, void*);
 TTB_EXPORT int ttb_dropout(const void*, const void*, void*, int, long long, int, unsigned, float, unsigned long long, const unsigned long long*,
                             long long, int, void*);
 TTB_EXPORT int ttb_tail_row_blocks(long long, int, int);

@@ -40,7 +40,8 @@ constexpr int BM = 128;
 constexpr int BK = 64;
 constexpr unsigned KID_GEMM = 1;
 
-enum Epi : int { EPI_STORE = 0, EPI_SWIGLU = 1, EPI_TAIL = 2, EPI_LSE = 3, EPI_DLOGITS = 4 };
+// EPI_PART: as EPI_STORE, of rows whose number only the device knows
+enum Epi : int { EPI_PART = -1, EPI_STORE = 0, EPI_SWIGLU = 1, EPI_TAIL = 2, EPI_LSE = 3, EPI_DLOGITS = 4 };
 
 // Expert-parallel fusion parameters (device side).
 struct EpFuse {
@@ -79,6 +80,7 @@ struct TailParams {
   long long vocab;
   float *part, *target_logit;
   const float *lse, *ent, *dlogp, *dent;
+  const int* rows;
   long long first_col;
 };
 
@@ -106,6 +108,9 @@ struct GemmParams {
   int k_splits, kb_per_split;  // > 1: "group" g covers k-blocks [g, g + 1) * kb_per_split of one product, stored at C[g]
   TailParams tail;
   int tile_cols;   // columns of a tile whose results are not stored (EPI_LSE)
+  // rows that there are of the M (or, for `part_k`, of the K) that the buffers have, known on the device only; those before row0 are another call's
+  const int* part_rows;
+  int row0, part_k;
   int a_bytes, stage_bytes, stages;   // of a product with a tail: A in a stage, a stage, how many there are
 };
 
@@ -209,8 +214,20 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
+  constexpr bool STORE = EPI == EPI_STORE || EPI == EPI_PART;
+  constexpr bool PART = EPI == EPI_PART || EPI == EPI_LSE || EPI == EPI_DLOGITS;
+  int m_tiles = p.m_tiles, m_rows = p.M, k_rows = p.K;
+  if (PART && p.part_rows) {
+    const int there = min(max(__ldg(p.part_rows) - p.row0, 0), p.part_k ? p.K : p.M);
+    if (p.part_k) {
+      k_rows = there;
+    } else {
+      m_rows = there;
+      m_tiles = (there + (PAIR ? 2 : 1) * BM - 1) / ((PAIR ? 2 : 1) * BM);
+    }
+  }
   const int groups = p.groups_k > 0 ? p.groups_k : p.k_splits;
-  const int tiles_per_group = p.m_tiles * p.n_tiles;      // the launch checks that all tiles can be counted in 31 bits
+  const int tiles_per_group = m_tiles * p.n_tiles;      // the launch checks that all tiles can be counted in 31 bits
   const int total_tiles = s_dead ? 0 : tiles_per_group * groups;
 
   // Decode tile -> (g, m_tile, n_tile).  Tiles are walked in bands of RASTER_M m-tiles: inside a band m runs
@@ -228,13 +245,15 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   auto fetch = [&](int t) {
     Tile x{0, 0, 0, 0, 0};
     if (t >= total_tiles) return x;
-    x.g = p.by_group(t);
+    // tile counts that the host does not know are divided by as they are
+    const bool counted = PART && p.part_rows != nullptr;
+    x.g = counted ? t / tiles_per_group : p.by_group(t);
     const int r = t - x.g * tiles_per_group;
     const int band = p.by_band(r);
     const int m_base = band * RASTER_M;
     const int w = r - band * RASTER_M * p.n_tiles;
-    const int left = p.m_tiles - m_base;
-    x.nt = left < RASTER_M ? p.by_rest(w) : w / RASTER_M;
+    const int left = m_tiles - m_base;
+    x.nt = left < RASTER_M ? (counted ? w / left : p.by_rest(w)) : w / RASTER_M;
     x.mt = m_base + w - x.nt * (left < RASTER_M ? left : RASTER_M);
     if (PAIR) x.mt = 2 * x.mt + rank;
     if (p.tile_group) {
@@ -254,10 +273,11 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
     } else if (p.k_splits > 1) {
       const int kb0 = x.g * p.kb_per_split;
       k0 = kb0 * BK;
-      nkb = min(p.kb_per_split, (p.K + BK - 1) / BK - kb0);
+      nkb = min(p.kb_per_split, (k_rows + BK - 1) / BK - kb0);
+      if (PART && nkb < 0) nkb = 0;
     } else {
       k0 = 0;
-      nkb = (p.K + BK - 1) / BK;
+      nkb = (k_rows + BK - 1) / BK;
     }
   };
 
@@ -446,7 +466,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       const long long gbase = static_cast<long long>(g) * p.c_group_stride;
       TailRow<EPI> tail;      // what the tail reads of this row, asked for ahead of the wait for the products
       const int tail_at = 64 * col_half, tail_cols = min(64, p.tile_cols - tail_at);      // `col_half`: which quarter
-      if constexpr (EPI == EPI_LSE || EPI == EPI_DLOGITS) tail.fetch(p, row);
+      if constexpr (EPI == EPI_LSE || EPI == EPI_DLOGITS) tail.fetch(p, row, m_rows);
       if constexpr (EPI == EPI_TAIL) {
         tail.fetch(p, row, nt * p.tile_cols + tail_at, tail_cols);
         if (t + walkers < total_tiles) tail.ahead(p, next.mt * BM + lane_group * 32 + lane, next.nt * p.tile_cols + tail_at, tail_cols);
@@ -493,7 +513,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
           tail_dlogits<BN>(p, tmC, tail, stage_at, t_row + col_half * (BN / 2), nt * BN + col_half * (BN / 2), row_base, lane, release);
         continue;
       }
-      if (EPI == EPI_STORE && p.tma_out) {
+      if (STORE && p.tma_out) {
         // Plain bf16 rows, 64 columns at a time: parked as bf16 (128 bytes a row, the copy engine's swizzle) and handed to the copy
         // engine, which clips at the edges of C.  An SM's ordinary stores leave at 32 bytes a clock however they are shaped, and a warp
         // that issues them waits: 2500 clocks of a tile's epilogue, which was 5000 with the decoding of the tile, against 2600 of
@@ -549,7 +569,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
         if (held) release();
         continue;
       }
-      if (EPI == EPI_STORE) {
+      if (STORE) {
         const int n0 = nt * BN;
         uint8_t* cbase = reinterpret_cast<uint8_t*>(p.C);
         const long long coff = gbase + static_cast<long long>(row) * p.ldc;
@@ -798,7 +818,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       }
       release();
     }
-    if ((EPI == EPI_STORE ? p.tma_out : EPI == EPI_TAIL || EPI == EPI_DLOGITS) && lane == 0) bulk_wait_all();
+    if ((STORE ? p.tma_out : EPI == EPI_TAIL || EPI == EPI_DLOGITS) && lane == 0) bulk_wait_all();
     if (p.ep.scat_on) __threadfence_system();   // this thread's peer stores are ordered before the "returned" flag
   } else if (p.ep.push_on) {
     // ------------------------------------------------------------ push warps (warps 10..11)
@@ -1098,7 +1118,7 @@ static int launch(const GemmArgs& a, cudaStream_t stream, int tile_cols = BN) {
     p.tail.bias = reinterpret_cast<const __nv_bfloat16*>(t.bias); p.tail.act = t.act;
     p.tail.drop = dropout_params(t.drop_t, t.drop_scale, t.seed, t.seed_dev, t.first_row);
     p.tail.targets = t.targets; p.tail.vocab = t.vocab; p.tail.part = t.part; p.tail.target_logit = t.target_logit; p.tail.entropy = t.entropy;
-    p.tail.lse = t.lse; p.tail.ent = t.ent; p.tail.dlogp = t.dlogp; p.tail.dent = t.dent; p.tail.first_col = t.first_col;
+    p.tail.lse = t.lse; p.tail.ent = t.ent; p.tail.dlogp = t.dlogp; p.tail.dent = t.dent; p.tail.first_col = t.first_col; p.tail.rows = t.rows;
   }
   const bool split = a.split_ws != nullptr && a.k_splits > 1;
   if (split) {
@@ -1116,7 +1136,8 @@ static int launch(const GemmArgs& a, cudaStream_t stream, int tile_cols = BN) {
   if (total >= (1ll << 31) - 65536) return 910;
   // ---- C map (3D, last dim = group)
   tmC = tmZ = tmA;       // placeholders where nothing is stored through them
-  p.tma_out = EPI == EPI_STORE && !split && !a.c_fp32 && !a.residual && !a.accumulate && !p.ep.scat_on && a.M > 0 && a.N > 0 &&
+  p.part_rows = a.part_rows; p.row0 = a.row0; p.part_k = a.part_k;
+  p.tma_out = (EPI == EPI_STORE || EPI == EPI_PART) && !split && !a.c_fp32 && !a.residual && !a.accumulate && !p.ep.scat_on && a.M > 0 && a.N > 0 &&
               (a.groups_k == 0 || a.c_group_stride % 8 == 0);
   if (p.tma_out) {
     const uint64_t dims[3] = {static_cast<uint64_t>(a.N), static_cast<uint64_t>(a.M), static_cast<uint64_t>(a.groups_k > 0 ? a.groups_k : 1)};
@@ -1270,6 +1291,14 @@ TTB_EXPORT int ttb_gemm_bf16(const ttb::GemmArgs* args, void* stream_ptr) {
     if (e.scat_on && (a.epi != EPI_STORE || a.c_fp32 || a.accumulate || a.residual || (a.N % 32) || !e.row_tag ||
                       !e.done_counter || (e.off_ret % 16)))
       return 908;
+  }
+  if (a.epi < EPI_STORE || a.epi > EPI_DLOGITS) return 905;
+  if (a.part_rows && (a.epi == EPI_SWIGLU || a.epi == EPI_TAIL || a.tile_group || a.groups_k > 0 || a.ep || a.residual)) return 914;
+  if (a.epi == EPI_STORE && a.part_rows) {
+    if (!a.b_mn || a.N <= 128 || a.part_k != a.a_mn) return 914;      // rows of the result, or of both operands
+    const bool pair = pays_in_pairs(a);
+    if (a.a_mn) return pair ? launch<256, true, true, EPI_PART, true>(a, stream) : launch<256, true, true, EPI_PART, false>(a, stream);
+    return pair ? launch<256, false, true, EPI_PART, true>(a, stream) : launch<256, false, true, EPI_PART, false>(a, stream);
   }
   if (a.epi >= EPI_TAIL) {
     if (!a.tail || a.epi > EPI_DLOGITS || a.a_mn || a.b_mn || a.tile_group || a.groups_k > 0 || a.ep || a.alpha || a.accumulate || a.c_fp32) return 911;

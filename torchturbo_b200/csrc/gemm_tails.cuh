@@ -35,7 +35,7 @@ __device__ __forceinline__ uint4 load16_here(const void* p) {
 // What an epilogue thread reads of its row (one row a thread) before the accumulator is there
 template <int EPI>
 struct TailRow {
-  __device__ __forceinline__ void fetch(const GemmParams&, int) {}
+  __device__ __forceinline__ void fetch(const GemmParams&, int, int) {}
 };
 template <>
 struct TailRow<EPI_TAIL> {
@@ -72,26 +72,27 @@ struct TailRow<EPI_TAIL> {
 template <>
 struct TailRow<EPI_LSE> {
   long long target;
-  __device__ __forceinline__ void fetch(const GemmParams& p, int r) { target = r < p.M ? __ldg(p.tail.targets + r) : -1; }
+  __device__ __forceinline__ void fetch(const GemmParams& p, int r, int rows) { target = r < rows ? __ldg(p.tail.targets + r) : -1; }
 };
 template <>
 struct TailRow<EPI_DLOGITS> {
   long long target;      // column of this product, or one that it does not have
   float lse2, g, e, shift;
-  __device__ __forceinline__ void fetch(const GemmParams& p, int r) {
+  __device__ __forceinline__ void fetch(const GemmParams& p, int r, int rows) {
     const TailParams& q = p.tail;
     target = -1;
     lse2 = g = e = shift = 0.f;
-    if (r >= p.M) return;
+    if (r >= rows) return;
+    const int from = q.rows ? __ldg(q.rows + r) : r;      // row of the caller's gradients
     const long long t = __ldg(q.targets + r);
     if (t >= 0 && t < q.vocab) {
       target = t - q.first_col;
-      g = q.dlogp ? __ldg(q.dlogp + r) : 0.f;
+      g = q.dlogp ? __ldg(q.dlogp + from) : 0.f;
     }
     const float lse = __ldg(q.lse + r);
     lse2 = lse * LOG2E;
     if (q.dent) {
-      e = __ldg(q.dent + r);
+      e = __ldg(q.dent + from);
       shift = __ldg(q.ent + r);
     }
   }

@@ -167,7 +167,7 @@ long long k_splits(long long M, long long N, long long K, int num_sms) {
 // ---------------------------------------------------------------------------------------------
 PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    Args in(args, n, 16);
+    Args in(args, n, 17);
     const Tensor &a = in.tensor(), &b = in.tensor();
     const bool a_mn = in.flag(), b_mn = in.flag();
     Tensor out = in.optional();
@@ -178,6 +178,7 @@ PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const long long ep = in.integer();
     const Tensor alpha = in.optional();
     const long long splits = in.integer();
+    const Tensor there = in.optional();
     need(is_bf16(a) && is_bf16(b), "operands must be bf16");
     need(a.stride(-1) == 1 && b.stride(-1) == 1, "operands must be contiguous along their last dimension");
     check_device(a);
@@ -242,6 +243,10 @@ PyObject* gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
       g.alpha = f32(alpha);
     }
     g.ep = reinterpret_cast<const ttb::EpFuseArgs*>(ep);
+    if (there.defined()) {
+      need(there.scalar_type() == at::kInt && there.numel() == 1 && there.device() == a.device(), "how many rows there are is one int32 value on the device");
+      g.part_rows = i32(there); g.part_k = a_mn;
+    }
     Tensor ws;
     int kernels = 1;
     if (K >= 4096 && !swiglu && !tile_group.defined() && !ep) {
@@ -458,20 +463,34 @@ PyObject* dropout(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-// log-probabilities of `targets`, log-sum-exp of every row of logits and, if wanted, its entropy
+// (logp, lse, ent, and with `compact` the rows that have a target: hidden states, targets, places, inverse places, count).  Log-probabilities of
+// `targets`, log-sum-exp of every row of logits (of the rows with a target, in their order) and, if wanted, its entropy
 PyObject* logprobs_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    Args in(args, n, 4);
+    Args in(args, n, 5);
     const Tensor h = operand(in.tensor()), w = operand(in.tensor());
     const Tensor& targets = in.tensor();
-    const bool want_ent = in.flag();
+    const bool want_ent = in.flag(), compact = in.flag();
     GemmArgs g = product(h, w);
-    const long long M = g.M;
+    const long long M = g.M, K = g.K;
     need(targets.scalar_type() == at::kLong && targets.dim() == 1 && targets.is_contiguous() && targets.numel() == M && targets.device() == h.device(),
          "targets: one int64 value a row");
-    need(g.N > 0 && g.K > 0, "a vocabulary and hidden states of at least one value");
+    need(g.N > 0 && K > 0, "a vocabulary and hidden states of at least one value");
+    need(!compact || (!want_ent && K % 8 == 0), "the entropy is of every row");
     const Tensor logp = empty({M}, at::kFloat, h), lse = empty({M}, at::kFloat, h), ent = want_ent ? empty({M}, at::kFloat, h) : Tensor();
-    if (M == 0) return wrap_all(logp, lse, ent);
+    Tensor hc, tc = targets, rows, place, count;
+    if (M == 0) return wrap_all(logp, lse, ent, hc, hc, hc, hc, hc);
+    if (compact) {
+      hc = empty({(M + 255) / 256 * 256, K}, at::kBFloat16, h);
+      tc = empty({M}, at::kLong, h); rows = empty({M}, at::kInt, h); place = empty({M}, at::kInt, h); count = empty({1}, at::kInt, h);
+      launch("ttb_rows_with_targets", 1, [&](void* st) {
+        return ttb_rows_with_targets(static_cast<const long long*>(at_(targets)), M, g.N, static_cast<int*>(to_(rows)), static_cast<int*>(to_(place)),
+                                     static_cast<long long*>(to_(tc)), static_cast<int*>(to_(count)), f32w(logp), st);
+      });
+      launch("ttb_gather_rows", 1, [&](void* st) { return ttb_gather_rows(at_(h), h.stride(0), i32(rows), i32(count), to_(hc), M, static_cast<int>(K), st); });
+      g.A = hc.const_data_ptr(); g.lda = K;
+      g.part_rows = i32(count);
+    }
     const Tensor hit = empty({M}, at::kFloat, h);
     ttb::TailArgs t{};
     t.vocab = g.N; t.entropy = want_ent;
@@ -479,38 +498,46 @@ PyObject* logprobs_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     // The statistics of all pieces are 8 or 12 bytes for every 128 logits; rows are taken in shares that keep them below 256 MB
     const int planes = want_ent ? 3 : 2;
     const long long share = std::max<long long>(256, (1ll << 26) / (planes * (2ll * ((g.N + 255) / 256) + 2)) / 256 * 256);
+    const void* first = g.A;
     Tensor part;
     for (long long r = 0; r < M; r += share) {
-      const long long rows = std::min(share, M - r);
-      g.A = static_cast<const char*>(h.const_data_ptr()) + r * g.lda * 2;
-      g.M = static_cast<int>(rows);
+      const long long some = std::min(share, M - r);
+      g.A = static_cast<const char*>(first) + r * g.lda * 2;
+      g.M = static_cast<int>(some);
+      g.row0 = static_cast<int>(r);
       const int slots = logprobs_slots(g, &t.tile_cols);
-      if (!part.defined() || part.numel() < planes * slots * rows) part = empty({planes * slots * rows}, at::kFloat, h);
-      t.targets = static_cast<const long long*>(at_(targets)) + r;
+      if (!part.defined() || part.numel() < planes * slots * some) part = empty({planes * slots * some}, at::kFloat, h);
+      t.targets = static_cast<const long long*>(at_(tc)) + r;
       t.part = f32w(part); t.target_logit = f32w(hit) + r;
       launch("ttb_gemm_bf16", 1, [&](void* st) { return ttb_gemm_bf16(&g, st); });
       launch("ttb_logprobs_join", 1, [&](void* st) {
-        return ttb_logprobs_join(f32(part), t.target_logit, t.targets, slots, rows, g.N, f32w(logp) + r, f32w(lse) + r, ent.defined() ? f32w(ent) + r : nullptr, st);
+        return ttb_logprobs_join(f32(part), t.target_logit, t.targets, compact ? i32(rows) + r : nullptr, g.part_rows, g.row0, slots, some, g.N,
+                                 compact ? f32w(logp) : f32w(logp) + r, f32w(lse) + r, ent.defined() ? f32w(ent) + r : nullptr, st);
       });
     }
-    return wrap_all(logp, lse, ent);
+    return wrap_all(logp, lse, ent, hc, compact ? tc : Tensor(), rows, place, count);
   });
 }
 
-// gradient of the logits of columns first_col .. first_col + w.size(0) - 1 of a vocabulary, into `out`
+// gradient of the logits of columns first_col .. first_col + w.size(0) - 1 of a vocabulary, into `out`; with `rows` and `count` of the rows
+// with a target alone
 PyObject* logprobs_dlogits(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    Args in(args, n, 10);
+    Args in(args, n, 12);
     const Tensor &h = in.tensor(), &w = in.tensor(), &targets = in.tensor(), &lse = in.tensor();
     const Tensor ent = in.optional(), dlogp = in.optional(), dent = in.optional();
     ttb::TailArgs t{};
     t.first_col = in.integer();
     t.vocab = in.integer();
     const Tensor& out = in.tensor();
+    const Tensor rows = in.optional(), count = in.optional();
     GemmArgs g = product(h, w);
     need(targets.scalar_type() == at::kLong && targets.is_contiguous() && targets.numel() == g.M && targets.device() == h.device(), "targets: one int64 value a row");
     for (const Tensor& r : {lse, ent, dlogp, dent})
       need(!r.defined() || (r.scalar_type() == at::kFloat && r.is_contiguous() && r.numel() == g.M && r.device() == h.device()), "statistics and gradients: one fp32 value a row");
+    for (const Tensor& r : {rows, count})
+      need(!r.defined() || (r.scalar_type() == at::kInt && r.is_contiguous() && r.device() == h.device()), "places of rows are int32");
+    need(rows.defined() == count.defined() && (!rows.defined() || (rows.numel() == g.M && count.numel() == 1)), "a place for each row, and how many there are");
     need(!dent.defined() || ent.defined(), "the entropy's gradient needs the entropy");
     t.rest = out.dim() == 2 && out.size(0) == 2ll * g.M;
     need_rows(out, t.rest ? 2ll * g.M : g.M, g.N, h, "the gradient is bf16, a row or two for each of the hidden states");
@@ -518,9 +545,27 @@ PyObject* logprobs_dlogits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (g.M == 0 || g.N == 0) return wrap(out);
     t.targets = static_cast<const long long*>(at_(targets));
     t.lse = f32(lse); t.ent = f32(ent); t.dlogp = f32(dlogp); t.dent = f32(dent);
+    t.rows = i32(rows);
+    g.part_rows = i32(count);
     g.C = out.data_ptr(); g.ldc = out.stride(0);
     g.epi = 4; g.tail = &t;
     launch("ttb_gemm_bf16", 1, [&](void* st) { return ttb_gemm_bf16(&g, st); });
+    return wrap(out);
+  });
+}
+
+// [R, cols] bf16: row place[r] of x, or zeros where that is negative
+PyObject* scatter_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    Args in(args, n, 2);
+    const Tensor &x = in.tensor(), &place = in.tensor();
+    check_device(x);
+    need(x.dim() == 2 && x.is_contiguous() && (is_bf16(x) || x.scalar_type() == at::kFloat) && x.size(1) % 8 == 0 && on_16_bytes(x), "bf16 or fp32 rows without gaps");
+    need(place.scalar_type() == at::kInt && place.is_contiguous() && place.dim() == 1 && place.device() == x.device(), "places of rows are int32");
+    const Tensor out = empty({place.numel(), x.size(1)}, at::kBFloat16, x);
+    launch("ttb_scatter_rows", 1, [&](void* st) {
+      return ttb_scatter_rows(at_(x), !is_bf16(x), i32(place), to_(out), place.numel(), static_cast<int>(x.size(1)), st);
+    });
     return wrap(out);
   });
 }
@@ -1104,7 +1149,7 @@ PyObject* launches(PyObject*, PyObject* const*, Py_ssize_t) { return PyLong_From
 
 #define ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {ENTRY(setup), ENTRY(launches), ENTRY(gemm), ENTRY(linear_tail), ENTRY(tail_bwd), ENTRY(linear_tail_bwd), ENTRY(dropout), ENTRY(logprobs_fwd),
-                         ENTRY(logprobs_dlogits), ENTRY(rmsnorm_fwd), ENTRY(rmsnorm_bwd), ENTRY(layernorm_fwd), ENTRY(layernorm_bwd),
+                         ENTRY(logprobs_dlogits), ENTRY(scatter_rows), ENTRY(rmsnorm_fwd), ENTRY(rmsnorm_bwd), ENTRY(layernorm_fwd), ENTRY(layernorm_bwd),
                          ENTRY(bias_act_fwd), ENTRY(bias_act_bwd), ENTRY(qknorm_rope_fwd), ENTRY(qknorm_rope_bwd), ENTRY(qkv_rope_fwd), ENTRY(qkv_rope_bwd), ENTRY(gdn_gate_fwd),
                          ENTRY(gdn_gate_bwd), ENTRY(scale), ENTRY(copy_words), ENTRY(kda_gate_fwd), ENTRY(kda_gate_bwd), ENTRY(delta_prep), ENTRY(delta_out), ENTRY(delta_bwd_pre),
                          ENTRY(delta_state_scan), ENTRY(rope), ENTRY(swiglu_fwd),

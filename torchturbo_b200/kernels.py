@@ -200,6 +200,7 @@ def gemm(
     ep: "EpFuseArgs | None" = None,
     alpha: torch.Tensor | None = None,
     splits: int = 0,
+    rows: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """tcgen05 GEMM ``C = op(A) @ op(B)`` on bf16 operands with fp32 accumulation.
 
@@ -214,9 +215,11 @@ def gemm(
         ``silu(gate) * up * row_scale`` of width ``F``; ``preact`` (``[M, 2F]``) optionally keeps gate|up.
       * ``alpha`` (one fp32 value on the device) is multiplied into the fp32 product before it is rounded or added.
       * ``splits`` pieces along K (from 4096 on) in place of `gemm_splits`'s.
+      * ``rows`` (one int32 value on the device; ``b_mn``, more than 128 columns): only so many of the rows of ``a`` and the result are there,
+        with ``a_mn`` of the rows of both operands; what lies behind them is not computed (with ``a_mn`` the operands' next 63 rows are zero).
     """
     return host().gemm(a, b, a_mn, b_mn, out, _is_f32(out_dtype), accumulate, residual, tile_group, group_rows, swiglu, row_scale, preact,
-                       C.addressof(ep) if ep is not None else 0, alpha, splits)
+                       C.addressof(ep) if ep is not None else 0, alpha, splits, rows)
 
 
 # --------------------------------------------------------------------------------------
@@ -244,16 +247,24 @@ def dropout(x, residual, drop):
     return host().dropout(x, residual, drop.t, drop.scale, drop.seed, drop.seed_tensor, drop.first_row)
 
 
-def logprobs_fwd(hidden, weight, targets, want_entropy: bool):
-    """(logp, lse, entropy) fp32 per row of ``hidden @ weight.T``, whose values are not stored; ``logp`` is 0 where the target lies
-    outside the vocabulary, ``entropy`` None unless wanted."""
-    return host().logprobs_fwd(hidden, weight, targets, want_entropy)
+def logprobs_fwd(hidden, weight, targets, want_entropy: bool, compact: bool = False):
+    """(logp, lse, entropy, rows) fp32 per row of ``hidden @ weight.T``, whose values are not stored; ``logp`` is 0 where the target lies
+    outside the vocabulary, ``entropy`` None unless wanted.  With ``compact`` only rows that have a target are computed; ``lse`` has theirs
+    first and ``rows`` is (their hidden states, targets, places, every row's place among them or -1, how many), else None."""
+    logp, lse, ent, *rows = host().logprobs_fwd(hidden, weight, targets, want_entropy, compact)
+    return logp, lse, ent, tuple(rows) if rows[0] is not None else None
 
 
-def logprobs_dlogits(hidden, weight, targets, lse, entropy, dlogp, dent, first_col: int, vocab: int, out):
+def logprobs_dlogits(hidden, weight, targets, lse, entropy, dlogp, dent, first_col: int, vocab: int, out, rows=None, count=None):
     """Gradient of the logits of the columns that ``weight`` (rows ``first_col ..`` of the head's) covers, bf16, into ``out``; an
-    ``out`` of twice the rows takes what the rounding left out behind them."""
-    return host().logprobs_dlogits(hidden, weight, targets, lse, entropy, dlogp, dent, first_col, vocab, out)
+    ``out`` of twice the rows takes what the rounding left out behind them.  ``rows`` and ``count`` as `logprobs_fwd` gives them: the
+    other operands are of the rows with a target, ``dlogp`` of all."""
+    return host().logprobs_dlogits(hidden, weight, targets, lse, entropy, dlogp, dent, first_col, vocab, out, rows, count)
+
+
+def scatter_rows(x, place):
+    """[len(place), cols] bf16: row ``place[r]`` of ``x`` (fp32 or bf16), zeros where it is negative."""
+    return host().scatter_rows(x, place)
 
 
 # --------------------------------------------------------------------------------------

@@ -990,15 +990,21 @@ class LinearLogprobsFn(torch.autograd.Function):
         return -(-vocab // (256 * count)) * 256
 
     @staticmethod
+    def compact(hidden, weight, want_entropy: bool) -> bool:
+        """Whether rows without a target (prompts, padding) are left out; the host does not know how many there are.  Finding and copying the
+        others takes 460 / V of the product's time, and small inputs have their tiles whether they are full or not."""
+        return not want_entropy and hidden.shape[0] > 256 and weight.shape[0] >= 32768 and hidden.shape[1] > 128
+
+    @staticmethod
     def forward(ctx, hidden, weight, targets, want_entropy):
-        logp, lse, ent = K.logprobs_fwd(hidden, weight, targets, want_entropy)
-        ctx.save_for_backward(hidden, weight, targets, lse, ent)
+        logp, lse, ent, rows = K.logprobs_fwd(hidden, weight, targets, want_entropy, LinearLogprobsFn.compact(hidden, weight, want_entropy))
+        ctx.save_for_backward(hidden, weight, targets, lse, ent, *(rows or ()))
         ctx.set_materialize_grads(False)
         return (logp, ent) if want_entropy else logp
 
     @staticmethod
     def backward(ctx, dlogp, dent=None):
-        hidden, weight, targets, lse, ent = ctx.saved_tensors
+        hidden, weight, targets, lse, ent, *rows_of = ctx.saved_tensors
         need_h, need_w = ctx.needs_input_grad[:2]
         if (dlogp is None and dent is None) or not (need_h or need_w):
             return None, None, None, None
@@ -1008,6 +1014,10 @@ class LinearLogprobsFn(torch.autograd.Function):
             return *_graph_of_gradients([y for y, _ in pairs], (hidden, weight), (need_h, need_w), [g for _, g in pairs]), None, None
         h2, w2 = _operand(hidden), _operand(weight)
         (T, H), V = h2.shape, w2.shape[0]
+        which = place = there = None
+        if rows_of:                       # of the rows with a target, `there` of them
+            h2, targets, which, place, there = rows_of
+            h2 = h2[:T]
         gs = [g.float().contiguous() if g is not None else None for g in (dlogp, dent)]
         mg = getattr(weight, "main_grad", None) if need_w else None
         dw = torch.empty(V, H, dtype=BF16, device=h2.device) if need_w and mg is None else None
@@ -1022,18 +1032,20 @@ class LinearLogprobsFn(torch.autograd.Function):
             n = min(step, V - s)
             piece = w2[s:s + n]
             dl = buf[:rows * (-(-n // 8) * 8)].view(rows, -1)[:, :n]
-            K.logprobs_dlogits(h2, piece, targets, lse, ent if dent is not None else None, *gs, s, V, dl)
+            K.logprobs_dlogits(h2, piece, targets, lse, ent if dent is not None else None, *gs, s, V, dl, which, there)
             if need_h:
                 splits = K.wave_splits(rows, H, n, sms)
                 if step >= V and rows == T:
-                    dh = K.gemm(dl, piece, b_mn=True, splits=splits)
+                    dh = K.gemm(dl, piece, b_mn=True, splits=splits, rows=there)
                 else:
-                    dh = K.gemm(dl, piece, b_mn=True, out=dh, out_dtype=torch.float32, accumulate=dh is not None, splits=splits)
+                    dh = K.gemm(dl, piece, b_mn=True, out=dh, out_dtype=torch.float32, accumulate=dh is not None, splits=splits, rows=there)
             if need_w:
                 if mg is not None:
-                    K.gemm(dl, h_rows, a_mn=True, b_mn=True, out=mg[s:s + n], accumulate=True)
+                    K.gemm(dl, h_rows, a_mn=True, b_mn=True, out=mg[s:s + n], accumulate=True, rows=there)
                 else:
-                    K.gemm(dl, h_rows, a_mn=True, b_mn=True, out=dw[s:s + n])
+                    K.gemm(dl, h_rows, a_mn=True, b_mn=True, out=dw[s:s + n], rows=there)
+        if need_h and place is not None:
+            return K.scatter_rows(dh, place), dw, None, None
         if not need_h or (step >= V and rows == T):
             return dh, dw, None, None
         dh16 = torch.empty(T, H, dtype=BF16, device=h2.device)
@@ -1052,7 +1064,8 @@ class B200LinearLogprobs(_B200Op):
             out = LinearLogprobsFn.apply(_matrix(hidden), weight, flat, want_entropy)
             logp, ent = out if want_entropy else (out, None)
         else:
-            logp, _, ent = K.logprobs_fwd(_matrix(hidden), weight, flat, want_entropy)
+            h2 = _matrix(hidden)
+            logp, _, ent, _ = K.logprobs_fwd(h2, weight, flat, want_entropy, LinearLogprobsFn.compact(h2, weight, want_entropy))
         if targets.dim() == 1:
             return logp, ent
         return logp.view(targets.shape), ent.view(targets.shape) if want_entropy else None
