@@ -84,7 +84,7 @@ def test_larger(T, H, V):
     _check(*_case(T, H, V), True, True)
 
 
-@pytest.mark.parametrize("T, share", [(257, 0.0), (300, 0.4), (700, 0.97), (520, 1.0), (1100, 0.5)])
+@pytest.mark.parametrize("T, share", [(513, 0.0), (600, 0.4), (700, 0.97), (520, 1.0), (1100, 0.5)])
 @pytest.mark.parametrize("pieces", [1, 3])
 def test_rows_without_a_target_are_left_out(monkeypatch, T, share, pieces):
     """Wide vocabularies: prompts and padding are not computed.  None, some, nearly all and all of the rows; not a number in them stays there."""

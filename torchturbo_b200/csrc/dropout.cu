@@ -1,4 +1,5 @@
-// Dropout whose mask is drawn again wherever it is needed (philox.cuh), by itself and in the backward of a biased projection.
+// Dropout whose mask is drawn again wherever it is needed (philox.cuh), by itself and in the backward of a biased projection.  What bounds
+// them is memory and, nearly as much, the draws: 16384 x 4096 bf16 54 us (a copy 45), with a residual 64 (61.5 at the rate of a copy).
 #include <algorithm>
 
 #include "act.cuh"
@@ -114,7 +115,8 @@ dropout_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* __res
 }
 
 // The same for rows of any width: eight values in a row of memory belong to two or three groups, so a block draws what its 2048 values
-// need once and parks it (C = 1: every value has a group of its own).
+// need once and parks it (C = 1: every value has a group of its own).  Bound by the draws, twenty products each, and the exchange: 4097 x 1003
+// fp32 10 us (5 at the rate of a copy), 16000 x 4001 bf16 96 (39; one half of a word read at a time 117).
 constexpr int FLAT = 2048;
 template <typename T>
 __global__ void __launch_bounds__(256)
@@ -203,7 +205,10 @@ dropout_flat_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* 
 }
 
 // Backward of C = residual + dropout(act(z)):  dz = dropout(dy) act'(z), and its column sums (partial ones per block of rows, reduced by
-// colsum_kernel).  `dz` is null where it is dy itself.  Two rows at a time, the next two's loads ahead of their arithmetic.
+// colsum_kernel).  `dz` is null where it is dy itself.  Two rows at a time, the next two's loads ahead of their arithmetic; blocks of 256
+// threads over 2048 columns, three an SM (blocks as wide as the row, one an SM, had 40 % of the warps and took 159 us for the first
+// of these).  8192 x 12288, GELU (erf), dropout and bias 144 us; without dropout 99, without the activation 89 (604, 604 and 403 MB: 92 and
+// 62 us at the rate of a copy): the arithmetic of erf and of the draws next to each other is the bound of the first.
 template <int ACT, bool DROP, bool SUM, typename Keys>
 __global__ void __launch_bounds__(256, 3)
 tail_bwd_kernel(const __nv_bfloat16* __restrict__ dy, const __nv_bfloat16* __restrict__ z, __nv_bfloat16* __restrict__ dz,

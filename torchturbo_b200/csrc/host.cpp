@@ -320,8 +320,8 @@ GemmArgs product(const Tensor& a, const Tensor& b) {
 }
 
 // Whether a linear layer's rows are so few that streaming the weight past them beats tiles of 128 rows, most of them empty.  Times in us,
-// rows kernel and tiles, weights from memory: 1 row 1152 x 1152 3.5 and 8.6, 4096 x 4096 8.0 and 22, 4096 -> 12288 20 and 38; 4 rows 3.9
-// and 8.7, 12 and 19, 28 and 34; 8 rows 6.4 and 8.6, 19 and 18, 46 and 34.
+// rows kernel and tiles, weights from memory: 1 row 1152 x 1152 3.0 and 8.0, 4096 x 4096 8.0 and 16, 4096 -> 12288 19 and 26; 4 rows 3.5
+// and 8.0, 12 and 16, 27 and 26; 8 rows 6.0 and 8.0, 19 and 16, 46 and 26.
 bool few_rows(const GemmArgs& g) { return g.M <= 4 || (g.M <= 8 && static_cast<long long>(g.N) * g.K <= (1 << 23)); }
 
 PyObject* linear_tail(PyObject*, PyObject* const* args, Py_ssize_t n) {

@@ -9,7 +9,8 @@
 namespace ttb {
 
 // Eight rows a block (a sector of neighbouring rows), the pieces dealt out to its 128 groups of eight lanes and joined in a fixed order,
-// four at a time under one largest: 1462 pieces are three rounds of loads.
+// four at a time under one largest: 1462 pieces are three rounds of loads.  Bound by latency: 61 rows of 1462 pieces 6 us (one warp's lanes
+// over 32 rows and a piece at a time: 29), 4096 rows of 1188 27 us of 39 MB, a sixtieth of the product before it.
 constexpr int JOIN_ROWS = 8, JOIN_GROUPS = 128;
 
 __global__ void __launch_bounds__(JOIN_ROWS * JOIN_GROUPS)
@@ -73,7 +74,7 @@ logprobs_join_kernel(const float* __restrict__ part, const float* __restrict__ t
 namespace ttb {
 
 // Rows that have a target: their places in order, the places' inverse (-1 for the others) and their targets; the others' log-probability is
-// zero.  One block: 4096 rows a step, their places by a sum over the threads before.
+// zero.  One block: 4096 rows a step, their places by a sum over the threads before; 4096 rows 8.5 us, 8 for copying 3686 of 2048 values.
 __global__ void __launch_bounds__(1024)
 rows_with_targets_kernel(const long long* __restrict__ targets, long long T, long long V, int* __restrict__ rows, int* __restrict__ place,
                          long long* __restrict__ row_targets, int* __restrict__ count, float* __restrict__ logp) {
