@@ -214,6 +214,25 @@ def test_rows_that_are_not_finite_stay_by_themselves():
     assert (logp[[7, 9]] == 0).all() and (dh[[7, 9]] == 0).all() and torch.isfinite(dh).all()
 
 
+@pytest.mark.parametrize("T", [5, 300])
+def test_tokens_that_a_head_rules_out(T):
+    """Logits of minus infinity, over whole tiles and inside of one: as if their tokens were not there."""
+    from torchturbo_b200.ops import ops
+
+    h, w, t = _case(T, 64, 1100)
+    h[:, 0] = 1.0
+    t[:] = torch.randint(0, 20, (T,), device="cuda")
+    ruled = torch.zeros(1100, dtype=torch.bool, device="cuda")
+    ruled[30:40] = ruled[200:1090] = True
+    want, _ = ops.linear_logprobs(h, w[~ruled].contiguous(), t)
+    w[ruled, 0] = float("-inf")
+    got, _ = ops.linear_logprobs(h, w, t)
+    # the same sums in other pieces: 2^-24 of the log-sum-exp for each of at most twelve roundings on each side
+    assert ((got - want).abs() <= 24 * 2.0 ** -24 * (want.abs() + 12)).all()
+    t[0] = 35
+    assert ops.linear_logprobs(h, w, t)[0][0] == float("-inf")
+
+
 def test_layouts_and_gradients_wanted_of_some():
     from torchturbo_b200.ops import ops
 

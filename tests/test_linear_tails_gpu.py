@@ -236,6 +236,22 @@ def test_captured_step_draws_by_its_seed():
         assert all(torch.equal(a, b) for a, b in zip(got, ref))
 
 
+@pytest.mark.parametrize("M, K", [(3, 64), (130, 64), (5, 4104)])
+@pytest.mark.parametrize("act", [None, "gelu", "gelu_tanh"])
+def test_columns_that_are_not_finite(M, K, act):
+    from torchturbo_b200.ops import ops
+
+    gen = torch.Generator().manual_seed(15)
+    x, w, b = _rand(gen, M, K, std=0.1), _rand(gen, 72, K, std=0.1), _rand(gen, 72)
+    want = ops.linear_bias_act(x, w, b, act)
+    b[3], b[5] = float("inf"), float("nan")
+    y = ops.linear_bias_act(x, w, b, act)
+    rest = [i for i in range(72) if i not in (3, 5)]
+    assert torch.equal(y[:, rest], want[:, rest]) and (y[:, 3] == float("inf")).all() and y[:, 5].isnan().all()
+    y = ops.linear_bias_act(x, w, b, act, dropout_p=0.5, seed=1)
+    assert ((y[:, 3] == float("inf")) | (y[:, 3] == 0)).all() and ((y[:, 5] == 0) == (y[:, 5] == y[:, 5])).all()
+
+
 def test_result_may_be_changed_in_place():
     """The kept pre-activations are no view of the result."""
     from torchturbo_b200.ops import ops
@@ -258,7 +274,7 @@ def test_refusals():
                  lambda: ops.linear_bias_act(x, w, torch.ones(24, 1, **bf)), lambda: ops.linear_bias_act(x, w, act="relu6"),
                  lambda: ops.linear_bias_act(x, w, residual=torch.ones(24, **bf)), lambda: ops.linear_bias_act(x, w, residual=torch.ones(1, 24, **bf)),
                  lambda: ops.linear_bias_act(x, w, residual=torch.ones(6, 16, **bf)), lambda: ops.linear_bias_act(x.view(2, 3, 16), w, residual=torch.ones(6, 24, **bf)),
-                 lambda: ops.linear_bias_act(x, w.cpu()), lambda: ops.linear_bias_act(x, w, dropout_p=1.5), lambda: ops.linear_bias_act(x, w, dropout_p=0.1, seed=-1)):
+                 lambda: ops.linear_bias_act(x[0, 0], w), lambda: ops.linear_bias_act(x, w.cpu()), lambda: ops.linear_bias_act(x, w, dropout_p=1.5), lambda: ops.linear_bias_act(x, w, dropout_p=0.1, seed=-1)):
         with pytest.raises(ValueError):
             call()
 

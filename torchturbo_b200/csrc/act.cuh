@@ -67,10 +67,11 @@ __device__ __forceinline__ void act_pair(float& a, float& b) {
     f2_unpack(f2_mul(v, f2_fma(f2_mul(v, v), f2_both(0.035677408136300125f), f2_both(0.7978845608028654f))), ua, ub);
     f2_unpack(f2_fma(h, f2_pack(tanh_approx(ua), tanh_approx(ub)), h), a, b);
   } else if (ACT == 2) {
-    // v Phi(v) = max(v, 0) - |v| (1 - Phi(|v|))
+    // v Phi(v) = max(v, 0) - |v| (1 - Phi(|v|)); the second term of infinity is none
     uint64_t upper, expo;
     gelu_erf_parts(a, b, upper, expo);
-    f2_unpack(f2_fma(f2_pack(-fabsf(a), -fabsf(b)), upper, f2_pack(fmaxf(a, 0.f), fmaxf(b, 0.f))), a, b);
+    const float big = 3e38f;
+    f2_unpack(f2_fma(f2_pack(-fabsf(fminf(a, big)), -fabsf(fminf(b, big))), upper, f2_pack(fmaxf(a, 0.f), fmaxf(b, 0.f))), a, b);
   }
 }
 // (a, b) -> act'(a), act'(b)

@@ -220,8 +220,7 @@ __device__ __forceinline__ void tail_stats(const GemmParams& p, const TailRow<EP
   float big = fmaxf(l[0], l[1]);
 #pragma unroll
   for (int i = 2; i < BN / 2; i += 2) big = fmax3(big, l[i], l[i + 1]);
-  const bool any = cols > 0;                    // of nothing: a weight of zero
-  const float m = any ? big * LOG2E : -1e30f;
+  const float m = fmaxf(big * LOG2E, -1e30f);   // of no columns, or where all are -infinity: a sum of zero
   float s0 = 0.f, s1 = 0.f, w0 = 0.f, w1 = 0.f;
   const uint64_t log2e = f2_pack(LOG2E, LOG2E), down = f2_pack(-m, -m);
   auto pass = [&](bool entropy) {
@@ -240,8 +239,8 @@ __device__ __forceinline__ void tail_stats(const GemmParams& p, const TailRow<EP
     const long long slots = 2ll * p.n_tiles, plane = slots * p.M;
     float* dst = q.part + slot * static_cast<long long>(p.M) + row;
     dst[0] = m;
-    dst[plane] = any ? s0 + s1 : 0.f;
-    if (q.entropy) dst[2 * plane] = any ? w0 + w1 : 0.f;
+    dst[plane] = s0 + s1;
+    if (q.entropy) dst[2 * plane] = w0 + w1;
   }
 }
 

@@ -452,7 +452,7 @@ PyObject* dropout(PyObject*, PyObject* const* args, Py_ssize_t n) {
     need(x.dim() == 2 && (is_bf16(x) || x.scalar_type() == at::kFloat), "bf16 or fp32 rows");
     need(!residual.defined() || (residual.scalar_type() == x.scalar_type() && residual.sizes() == x.sizes() && residual.device() == x.device()),
          "the residual has the type and shape of the rows");
-    need(x.size(1) < (1ll << 31) - 8, "rows of fewer than 2^31 values");
+    need(x.size(1) < (1ll << 31) - 4096, "rows of fewer than 2^31 - 4096 values");
     const Tensor y = empty_rows(x);
     if (x.numel())
       launch("ttb_dropout", 1, [&](void* st) {

@@ -430,7 +430,7 @@ class B200LinearBiasAct(_B200Op):
 
     def __call__(self, x, weight, bias=None, act=None, *, residual=None, dropout_p=0.0, seed=None, first_row=0):
         drop = dropout_args(dropout_p, seed, first_row)
-        if not _ok(x, weight, bias, residual) or act not in K.ACT or weight.dim() != 2 or weight.shape[0] % 8 or weight.shape[1] % 8 or not weight.numel() \
+        if not _ok(x, weight, bias, residual) or act not in K.ACT or weight.dim() != 2 or x.dim() == 0 or weight.shape[0] % 8 or weight.shape[1] % 8 or not weight.numel() \
                 or drop.t > 65535 or _traced(x, weight, bias, residual):
             N.check_linear_bias_act(x, weight, bias, act, residual)
             return N.linear_bias_act_ref(x, weight, bias, act, residual, drop)
