@@ -122,6 +122,31 @@ def test_long_sums_in_pieces(M, N, K, act, p):
     assert Kn.status() == (0, 0)
 
 
+@pytest.mark.parametrize("K", [8, 16, 24, 32, 40, 64])
+@pytest.mark.parametrize("M, N", [(2, 8), (31, 256), (33, 264), (9511, 24), (5000, 1032), (700, 4104)])
+def test_few_features(M, N, K):
+    """Adapters: the backward walks the gradient once, in shares of rows that end inside a step and blocks of columns that are cut."""
+    from torchturbo_b200 import kernels as Kn
+
+    gen = torch.Generator().manual_seed(M + N + K)
+    for act, p, biased in (("gelu", 0.3, True), (None, 0.0, False), (None, 0.05, False), ("gelu_tanh", 0.0, True)):
+        _check(_rand(gen, M, K), _rand(gen, N, K), _rand(gen, N) if biased else None, _rand(gen, M, N), act, p, 5, _rand(gen, M, N), first_row=2 ** 32 - 40)
+    assert Kn.status() == (0, 0)
+
+
+def test_few_features_of_wider_rows():
+    """Inputs and weights that are parts of wider matrices, and a seed in memory."""
+    from torchturbo_b200.ops import ops
+
+    gen = torch.Generator().manual_seed(16)
+    x, w, dy = _rand(gen, 90, 48), _rand(gen, 520, 72), _rand(gen, 90, 520)
+    got = []
+    for xs, ws, seed in ((x[:, 8:32], w[:, 16:40], torch.tensor([9], device="cuda")), (x[:, 8:32].clone(), w[:, 16:40].clone(), 9)):
+        leaves = [xs.detach().requires_grad_(), ws.detach().requires_grad_()]
+        got.append(torch.autograd.grad(ops.linear_bias_act(*leaves, act="gelu", dropout_p=0.3, seed=seed), leaves, dy))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
 @pytest.mark.parametrize("M", [1, 2, 3, 4, 5, 6, 7, 8])
 @pytest.mark.parametrize("N, K", [(8, 8), (24, 264), (2376, 520), (1200, 1032), (4744, 256), (72, 4104)])
 def test_few_rows(M, N, K):

@@ -437,6 +437,14 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   return d;
 }
 
+// A load that stays where it is written, under way while something else is waited for: the compiler otherwise moves the unpacking of what
+// it brings up to it, and the thread waits there
+__device__ __forceinline__ uint4 load16_here(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

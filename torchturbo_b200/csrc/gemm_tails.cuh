@@ -30,12 +30,6 @@ __device__ __forceinline__ void add8(float (&f)[8], const uint4& u) {
 __device__ __forceinline__ void add_bias8(float (&f)[8], const __nv_bfloat16* bias, int col) {
   if (bias) add8(f, __ldg(reinterpret_cast<const uint4*>(bias + col)));
 }
-// a load that stays where it is written: it has to be under way while the products are waited for
-__device__ __forceinline__ uint4 load16_here(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
 // What an epilogue thread reads of its row (one row a thread) before the accumulator is there
 template <int EPI>
 struct TailRow {

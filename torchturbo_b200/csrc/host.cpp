@@ -147,6 +147,7 @@ PyObject* wrap_all(const Ts&... ts) {
 Tensor rows2d(const Tensor& t) { return t.dim() == 2 ? t.contiguous() : t.reshape({-1, t.size(-1)}).contiguous(); }
 Tensor like_shape(const Tensor& t2, const Tensor& x) { return x.dim() == 2 ? t2 : t2.view(x.sizes()); }
 int tail_row_blocks(long long rows, long long cols, int num_sms) { return ttb_tail_row_blocks(rows, static_cast<int>(cols), num_sms); }
+int narrow_parts(long long rows, int cols, int features, int num_sms, long long* parts) { return ttb_linear_narrow_parts(rows, cols, features, num_sms, parts); }
 int logprobs_slots(const GemmArgs& g, int* tile_cols) { return ttb_logprobs_slots(g.M, g.N, g.K, g.num_sms, tile_cols); }
 int kda_gate_row_blocks(long long rows, int heads) { return ttb_kda_gate_row_blocks(rows, heads); }
 int row_blocks(long long rows, const Tensor& t) { return static_cast<int>(std::max<long long>(1, std::min<long long>(rows, 2 * sms(t)))); }
@@ -425,6 +426,32 @@ Tensor backward_product(const Tensor& a, const Tensor& b, bool a_mn) {
   return out;
 }
 
+// Whether the backward walks the gradient once for all that is wanted of it (linear_narrow.cu): up to 16 input features, or up to 64 of a
+// gradient so small that launches are what its time is.  us, a walk with its sums and separate passes: 8190 x 16 -> 4096 24 and 37, with dropout
+// 43 and 63, with GELU (erf) and dropout 67 and 83; 32 features 42 and 36, 62 and 62, 95 and 81; 64 features 61 and 34, but 300 rows 11 and 16,
+// with dropout 13 and 19.
+bool narrow(const Tensor& dy, const Tensor& x) {
+  const long long K = x.size(1);
+  return K > 0 && (K <= 16 || (K <= 64 && dy.numel() <= (1ll << 21))) && dy.numel() > 0 && dy.size(0) < (1ll << 30);
+}
+PyObject* narrow_bwd(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& z, int act, const Dropout& d, bool want_db, bool f32out) {
+  check_device(dy);
+  need(is_bf16(dy) && dy.dim() == 2 && dy.is_contiguous() && on_16_bytes(dy) && dy.size(1) % 8 == 0 && x.size(1) % 8 == 0 && w.size(1) == x.size(1),
+       "gradients: bf16 rows without gaps, widths are multiples of eight");
+  need(!z.defined() || (is_bf16(z) && z.is_contiguous() && z.sizes() == dy.sizes() && z.device() == dy.device()), "pre-activations: bf16 rows without gaps");
+  const long long R = dy.size(0);
+  const int C = static_cast<int>(dy.size(1)), K = static_cast<int>(x.size(1)), num_sms = sms(dy);
+  const Tensor dx = empty({R, K}, at::kBFloat16, dy), dw = empty({C, K}, at::kBFloat16, dy), db = want_db ? empty({C}, out_type(f32out), dy) : Tensor();
+  long long values = 0;
+  narrow_parts(R, C, K, num_sms, &values);
+  const Tensor parts = empty({values}, at::kFloat, dy);
+  launch("ttb_linear_narrow_bwd", 2, [&](void* st) {
+    return ttb_linear_narrow_bwd(at_(dy), at_(z), at_(x), x.stride(0), at_(w), w.stride(0), to_(dx), to_(dw), to_(db), !f32out, f32w(parts), R, C, K, act, d.t,
+                                 d.scale, d.seed, d.dev(), d.first_row, num_sms, st);
+  });
+  return wrap_all(dx, dw, db);
+}
+
 // (dx, dw, db) of linear_tail, in one call: the three are four launches
 PyObject* linear_tail_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
@@ -436,6 +463,7 @@ PyObject* linear_tail_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     need((!need_x || (w.defined() && is_bf16(w) && w.dim() == 2 && w.size(0) == dy.size(1) && w.device() == dy.device())) &&
              (!need_w || (x.defined() && is_bf16(x) && x.dim() == 2 && x.size(0) == dy.size(0) && x.device() == dy.device())),
          "operands of the backward: bf16 matrices that fit the gradient");
+    if (need_x && need_w && narrow(dy, x)) return narrow_bwd(dy, x, w, z, act, d, want_db, f32out);
     Tensor dz, db;
     tail_gradient(dy, z, act, d, want_db, f32out, dz, db);
     const Tensor dx = need_x ? backward_product(dz, w, false) : Tensor(), dw = need_w ? backward_product(dz, x, true) : Tensor();

@@ -1,0 +1,363 @@
+// Backward of a biased linear layer with a few input features (an adapter's up-projection),  C = residual + dropout(act(z)),  z = x W^T + bias:
+//   dz = dropout(dC) act'(z),   dx = dz W,   dW = dz^T x,   db = column sums of dz
+// in one walk over dC (and z).  What a row of C holds outweighs what one of x holds a hundred times, so reading dC and z is what it costs:
+// dz never leaves the block, as two products that read it again would have it.
+//
+// A block owns 256 columns and a share of the rows.  Its threads form dz for 32 rows at a time, the next 32 rows' loads under way, and park it
+// in bf16, from where it is an operand of both products: of dx as it lies (every step's sum over the block's columns goes to memory), of
+// dW transposed (summed over the block's rows in registers).  Sums over blocks of columns, and over shares of rows, are added up by
+// linear_narrow_sum_kernel in a fixed order.  The products are 32 x 64 and 256 x 64 wide at most and hidden under the loads and draws, so they are
+// mma.sync from registers: an accumulator in TMEM would have to be read back at every step.
+#include <algorithm>
+
+#include "act.cuh"
+#include "philox.cuh"
+#include "rowops.cuh"
+
+namespace ttb {
+
+struct NarrowParams {
+  const __nv_bfloat16 *dy, *z, *x, *w;
+  long long ldx, ldw;
+  float *dx, *dw, *db;         // [column blocks, R, K], [shares, C, K], [shares, C] or null
+  long long R;
+  int C, K, steps;             // steps of 32 rows in a share
+  DropoutParams drop;
+};
+constexpr int NB_COLS = 256, NB_ROWS = 32, NB_LD = NB_COLS + 8;      // rows of the parked dz 528 bytes apart: eight of them lie on distinct banks
+
+template <int KT>
+struct NarrowSmem {
+  static constexpr int LD = KT + 8;                                  // of x and W, and (in floats) of the sums
+  static constexpr int RING = KT <= 16 ? 2 : 3;                      // steps: one at work, the others' loads under way
+  static constexpr int TILE = NB_ROWS * NB_LD * 2, X = NB_ROWS * LD * 2, W = NB_COLS * LD * 2, RED = 4 * NB_ROWS * LD * 4;
+  static constexpr int TOTAL = RING * (TILE + X) + W + 2 * RED;
+  static constexpr int PER_SM = KT <= 16 ? 3 : KT <= 32 ? 2 : 1;     // blocks
+};
+
+__device__ __forceinline__ void nb_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void nb_ldm(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void nb_ldm_t(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+
+// 16 bytes that the copying thread may read after its own wait, others after a barrier as well; zeros in place of what is not there
+__device__ __forceinline__ void nb_copy(uint32_t to, const void* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void nb_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void nb_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// KT: K rounded up to 16, 32 or 64
+template <int KT, int ACT, bool DROP, typename Keys>
+__global__ void __launch_bounds__(256, NarrowSmem<KT>::PER_SM) linear_narrow_bwd_kernel(const NarrowParams p) {
+  using S = NarrowSmem<KT>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  uint8_t *tile = smem, *xs = tile + S::RING * S::TILE, *ws = xs + S::RING * S::X;
+  float* red = reinterpret_cast<float*>(ws + S::W);
+  constexpr int RED = S::RED / 4, NT = KT / 8, AHEAD = S::RING - 1;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int c0 = blockIdx.x * NB_COLS, g = blockIdx.x * (NB_COLS / 8) + lane;      // this thread's eight columns
+  const bool live = 8 * g < p.C;
+  const long long first = static_cast<long long>(blockIdx.y) * p.steps * NB_ROWS;
+  const long long last = first + static_cast<long long>(p.steps) * NB_ROWS < p.R ? first + static_cast<long long>(p.steps) * NB_ROWS : p.R;
+  const int xr = tid / NT, xk = tid % NT * 8;      // the eight values of x that this thread brings
+  const int mt = warp & 1, quarter = warp >> 1;    // its warp's share of dx: 16 rows, 64 columns
+
+  // copies run AHEAD steps before their use
+  const __nv_bfloat16 *from = p.dy + (live ? (first + warp) * p.C + 8 * g : 0), *from_x = p.x + (first + xr) * p.ldx + xk;
+  const long long apart = 8ll * p.C, step_x = NB_ROWS * p.ldx;
+  int left = static_cast<int>(last - first);      // rows from the next copied step on
+  const uint32_t to = smem_u32(tile) + (warp * NB_LD + 8 * lane) * 2, to_x = smem_u32(xs) + (xr * S::LD + xk) * 2;
+  auto copy = [&](int b) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool there = live && warp + 8 * i < left;
+      nb_copy(to + b * S::TILE + 8 * i * NB_LD * 2, there ? from + i * apart : p.dy, there);
+    }
+    if (tid < NB_ROWS * NT) {
+      const bool there = xk < p.K && xr < left;
+      nb_copy(to_x + b * S::X, there ? from_x : p.x, there);
+    }
+    from += 4 * apart;
+    from_x += step_x;
+    left -= NB_ROWS;
+  };
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j) {
+    copy(j);
+    nb_commit();
+  }
+  // W of these columns, zeros behind its edges, as the operand that a warp's share of dx takes
+  for (int i = tid; i < NB_COLS * NT; i += 256) {
+    const int c = i / NT, k = i % NT * 8;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (c0 + c < p.C && k < p.K) v = *reinterpret_cast<const uint4*>(p.w + static_cast<long long>(c0 + c) * p.ldw + k);
+    *reinterpret_cast<uint4*>(ws + (c * S::LD + k) * 2) = v;
+  }
+  const Keys key(p.drop);
+  uint32_t high = 0;
+  PhiloxColumn col{};
+  if (DROP) {
+    high = static_cast<uint32_t>(static_cast<uint64_t>(p.drop.first_row + first) >> 32);
+    col = philox_column(g, high, key);
+  }
+  uint4 zn[ACT ? 4 : 1];
+  auto load_z = [&](long long r0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const long long r = r0 + warp + 8 * i;
+      zn[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (live && r < last) zn[i] = load16_here(p.z + r * p.C + 8 * g);
+    }
+  };
+  if constexpr (ACT != 0) load_z(first);
+
+  float db[8] = {}, dw[2][NT][4] = {};
+  int buf = 0, half = 0;
+  bool parked = false;
+  auto sums_out = [&](long long r0, int b) {
+    for (int e = tid; e < NB_ROWS * KT; e += 256) {
+      const int r = e / KT, k = e % KT;
+      if (k < p.K && r0 + r < last) {
+        const float* src = red + b * RED + r * S::LD + k;
+        constexpr int Q = NB_ROWS * S::LD;
+        p.dx[(static_cast<long long>(blockIdx.x) * p.R + r0 + r) * p.K + k] = (src[0] + src[Q]) + (src[2 * Q] + src[3 * Q]);
+      }
+    }
+  };
+  for (long long r0 = first; r0 < last; r0 += NB_ROWS) {
+    const uint32_t at = smem_u32(tile + buf * S::TILE), at_x = smem_u32(xs + buf * S::X);
+    nb_wait<AHEAD - 1>();
+    // ---- dz of 32 rows, each thread in place of what it copied
+    if (DROP || ACT || p.db) {
+      uint4 zu[ACT ? 4 : 1];
+      if constexpr (ACT != 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) zu[i] = zn[i];
+        load_z(r0 + NB_ROWS);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const long long r = r0 + warp + 8 * i;
+        uint4* mine = reinterpret_cast<uint4*>(tile + buf * S::TILE + ((warp + 8 * i) * NB_LD + 8 * lane) * 2);
+        const uint4 du = *mine;
+        float f[8];
+        const uint32_t dv[4] = {du.x, du.y, du.z, du.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[2 * j] = __uint_as_float(dv[j] << 16);
+          f[2 * j + 1] = __uint_as_float(dv[j] & 0xffff0000u);
+        }
+        if (DROP) {
+          const uint64_t whole = static_cast<uint64_t>(p.drop.first_row + r);
+          if (static_cast<uint32_t>(whole >> 32) != high) {
+            high = static_cast<uint32_t>(whole >> 32);
+            col = philox_column(g, high, key);
+          }
+          dropout8(f, philox(col, philox_row(static_cast<uint32_t>(whole), key), key), p.drop.t << 16, p.drop.scale);
+        }
+        if (ACT) {
+          const uint32_t zv[4] = {zu[i].x, zu[i].y, zu[i].z, zu[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float a = __uint_as_float(zv[j] << 16), b = __uint_as_float(zv[j] & 0xffff0000u);
+            act_slope_pair<ACT>(a, b);
+            f[2 * j] *= a;
+            f[2 * j + 1] *= b;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) db[j] += f[j];
+        if (DROP || ACT) *mine = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+      }
+    }
+    // One barrier a step: behind it everyone has done with the step before, whose place takes the copies of the step AHEAD of this one, and
+    // its parked sums are there
+    __syncthreads();
+    copy(buf == 0 ? AHEAD : buf - 1);
+    nb_commit();
+    if (parked) sums_out(r0 - NB_ROWS, half ^ 1);
+    parked = true;
+    // ---- dx: 16 rows x K over 64 columns a warp
+    float acc[NT][4] = {};
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      uint32_t a[4];
+      nb_ldm(a, at + ((16 * mt + (lane & 15)) * NB_LD + 64 * quarter + 16 * ks + (lane >> 4) * 8) * 2);
+#pragma unroll
+      for (int nt = 0; nt < NT; nt += 2) {
+        uint32_t b[4];
+        nb_ldm_t(b, smem_u32(ws) + ((64 * quarter + 16 * ks + (lane & 15)) * S::LD + 8 * nt + (lane >> 4) * 8) * 2);
+        nb_mma(acc[nt], a, b[0], b[1]);
+        nb_mma(acc[nt + 1], a, b[2], b[3]);
+      }
+    }
+    float* out = red + half * RED + (quarter * NB_ROWS + 16 * mt + (lane >> 2)) * S::LD + 2 * (lane & 3);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      *reinterpret_cast<float2*>(out + 8 * nt) = make_float2(acc[nt][0], acc[nt][1]);
+      *reinterpret_cast<float2*>(out + 8 * S::LD + 8 * nt) = make_float2(acc[nt][2], acc[nt][3]);
+    }
+    // ---- dW: 32 columns x K over 32 rows a warp
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      uint32_t a[2][4];
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+        nb_ldm_t(a[m], at + ((16 * ks + (lane & 7) + (lane >> 4) * 8) * NB_LD + 32 * warp + 16 * m + ((lane >> 3) & 1) * 8) * 2);
+#pragma unroll
+      for (int nt = 0; nt < NT; nt += 2) {
+        uint32_t b[4];
+        nb_ldm_t(b, at_x + ((16 * ks + (lane & 15)) * S::LD + 8 * nt + (lane >> 4) * 8) * 2);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          nb_mma(dw[m][nt], a[m], b[0], b[1]);
+          nb_mma(dw[m][nt + 1], a[m], b[2], b[3]);
+        }
+      }
+    }
+    buf = buf == AHEAD ? 0 : buf + 1;
+    half ^= 1;
+  }
+  nb_wait<0>();
+  __syncthreads();
+  if (parked) sums_out(first + (last - first - 1) / NB_ROWS * NB_ROWS, half ^ 1);
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int c = c0 + 32 * warp + 16 * m + (lane >> 2) + 8 * h, k = 8 * nt + 2 * (lane & 3);
+        if (c < p.C && k < p.K)
+          *reinterpret_cast<float2*>(p.dw + (static_cast<long long>(blockIdx.y) * p.C + c) * p.K + k) = make_float2(dw[m][nt][2 * h], dw[m][nt][2 * h + 1]);
+      }
+  if (!p.db) return;
+  // the eight warps' sums of a column, in order
+  __syncthreads();
+  float* part = red;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) part[warp * NB_COLS + 8 * lane + j] = db[j];
+  __syncthreads();
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += part[i * NB_COLS + tid];
+  if (c0 + tid < p.C) p.db[static_cast<long long>(blockIdx.y) * p.C + c0 + tid] = s;
+}
+
+struct NarrowSums {
+  const float *dx, *dw, *db;
+  __nv_bfloat16 *out_x, *out_w;
+  void* out_b;
+  int b_bf16, blocks, shares;
+  long long nx, nw, nb;      // pairs of values
+};
+__global__ void __launch_bounds__(256) linear_narrow_sum_kernel(const NarrowSums p) {
+  long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x;
+  const float* src;
+  long long n;
+  int parts, which;
+  if (i < p.nx) {
+    src = p.dx; n = p.nx; parts = p.blocks; which = 0;
+  } else if ((i -= p.nx) < p.nw) {
+    src = p.dw; n = p.nw; parts = p.shares; which = 1;
+  } else if ((i -= p.nw) < p.nb) {
+    src = p.db; n = p.nb; parts = p.shares; which = 2;
+  } else {
+    return;
+  }
+  float2 s = make_float2(0.f, 0.f);
+  const float2* at = reinterpret_cast<const float2*>(src) + i;
+  for (int j = 0; j < parts; j += 16, at += 16 * n) {      // sixteen loads under way
+    float2 v[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) v[u] = j + u < parts ? __ldg(at + u * n) : make_float2(0.f, 0.f);
+#pragma unroll
+    for (int u = 0; u < 16; ++u) {
+      s.x += v[u].x;
+      s.y += v[u].y;
+    }
+  }
+  const uint32_t u = pack_bf16(s.x, s.y);
+  if (which == 0) reinterpret_cast<uint32_t*>(p.out_x)[i] = u;
+  else if (which == 1) reinterpret_cast<uint32_t*>(p.out_w)[i] = u;
+  else if (p.b_bf16) reinterpret_cast<uint32_t*>(p.out_b)[i] = u;
+  else reinterpret_cast<float2*>(p.out_b)[i] = s;
+}
+
+// Blocks of columns, shares of rows (as many as the SMs hold) and steps of 32 rows in a share
+struct NarrowPlan {
+  int blocks, shares, steps;
+};
+static NarrowPlan narrow_plan(long long R, int C, int K, int sms) {
+  NarrowPlan q;
+  q.blocks = (C + NB_COLS - 1) / NB_COLS;
+  const int per_sm = K <= 16 ? NarrowSmem<16>::PER_SM : K <= 32 ? NarrowSmem<32>::PER_SM : NarrowSmem<64>::PER_SM;
+  const long long steps = (R + NB_ROWS - 1) / NB_ROWS, most = std::max<long long>(1, static_cast<long long>(per_sm) * sms / q.blocks);
+  q.steps = static_cast<int>((steps + std::min(most, steps) - 1) / std::min(most, steps));
+  q.shares = static_cast<int>((steps + q.steps - 1) / q.steps);
+  return q;
+}
+
+template <int KT, int ACT, bool DROP, typename Keys>
+static int narrow_launch(const NarrowParams& p, const NarrowPlan& q, cudaStream_t st) {
+  auto kernel = linear_narrow_bwd_kernel<KT, ACT, DROP, Keys>;
+  constexpr int smem = NarrowSmem<KT>::TOTAL;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return 300 + static_cast<int>(e);
+  kernel<<<dim3(q.blocks, q.shares), 256, smem, st>>>(p);
+  return 0;
+}
+template <int KT, int ACT>
+static int narrow_drop(const NarrowParams& p, const NarrowPlan& q, cudaStream_t st) {
+  if (!p.drop.t) return narrow_launch<KT, ACT, false, KeysOfLaunch>(p, q, st);
+  if (p.drop.seed_dev) return narrow_launch<KT, ACT, true, KeysOfSeed>(p, q, st);
+  return narrow_launch<KT, ACT, true, KeysOfLaunch>(p, q, st);
+}
+template <int KT>
+static int narrow_act(const NarrowParams& p, const NarrowPlan& q, int act, cudaStream_t st) {
+  if (act == 1) return narrow_drop<KT, 1>(p, q, st);
+  if (act == 2) return narrow_drop<KT, 2>(p, q, st);
+  return narrow_drop<KT, 0>(p, q, st);
+}
+
+}  // namespace ttb
+
+// fp32 values that ttb_linear_narrow_bwd keeps its partial sums in
+TTB_EXPORT int ttb_linear_narrow_parts(long long R, int C, int K, int sms, long long* parts) {
+  const ttb::NarrowPlan q = ttb::narrow_plan(R, C, K, sms);
+  *parts = q.blocks * R * K + static_cast<long long>(q.shares) * C * (K + 1);
+  return 0;
+}
+
+// dy, z: [R, C] bf16 without gaps; x: [R, K] and w: [C, K], rows ldx and ldw apart; all on 16-byte boundaries; C % 8 == 0, K % 8 == 0, K <= 64.
+// dx [R, K] and dw [C, K] bf16, db [C] (or null) bf16 or fp32
+TTB_EXPORT int ttb_linear_narrow_bwd(const void* dy, const void* z, const void* x, long long ldx, const void* w, long long ldw, void* dx, void* dw, void* db,
+                                     int db_bf16, float* parts, long long R, int C, int K, int act, unsigned t, float scale, unsigned long long seed,
+                                     const unsigned long long* seed_dev, long long first_row, int sms, void* stream) {
+  using namespace ttb;
+  if (C <= 0 || K <= 0 || C % 8 || K % 8 || K > 64 || ldx % 8 || ldw % 8 || act < 0 || act > 2 || (act && !z)) return 901;
+  if (t > 65535 || R <= 0 || R >= (1ll << 30)) return 903;
+  const NarrowPlan q = narrow_plan(R, C, K, sms);
+  if (q.shares > 65535) return 903;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  float *px = parts, *pw = px + q.blocks * R * K, *pb = pw + static_cast<long long>(q.shares) * C * K;
+  const NarrowParams p{static_cast<const __nv_bfloat16*>(dy), static_cast<const __nv_bfloat16*>(z), static_cast<const __nv_bfloat16*>(x),
+                       static_cast<const __nv_bfloat16*>(w), ldx, ldw, px, pw, db ? pb : nullptr, R, C, K, q.steps,
+                       dropout_params(t, scale, seed, seed_dev, first_row)};
+  const int r = K <= 16 ? narrow_act<16>(p, q, act, st) : K <= 32 ? narrow_act<32>(p, q, act, st) : narrow_act<64>(p, q, act, st);
+  if (r) return r;
+  const NarrowSums s{px, pw, pb, static_cast<__nv_bfloat16*>(dx), static_cast<__nv_bfloat16*>(dw), db, db_bf16, q.blocks, q.shares,
+                     R * K / 2, static_cast<long long>(C) * K / 2, db ? C / 2 : 0};
+  linear_narrow_sum_kernel<<<static_cast<unsigned>((s.nx + s.nw + s.nb + 255) / 256), 256, 0, st>>>(s);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 400 + static_cast<int>(e);
+}
