@@ -434,14 +434,17 @@ bool narrow(const Tensor& dy, const Tensor& x) {
   const long long K = x.size(1);
   return K > 0 && (K <= 16 || (K <= 64 && dy.numel() <= (1ll << 21))) && dy.numel() > 0 && dy.size(0) < (1ll << 30);
 }
-PyObject* narrow_bwd(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& z, int act, const Dropout& d, bool want_db, bool f32out) {
+PyObject* narrow_bwd(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& z, int act, const Dropout& d, bool need_x, bool need_w, bool want_db,
+                     bool f32out) {
   check_device(dy);
-  need(is_bf16(dy) && dy.dim() == 2 && dy.is_contiguous() && on_16_bytes(dy) && dy.size(1) % 8 == 0 && x.size(1) % 8 == 0 && w.size(1) == x.size(1),
+  need(is_bf16(dy) && dy.dim() == 2 && dy.is_contiguous() && on_16_bytes(dy) && dy.size(1) % 8 == 0 && is_bf16(x) && is_bf16(w) && x.size(1) % 8 == 0 &&
+           w.size(1) == x.size(1),
        "gradients: bf16 rows without gaps, widths are multiples of eight");
   need(!z.defined() || (is_bf16(z) && z.is_contiguous() && z.sizes() == dy.sizes() && z.device() == dy.device()), "pre-activations: bf16 rows without gaps");
   const long long R = dy.size(0);
   const int C = static_cast<int>(dy.size(1)), K = static_cast<int>(x.size(1)), num_sms = sms(dy);
-  const Tensor dx = empty({R, K}, at::kBFloat16, dy), dw = empty({C, K}, at::kBFloat16, dy), db = want_db ? empty({C}, out_type(f32out), dy) : Tensor();
+  const Tensor dx = need_x ? empty({R, K}, at::kBFloat16, dy) : Tensor(), dw = need_w ? empty({C, K}, at::kBFloat16, dy) : Tensor(),
+               db = want_db ? empty({C}, out_type(f32out), dy) : Tensor();
   long long values = 0;
   narrow_parts(R, C, K, num_sms, &values);
   const Tensor parts = empty({values}, at::kFloat, dy);
@@ -463,7 +466,8 @@ PyObject* linear_tail_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     need((!need_x || (w.defined() && is_bf16(w) && w.dim() == 2 && w.size(0) == dy.size(1) && w.device() == dy.device())) &&
              (!need_w || (x.defined() && is_bf16(x) && x.dim() == 2 && x.size(0) == dy.size(0) && x.device() == dy.device())),
          "operands of the backward: bf16 matrices that fit the gradient");
-    if (need_x && need_w && narrow(dy, x)) return narrow_bwd(dy, x, w, z, act, d, want_db, f32out);
+    if ((need_x || need_w || want_db) && x.defined() && w.defined() && narrow(dy, x))
+      return narrow_bwd(dy, x, w, z, act, d, need_x, need_w, want_db, f32out);
     Tensor dz, db;
     tail_gradient(dy, z, act, d, want_db, f32out, dz, db);
     const Tensor dx = need_x ? backward_product(dz, w, false) : Tensor(), dw = need_w ? backward_product(dz, x, true) : Tensor();

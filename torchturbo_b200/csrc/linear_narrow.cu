@@ -3,11 +3,17 @@
 // in one walk over dC (and z).  What a row of C holds outweighs what one of x holds a hundred times, so reading dC and z is what it costs:
 // dz never leaves the block, as two products that read it again would have it.
 //
-// A block owns 256 columns and a share of the rows.  Its threads form dz for 32 rows at a time, the next 32 rows' loads under way, and park it
-// in bf16, from where it is an operand of both products: of dx as it lies (every step's sum over the block's columns goes to memory), of
-// dW transposed (summed over the block's rows in registers).  Sums over blocks of columns, and over shares of rows, are added up by
-// linear_narrow_sum_kernel in a fixed order.  The products are 32 x 64 and 256 x 64 wide at most and hidden under the loads and draws, so they are
-// mma.sync from registers: an accumulator in TMEM would have to be read back at every step.
+// A block owns 256 columns and a share of the rows.  Its threads form dz for 32 rows at a time in place of what they copied there, the
+// next step's copy under way, and it is an operand of both products: of dx as it lies (every step's sum over the block's columns is
+// joined across the warps and goes to memory), of dW transposed (summed over the block's rows in registers).  Sums over blocks of columns,
+// and over shares of rows, are added up by linear_narrow_sum_kernel in a fixed order.  The products are 32 x 64 and 256 x 64 wide at most and
+// hidden under the loads and draws, so they are mma.sync: an accumulator in TMEM would have to be read back at every step.
+// Dropout's factor is left to the sums: without an activation dz is then dC with zeros in it, exact in bf16, and is never unpacked.
+//
+// 8190 x 16 -> 4096: 18 us and 5 for the sums (67 MB: 10 at the rate of a copy; three passes 37), with dropout 37 and 5 (63), with GELU (erf) too
+// 67 together (83).  The first is bound by the latency of a step (wait, barrier, products, joining) at three blocks an SM, the others
+// by the instructions of the draws and of the error function, 146 for eight values.  Two blocks an SM with three steps' copies under way 27 and
+// 46; dz kept in registers and transposed across the warp (movmatrix) 27 and 47.
 #include <algorithm>
 
 #include "act.cuh"
@@ -19,7 +25,7 @@ namespace ttb {
 struct NarrowParams {
   const __nv_bfloat16 *dy, *z, *x, *w;
   long long ldx, ldw;
-  float *dx, *dw, *db;         // [column blocks, R, K], [shares, C, K], [shares, C] or null
+  float *dx, *dw, *db;         // [column blocks, R, K], [shares, C, K], [shares, C]; null where not wanted
   long long R;
   int C, K, steps;             // steps of 32 rows in a share
   DropoutParams drop;
@@ -82,7 +88,7 @@ __global__ void __launch_bounds__(256, NarrowSmem<KT>::PER_SM) linear_narrow_bwd
       const bool there = live && warp + 8 * i < left;
       nb_copy(to + b * S::TILE + 8 * i * NB_LD * 2, there ? from + i * apart : p.dy, there);
     }
-    if (tid < NB_ROWS * NT) {
+    if (p.dw && tid < NB_ROWS * NT) {
       const bool there = xk < p.K && xr < left;
       nb_copy(to_x + b * S::X, there ? from_x : p.x, there);
     }
@@ -96,7 +102,7 @@ __global__ void __launch_bounds__(256, NarrowSmem<KT>::PER_SM) linear_narrow_bwd
     nb_commit();
   }
   // W of these columns, zeros behind its edges, as the operand that a warp's share of dx takes
-  for (int i = tid; i < NB_COLS * NT; i += 256) {
+  for (int i = tid; p.dx && i < NB_COLS * NT; i += 256) {
     const int c = i / NT, k = i % NT * 8;
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
     if (c0 + c < p.C && k < p.K) v = *reinterpret_cast<const uint4*>(p.w + static_cast<long long>(c0 + c) * p.ldw + k);
@@ -120,6 +126,9 @@ __global__ void __launch_bounds__(256, NarrowSmem<KT>::PER_SM) linear_narrow_bwd
   };
   if constexpr (ACT != 0) load_z(first);
 
+  const uint32_t top = p.drop.t << 16;
+  // what dropout leaves of two values, but for its factor, which the sums take
+  auto kept = [&](uint32_t two, uint32_t draws) { return ((draws << 16) >= top ? two & 0xffffu : 0u) | (draws >= top ? two & 0xffff0000u : 0u); };
   float db[8] = {}, dw[2][NT][4] = {};
   int buf = 0, half = 0;
   bool parked = false;
@@ -137,46 +146,49 @@ __global__ void __launch_bounds__(256, NarrowSmem<KT>::PER_SM) linear_narrow_bwd
     const uint32_t at = smem_u32(tile + buf * S::TILE), at_x = smem_u32(xs + buf * S::X);
     nb_wait<AHEAD - 1>();
     // ---- dz of 32 rows, each thread in place of what it copied
-    if (DROP || ACT || p.db) {
-      uint4 zu[ACT ? 4 : 1];
-      if constexpr (ACT != 0) {
+    uint4 zu[ACT ? 4 : 1];
+    if constexpr (ACT != 0) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) zu[i] = zn[i];
-        load_z(r0 + NB_ROWS);
-      }
+      for (int i = 0; i < 4; ++i) zu[i] = zn[i];
+      load_z(r0 + NB_ROWS);
+    }
+    if (DROP || ACT || p.db) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const long long r = r0 + warp + 8 * i;
         uint4* mine = reinterpret_cast<uint4*>(tile + buf * S::TILE + ((warp + 8 * i) * NB_LD + 8 * lane) * 2);
-        const uint4 du = *mine;
-        float f[8];
-        const uint32_t dv[4] = {du.x, du.y, du.z, du.w};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          f[2 * j] = __uint_as_float(dv[j] << 16);
-          f[2 * j + 1] = __uint_as_float(dv[j] & 0xffff0000u);
-        }
+        uint4 du = *mine;
         if (DROP) {
-          const uint64_t whole = static_cast<uint64_t>(p.drop.first_row + r);
+          const uint64_t whole = static_cast<uint64_t>(p.drop.first_row + r0 + warp + 8 * i);
           if (static_cast<uint32_t>(whole >> 32) != high) {
             high = static_cast<uint32_t>(whole >> 32);
             col = philox_column(g, high, key);
           }
-          dropout8(f, philox(col, philox_row(static_cast<uint32_t>(whole), key), key), p.drop.t << 16, p.drop.scale);
+          const uint4 u = philox(col, philox_row(static_cast<uint32_t>(whole), key), key);
+          du = make_uint4(kept(du.x, u.x), kept(du.y, u.y), kept(du.z, u.z), kept(du.w, u.w));
         }
-        if (ACT) {
-          const uint32_t zv[4] = {zu[i].x, zu[i].y, zu[i].z, zu[i].w};
+        if (ACT || p.db) {
+          float f[8];
+          const uint32_t dv[4] = {du.x, du.y, du.z, du.w};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float a = __uint_as_float(zv[j] << 16), b = __uint_as_float(zv[j] & 0xffff0000u);
-            act_slope_pair<ACT>(a, b);
-            f[2 * j] *= a;
-            f[2 * j + 1] *= b;
+            f[2 * j] = __uint_as_float(dv[j] << 16);
+            f[2 * j + 1] = __uint_as_float(dv[j] & 0xffff0000u);
           }
-        }
+          if (ACT) {
+            const uint32_t zv[4] = {zu[i].x, zu[i].y, zu[i].z, zu[i].w};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) db[j] += f[j];
-        if (DROP || ACT) *mine = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+            for (int j = 0; j < 4; ++j) {
+              float a = __uint_as_float(zv[j] << 16), b = __uint_as_float(zv[j] & 0xffff0000u);
+              act_slope_pair<ACT>(a, b);
+              f[2 * j] *= a;
+              f[2 * j + 1] *= b;
+            }
+            du = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) db[j] += f[j];
+        }
+        if (DROP || ACT) *mine = du;
       }
     }
     // One barrier a step: behind it everyone has done with the step before, whose place takes the copies of the step AHEAD of this one, and
@@ -184,43 +196,47 @@ __global__ void __launch_bounds__(256, NarrowSmem<KT>::PER_SM) linear_narrow_bwd
     __syncthreads();
     copy(buf == 0 ? AHEAD : buf - 1);
     nb_commit();
-    if (parked) sums_out(r0 - NB_ROWS, half ^ 1);
+    if (parked && p.dx) sums_out(r0 - NB_ROWS, half ^ 1);
     parked = true;
     // ---- dx: 16 rows x K over 64 columns a warp
-    float acc[NT][4] = {};
+    if (p.dx) {
+      float acc[NT][4] = {};
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      uint32_t a[4];
-      nb_ldm(a, at + ((16 * mt + (lane & 15)) * NB_LD + 64 * quarter + 16 * ks + (lane >> 4) * 8) * 2);
+      for (int ks = 0; ks < 4; ++ks) {
+        uint32_t a[4];
+        nb_ldm(a, at + ((16 * mt + (lane & 15)) * NB_LD + 64 * quarter + 16 * ks + (lane >> 4) * 8) * 2);
 #pragma unroll
-      for (int nt = 0; nt < NT; nt += 2) {
-        uint32_t b[4];
-        nb_ldm_t(b, smem_u32(ws) + ((64 * quarter + 16 * ks + (lane & 15)) * S::LD + 8 * nt + (lane >> 4) * 8) * 2);
-        nb_mma(acc[nt], a, b[0], b[1]);
-        nb_mma(acc[nt + 1], a, b[2], b[3]);
+        for (int nt = 0; nt < NT; nt += 2) {
+          uint32_t b[4];
+          nb_ldm_t(b, smem_u32(ws) + ((64 * quarter + 16 * ks + (lane & 15)) * S::LD + 8 * nt + (lane >> 4) * 8) * 2);
+          nb_mma(acc[nt], a, b[0], b[1]);
+          nb_mma(acc[nt + 1], a, b[2], b[3]);
+        }
+      }
+      float* out = red + half * RED + (quarter * NB_ROWS + 16 * mt + (lane >> 2)) * S::LD + 2 * (lane & 3);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        *reinterpret_cast<float2*>(out + 8 * nt) = make_float2(acc[nt][0], acc[nt][1]);
+        *reinterpret_cast<float2*>(out + 8 * S::LD + 8 * nt) = make_float2(acc[nt][2], acc[nt][3]);
       }
     }
-    float* out = red + half * RED + (quarter * NB_ROWS + 16 * mt + (lane >> 2)) * S::LD + 2 * (lane & 3);
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      *reinterpret_cast<float2*>(out + 8 * nt) = make_float2(acc[nt][0], acc[nt][1]);
-      *reinterpret_cast<float2*>(out + 8 * S::LD + 8 * nt) = make_float2(acc[nt][2], acc[nt][3]);
-    }
     // ---- dW: 32 columns x K over 32 rows a warp
+    if (p.dw) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      uint32_t a[2][4];
+      for (int ks = 0; ks < 2; ++ks) {
+        uint32_t a[2][4];
 #pragma unroll
-      for (int m = 0; m < 2; ++m)
-        nb_ldm_t(a[m], at + ((16 * ks + (lane & 7) + (lane >> 4) * 8) * NB_LD + 32 * warp + 16 * m + ((lane >> 3) & 1) * 8) * 2);
+        for (int m = 0; m < 2; ++m)
+          nb_ldm_t(a[m], at + ((16 * ks + (lane & 7) + (lane >> 4) * 8) * NB_LD + 32 * warp + 16 * m + ((lane >> 3) & 1) * 8) * 2);
 #pragma unroll
-      for (int nt = 0; nt < NT; nt += 2) {
-        uint32_t b[4];
-        nb_ldm_t(b, at_x + ((16 * ks + (lane & 15)) * S::LD + 8 * nt + (lane >> 4) * 8) * 2);
+        for (int nt = 0; nt < NT; nt += 2) {
+          uint32_t b[4];
+          nb_ldm_t(b, at_x + ((16 * ks + (lane & 15)) * S::LD + 8 * nt + (lane >> 4) * 8) * 2);
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          nb_mma(dw[m][nt], a[m], b[0], b[1]);
-          nb_mma(dw[m][nt + 1], a[m], b[2], b[3]);
+          for (int m = 0; m < 2; ++m) {
+            nb_mma(dw[m][nt], a[m], b[0], b[1]);
+            nb_mma(dw[m][nt + 1], a[m], b[2], b[3]);
+          }
         }
       }
     }
@@ -229,7 +245,7 @@ __global__ void __launch_bounds__(256, NarrowSmem<KT>::PER_SM) linear_narrow_bwd
   }
   nb_wait<0>();
   __syncthreads();
-  if (parked) sums_out(first + (last - first - 1) / NB_ROWS * NB_ROWS, half ^ 1);
+  if (parked && p.dx) sums_out(first + (last - first - 1) / NB_ROWS * NB_ROWS, half ^ 1);
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -237,7 +253,7 @@ __global__ void __launch_bounds__(256, NarrowSmem<KT>::PER_SM) linear_narrow_bwd
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int c = c0 + 32 * warp + 16 * m + (lane >> 2) + 8 * h, k = 8 * nt + 2 * (lane & 3);
-        if (c < p.C && k < p.K)
+        if (p.dw && c < p.C && k < p.K)
           *reinterpret_cast<float2*>(p.dw + (static_cast<long long>(blockIdx.y) * p.C + c) * p.K + k) = make_float2(dw[m][nt][2 * h], dw[m][nt][2 * h + 1]);
       }
   if (!p.db) return;
@@ -258,6 +274,7 @@ struct NarrowSums {
   __nv_bfloat16 *out_x, *out_w;
   void* out_b;
   int b_bf16, blocks, shares;
+  float scale;
   long long nx, nw, nb;      // pairs of values
 };
 __global__ void __launch_bounds__(256) linear_narrow_sum_kernel(const NarrowSums p) {
@@ -286,6 +303,8 @@ __global__ void __launch_bounds__(256) linear_narrow_sum_kernel(const NarrowSums
       s.y += v[u].y;
     }
   }
+  s.x *= p.scale;
+  s.y *= p.scale;
   const uint32_t u = pack_bf16(s.x, s.y);
   if (which == 0) reinterpret_cast<uint32_t*>(p.out_x)[i] = u;
   else if (which == 1) reinterpret_cast<uint32_t*>(p.out_w)[i] = u;
@@ -339,7 +358,7 @@ TTB_EXPORT int ttb_linear_narrow_parts(long long R, int C, int K, int sms, long 
 }
 
 // dy, z: [R, C] bf16 without gaps; x: [R, K] and w: [C, K], rows ldx and ldw apart; all on 16-byte boundaries; C % 8 == 0, K % 8 == 0, K <= 64.
-// dx [R, K] and dw [C, K] bf16, db [C] (or null) bf16 or fp32
+// dx [R, K] and dw [C, K] bf16, db [C] bf16 or fp32; each null unless wanted
 TTB_EXPORT int ttb_linear_narrow_bwd(const void* dy, const void* z, const void* x, long long ldx, const void* w, long long ldw, void* dx, void* dw, void* db,
                                      int db_bf16, float* parts, long long R, int C, int K, int act, unsigned t, float scale, unsigned long long seed,
                                      const unsigned long long* seed_dev, long long first_row, int sms, void* stream) {
@@ -351,12 +370,12 @@ TTB_EXPORT int ttb_linear_narrow_bwd(const void* dy, const void* z, const void* 
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   float *px = parts, *pw = px + q.blocks * R * K, *pb = pw + static_cast<long long>(q.shares) * C * K;
   const NarrowParams p{static_cast<const __nv_bfloat16*>(dy), static_cast<const __nv_bfloat16*>(z), static_cast<const __nv_bfloat16*>(x),
-                       static_cast<const __nv_bfloat16*>(w), ldx, ldw, px, pw, db ? pb : nullptr, R, C, K, q.steps,
+                       static_cast<const __nv_bfloat16*>(w), ldx, ldw, dx ? px : nullptr, dw ? pw : nullptr, db ? pb : nullptr, R, C, K, q.steps,
                        dropout_params(t, scale, seed, seed_dev, first_row)};
   const int r = K <= 16 ? narrow_act<16>(p, q, act, st) : K <= 32 ? narrow_act<32>(p, q, act, st) : narrow_act<64>(p, q, act, st);
   if (r) return r;
-  const NarrowSums s{px, pw, pb, static_cast<__nv_bfloat16*>(dx), static_cast<__nv_bfloat16*>(dw), db, db_bf16, q.blocks, q.shares,
-                     R * K / 2, static_cast<long long>(C) * K / 2, db ? C / 2 : 0};
+  const NarrowSums s{px, pw, pb, static_cast<__nv_bfloat16*>(dx), static_cast<__nv_bfloat16*>(dw), db, db_bf16, q.blocks, q.shares, t ? scale : 1.f,
+                     dx ? R * K / 2 : 0, dw ? static_cast<long long>(C) * K / 2 : 0, db ? C / 2 : 0};
   linear_narrow_sum_kernel<<<static_cast<unsigned>((s.nx + s.nw + s.nb + 255) / 256), 256, 0, st>>>(s);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? 0 : 400 + static_cast<int>(e);
