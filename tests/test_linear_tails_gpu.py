@@ -156,6 +156,40 @@ def test_few_rows(M, N, K):
         _check(_rand(gen, M, K, std=0.2), _rand(gen, N, K, std=0.2), _rand(gen, N), _rand(gen, M, N), act, p, 5, _rand(gen, M, N))
 
 
+@pytest.mark.parametrize("M, N, K", [(1500, 1152, 2304), (3001, 4304, 1152), (300, 136, 264), (4200, 520, 1160)])
+def test_products_of_the_backward_run_into_one_another(M, N, K):
+    """Whatever follows sees both products whole, over many steps in a row and replayed: the same bits as one after the other."""
+    from torchturbo_b200 import kernels as Kn
+    from torchturbo_b200.ops.dropout import NONE
+
+    gen = torch.Generator().manual_seed(M)
+    x, w, dys = _rand(gen, M, K), _rand(gen, N, K), [_rand(gen, M, N) for _ in range(4)]
+    z = _rand(gen, M, N, std=2.0)
+    want = []
+    for dy in dys:
+        dz, db = Kn.tail_bwd(dy, z, "gelu", NONE, True, torch.bfloat16)
+        want.append((Kn.gemm(dz, w, b_mn=True), Kn.gemm(dz, x, a_mn=True, b_mn=True), db))
+    torch.cuda.synchronize()
+
+    def steps():
+        got = []
+        for dy in dys * 5:
+            grads = Kn.linear_tail_bwd(dy, x, w, z, "gelu", NONE, True, True, True)
+            got.append([g + 0 for g in grads])
+            del grads                   # their memory is the next step's
+        return got
+
+    graph = torch.cuda.CUDAGraph()
+    eager = steps()
+    with torch.cuda.graph(graph):
+        replayed = steps()
+    graph.replay()
+    for got in (eager, replayed):
+        for i, grads in enumerate(got):
+            assert all(torch.equal(a, b) for a, b in zip(grads, want[i % 4]))
+    assert Kn.status() == (0, 0)
+
+
 def test_wide_rows():
     gen = torch.Generator().manual_seed(14)
     _check(_rand(gen, 20, 16), _rand(gen, 20000, 16), _rand(gen, 20000), None, "gelu", 0.1, 3, _rand(gen, 20, 20000))

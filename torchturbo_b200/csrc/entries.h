@@ -69,6 +69,9 @@ struct GemmArgs {
   // row0 on that lie below *part_rows; what lies behind is neither read nor written but to the end of a tile.
   const int* part_rows;
   int row0, part_k;
+  // Launches that do not need one another, one directly after the other: 1 lets the next one begin on SMs that this one leaves idle, 2 does
+  // not wait for the one before (which has to let it) but does not end before that one has.
+  int overlap;
 };
 
 // inputs of the chunk-parallel delta-rule kernels (delta_chunk.cuh)

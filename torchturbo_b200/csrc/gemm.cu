@@ -111,6 +111,7 @@ struct GemmParams {
   // rows that there are of the M (or, for `part_k`, of the K) that the buffers have, known on the device only; those before row0 are another call's
   const int* part_rows;
   int row0, part_k;
+  int overlap;
   int a_bytes, stage_bytes, stages;   // of a product with a tail: A in a stage, a stage, how many there are
 };
 
@@ -213,6 +214,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
   if (PAIR) cluster_sync();     // the barriers of both CTAs are set up
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if (p.overlap & 1) asm volatile("griddepcontrol.launch_dependents;");
 
   constexpr bool STORE = EPI == EPI_STORE || EPI == EPI_PART;
   constexpr bool PART = EPI == EPI_PART || EPI == EPI_LSE || EPI == EPI_DLOGITS;
@@ -921,6 +923,8 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       if (threadIdx.x == 0) *p.ep.done_counter = 0;
     }
   }
+  // whatever follows in the stream counts on the launch before having ended
+  if (p.overlap & 2) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // ----------------------------------------------------------------------------
@@ -1136,6 +1140,7 @@ static int launch(const GemmArgs& a, cudaStream_t stream, int tile_cols = BN) {
   if (total >= (1ll << 31) - 65536) return 910;
   // ---- C map (3D, last dim = group)
   tmC = tmZ = tmA;       // placeholders where nothing is stored through them
+  p.overlap = a.overlap;
   p.part_rows = a.part_rows; p.row0 = a.row0; p.part_k = a.part_k;
   p.tma_out = (EPI == EPI_STORE || EPI == EPI_PART) && !split && !a.c_fp32 && !a.residual && !a.accumulate && !p.ep.scat_on && a.M > 0 && a.N > 0 &&
               (a.groups_k == 0 || a.c_group_stride % 8 == 0);
@@ -1170,24 +1175,26 @@ static int launch(const GemmArgs& a, cudaStream_t stream, int tile_cols = BN) {
     const cudaError_t e = ensure_dynamic_smem(reinterpret_cast<const void*>(kfn), L::TOTAL, smem_done);
     if (e != cudaSuccess) return 300 + static_cast<int>(e);
   }
+  const int walkers = PAIR ? a.num_sms / 2 : a.num_sms;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>((PAIR ? 2 : 1) * (total < walkers ? total : walkers)));
+  cfg.blockDim = dim3(p.ep.push_on ? GEMM_THREADS_PUSH : L::THREADS);
+  cfg.dynamicSmemBytes = L::TOTAL;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
   if (PAIR) {
-    const int pairs = static_cast<int>(total < a.num_sms / 2 ? total : a.num_sms / 2);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(2 * pairs);
-    cfg.blockDim = dim3(L::THREADS);
-    cfg.dynamicSmemBytes = L::TOTAL;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kfn, tmA, tmB, tmC, tmZ, p);
-    if (e != cudaSuccess) return 400 + static_cast<int>(e);
-  } else {
-    const int grid = static_cast<int>(total < a.num_sms ? total : a.num_sms);
-    kfn<<<grid, p.ep.push_on ? GEMM_THREADS_PUSH : L::THREADS, L::TOTAL, stream>>>(tmA, tmB, tmC, tmZ, p);
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = 2; attr[cfg.numAttrs].val.clusterDim.y = 1; attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
   }
+  if (a.overlap & 2) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  const cudaError_t launched = cudaLaunchKernelEx(&cfg, kfn, tmA, tmB, tmC, tmZ, p);
+  if (launched != cudaSuccess) return 400 + static_cast<int>(launched);
   if (split && a.tail) {
     const long long n = static_cast<long long>(a.M) * (a.N / 8);
     split_tail_kernel<<<static_cast<unsigned>((n + 255) / 256), 256, 0, stream>>>(

@@ -373,8 +373,9 @@ PyObject* linear_tail(PyObject*, PyObject* const* args, Py_ssize_t n) {
   });
 }
 
-// (dz, db): dz = dropout(dy) act'(z), its column sums
-void tail_gradient(const Tensor& dy, const Tensor& z, int act, const Dropout& d, bool want_db, bool f32out, Tensor& dz, Tensor& db) {
+// (dz, db): dz = dropout(dy) act'(z), its column sums.  `part`, their parts, has to be kept for as long as what is launched next may overlap
+// (GemmArgs.overlap); defined if that may be
+void tail_gradient(const Tensor& dy, const Tensor& z, int act, const Dropout& d, bool want_db, bool f32out, Tensor& dz, Tensor& db, Tensor& part) {
   check_device(dy);
   need(dy.dim() == 2 && is_bf16(dy) && dy.is_contiguous() && on_16_bytes(dy), "gradients: bf16 rows without gaps");
   need(!z.defined() || (is_bf16(z) && z.is_contiguous() && z.sizes() == dy.sizes() && z.device() == dy.device()), "pre-activations: bf16 rows without gaps");
@@ -382,7 +383,7 @@ void tail_gradient(const Tensor& dy, const Tensor& z, int act, const Dropout& d,
   const bool own = act != 0 || d.t != 0;
   dz = own ? empty_rows(dy) : dy;
   const int grid = tail_row_blocks(R, C, sms(dy));
-  const Tensor part = want_db ? empty({grid, C}, at::kFloat, dy) : Tensor();
+  part = want_db && R ? empty({grid, C}, at::kFloat, dy) : Tensor();
   db = !want_db ? Tensor() : R ? empty({C}, out_type(f32out), dy) : at::zeros({C}, plain(dy).dtype(out_type(f32out)));
   if (R && (own || want_db))
     launch("ttb_tail_bwd", want_db ? 2 : 1, [&](void* st) {
@@ -398,18 +399,21 @@ PyObject* tail_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int act = static_cast<int>(in.integer());
     const Dropout d = dropout_args(in, dy);
     const bool want_db = in.flag(), f32out = in.flag();
-    Tensor dz, db;
-    tail_gradient(dy, z, act, d, want_db, f32out, dz, db);
+    Tensor dz, db, part;
+    tail_gradient(dy, z, act, d, want_db, f32out, dz, db, part);
     return wrap_all(dz, db);
   });
 }
 
 // plain bf16 product of MN-major operands as the backward of a linear layer has them
-Tensor backward_product(const Tensor& a, const Tensor& b, bool a_mn) {
+Tensor backward_product(const Tensor& a, const Tensor& b, bool a_mn, int& overlap) {
   GemmArgs g{};
   const long long M = a.size(a_mn ? 1 : 0), K = a.size(a_mn ? 0 : 1), N = b.size(1);
   const Tensor out = K ? empty({M, N}, at::kBFloat16, a) : at::zeros({M, N}, plain(a));
-  if (M == 0 || N == 0 || K == 0) return out;
+  if (M == 0 || N == 0 || K == 0) {
+    overlap = 0;
+    return out;
+  }
   g.A = a.const_data_ptr(); g.lda = a.stride(0);
   g.B = b.const_data_ptr(); g.ldb = b.stride(0); g.b_groups = 1;
   g.C = out.data_ptr(); g.ldc = N;
@@ -422,6 +426,10 @@ Tensor backward_product(const Tensor& a, const Tensor& b, bool a_mn) {
     ws = empty({s, M, N}, at::kFloat, a);
     g.split_ws = f32w(ws); g.k_splits = static_cast<int>(s);
   }
+  // Of a product in pieces the second launch, their sum, would be what the next product need not wait for; and its pieces' memory is free
+  // again as soon as this returns, so that the next one could take it while it is in use.
+  if (s > 1) overlap &= ~1;
+  g.overlap = overlap;
   launch("ttb_gemm_bf16", s > 1 ? 2 : 1, [&](void* st) { return ttb_gemm_bf16(&g, st); });
   return out;
 }
@@ -468,9 +476,19 @@ PyObject* linear_tail_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
          "operands of the backward: bf16 matrices that fit the gradient");
     if ((need_x || need_w || want_db) && x.defined() && w.defined() && narrow(dy, x))
       return narrow_bwd(dy, x, w, z, act, d, need_x, need_w, want_db, f32out);
-    Tensor dz, db;
-    tail_gradient(dy, z, act, d, want_db, f32out, dz, db);
-    const Tensor dx = need_x ? backward_product(dz, w, false) : Tensor(), dw = need_w ? backward_product(dz, x, true) : Tensor();
+    Tensor dz, db, part;
+    tail_gradient(dy, z, act, d, want_db, f32out, dz, db, part);
+    // Neither product needs the other, nor the bias's sums: tiles begin on SMs that the launch before leaves idle.  3001 x 1152 -> 4304, 60 tiles
+    // on 74 pairs of SMs and then 85: 75 us one after the other, 58 so, with GELU (erf) and bias 99 and 81; 300 x 1024 -> 1024 34 and 22, 43 and
+    // 28.  Products that fill all SMs for long gain nothing: 8192 x 4096 -> 12288 is bound by power.
+    int overlap = part.defined() ? 2 : 0;
+    Tensor dx, dw;
+    if (need_x) {
+      overlap |= need_w ? 1 : 0;
+      dx = backward_product(dz, w, false, overlap);
+      overlap = overlap & 1 ? 2 : 0;
+    }
+    if (need_w) dw = backward_product(dz, x, true, overlap);
     return wrap_all(dx, dw, db);
   });
 }

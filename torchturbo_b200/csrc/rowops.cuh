@@ -22,6 +22,7 @@ __device__ __forceinline__ void store_scalar(__nv_bfloat16* p, float v) { *p = _
 template <typename Out>
 static __global__ void __launch_bounds__(1024) colsum_kernel(const float* __restrict__ partial, Out* __restrict__ out, int rows, int H) {
   __shared__ float part[32][33];
+  asm volatile("griddepcontrol.launch_dependents;");      // a product that does not need these sums may begin (GemmArgs.overlap)
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + x;
   float s = 0.f;
