@@ -134,6 +134,13 @@ def test_few_features(M, N, K):
     assert Kn.status() == (0, 0)
 
 
+def test_few_features_of_many_rows():
+    """More than is walked row by row in the forward."""
+    gen = torch.Generator().manual_seed(17)
+    M, N = 4100, 4104
+    _check(_rand(gen, M, 16), _rand(gen, N, 16), _rand(gen, N), _rand(gen, M, N), None, 0.1, 5, _rand(gen, M, N))
+
+
 def test_few_features_of_wider_rows():
     """Inputs and weights that are parts of wider matrices, and a seed in memory."""
     from torchturbo_b200.ops import ops

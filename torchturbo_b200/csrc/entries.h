@@ -100,6 +100,7 @@ TTB_EXPORT int ttb_tail_row_blocks(long long, int, int);
 TTB_EXPORT int ttb_tail_bwd(const void*, const void*, void*, float*, void*, int, long long, int, int, unsigned, float, unsigned long long,
                             const unsigned long long*, long long, int, void*);
 TTB_EXPORT int ttb_linear_rows(const ttb::GemmArgs*, void*);
+TTB_EXPORT int ttb_linear_narrow(const ttb::GemmArgs*, void*);
 TTB_EXPORT int ttb_linear_narrow_parts(long long, int, int, int, long long*);
 TTB_EXPORT int ttb_linear_narrow_bwd(const void*, const void*, const void*, long long, const void*, long long, void*, void*, void*, int, float*, long long,
                             int, int, int, unsigned, float, unsigned long long, const unsigned long long*, long long, int, void*);

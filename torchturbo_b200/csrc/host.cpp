@@ -325,6 +325,10 @@ GemmArgs product(const Tensor& a, const Tensor& b) {
 // and 8.0, 12 and 16, 27 and 26; 8 rows 6.0 and 8.0, 19 and 16, 46 and 26.
 bool few_rows(const GemmArgs& g) { return g.M <= 4 || (g.M <= 8 && static_cast<long long>(g.N) * g.K <= (1 << 23)); }
 
+// Whether the rows are walked and not tiled (linear_narrow.cu).  us, walk and tiles, with residual: 2048 x 16 -> 4096 12 and 14, 16384 x 16 -> 1024 17 and 23,
+// 4096 x 16 -> 4096 23 and 22, 6000 x 16 -> 4096 32 and 28.  With 64 features the tiles are as fast from 300 rows on.
+bool few_features(const GemmArgs& g) { return g.K <= 16 && static_cast<long long>(g.M) * g.N <= (1ll << 24); }
+
 PyObject* linear_tail(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Args in(args, n, 11);
@@ -361,6 +365,10 @@ PyObject* linear_tail(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Tensor ws;
     if (few_rows(g)) {
       launch("ttb_linear_rows", 1, [&](void* st) { return ttb_linear_rows(&g, st); });
+      return wrap_all(y, pre);
+    }
+    if (few_features(g)) {
+      launch("ttb_linear_narrow", 1, [&](void* st) { return ttb_linear_narrow(&g, st); });
       return wrap_all(y, pre);
     }
     const long long s = g.K >= 4096 ? k_splits(M, N, g.K, g.num_sms) : 1;

@@ -348,7 +348,145 @@ static int narrow_act(const NarrowParams& p, const NarrowPlan& q, int act, cudaS
   return narrow_drop<KT, 0>(p, q, st);
 }
 
+// ---------------------------------------------------------------------------------------------
+// The layer itself with up to 16 input features, where C stays in the L2: one walk over its rows.  A warp owns 32 columns, whose weights stay in
+// registers, and multiplies 16 rows at a time, the next 16 rows' loads under way.  The columns are dealt to the products' columns so that
+// a thread ends up with eight neighbouring ones of a row: 16 bytes of the residual and of C, and what one draw of the dropout is for.
+// Bound by its loads and stores; no TMEM to fill and to read, no tile to wait for.  us, and by the tiles of gemm.cu: 300 x 16 -> 4096 3.0 (5.6), with dropout
+// and residual 4.2 (6.8); 16384 x 16 -> 1024 13 (17), 21 (28), with GELU (tanh) and pre-activations 16 (30).
+// ---------------------------------------------------------------------------------------------
+struct NarrowFwd {
+  const __nv_bfloat16 *x, *w, *bias, *residual;
+  __nv_bfloat16 *y, *pre;
+  long long ldx, ldw, ldr, R;
+  int N, K, across, per_block, down;      // warps across a row, of a block, and rows of warps in it
+  DropoutParams drop;
+};
+
+template <int ACT, bool DROP, typename Keys>
+__global__ void __launch_bounds__(256, 3) linear_narrow_fwd_kernel(const NarrowFwd p) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int place = blockIdx.x * p.per_block + warp % p.per_block;
+  if (warp >= p.per_block * p.down || place >= p.across) return;
+  const int col = 32 * place + 8 * t;
+  const bool live = col < p.N;
+  // column 2 t + e of the j-th product is column 8 t + 2 j + e of the warp's
+  uint32_t wf[4][2];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int c = 32 * place + 8 * (g >> 1) + 2 * j + (g & 1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) wf[j][h] = c < p.N && 8 * h < p.K ? __ldg(reinterpret_cast<const uint32_t*>(p.w + c * p.ldw + 8 * h + 2 * t)) : 0u;
+  }
+  uint4 bias = make_uint4(0u, 0u, 0u, 0u);
+  if (p.bias && live) bias = __ldg(reinterpret_cast<const uint4*>(p.bias + col));
+  const Keys key(p.drop);
+  uint32_t high = 0;
+  PhiloxColumn column{};
+  const long long step = static_cast<long long>(gridDim.y) * p.down * 16;
+  long long r0 = (static_cast<long long>(blockIdx.y) * p.down + warp / p.per_block) * 16;
+  if (DROP) {
+    high = static_cast<uint32_t>(static_cast<uint64_t>(p.drop.first_row + r0) >> 32);
+    column = philox_column(col >> 3, high, key);
+  }
+  uint4 rn[2];
+  uint32_t xn[4];
+  auto load = [&](long long first) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const long long r = first + 8 * i + g;
+      if (p.residual && live && r < p.R) rn[i] = load16_here(p.residual + r * p.ldr + col);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const long long r = first + 8 * i + g;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) xn[i + 2 * h] = r < p.R && 8 * h < p.K ? __ldg(reinterpret_cast<const uint32_t*>(p.x + r * p.ldx + 8 * h + 2 * t)) : 0u;
+    }
+  };
+  load(r0);
+  for (; r0 < p.R; r0 += step) {
+    uint4 rs[2];
+    float acc[4][4] = {};
+#pragma unroll
+    for (int i = 0; i < 2; ++i) rs[i] = rn[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) nb_mma(acc[j], xn, wf[j][0], wf[j][1]);
+    load(r0 + step);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const long long r = r0 + 8 * i + g;
+      if (!live || r >= p.R) continue;
+      float f[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        f[2 * j] = acc[j][2 * i];
+        f[2 * j + 1] = acc[j][2 * i + 1];
+      }
+      auto add = [&](const uint4& v) {
+        const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          f[2 * j] += __uint_as_float(u[j] << 16);
+          f[2 * j + 1] += __uint_as_float(u[j] & 0xffff0000u);
+        }
+      };
+      if (p.bias) add(bias);
+      if (p.pre) store8(p.pre + r * p.N + col, f);
+      if (ACT) {
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) act_pair<ACT>(f[j], f[j + 1]);
+      }
+      if (DROP) {
+        const uint64_t whole = static_cast<uint64_t>(p.drop.first_row + r);
+        if (static_cast<uint32_t>(whole >> 32) != high) {
+          high = static_cast<uint32_t>(whole >> 32);
+          column = philox_column(col >> 3, high, key);
+        }
+        dropout8(f, philox(column, philox_row(static_cast<uint32_t>(whole), key), key), p.drop.t << 16, p.drop.scale);
+      }
+      if (p.residual) add(rs[i]);
+      store8(p.y + r * p.N + col, f);
+    }
+  }
+}
+
+template <int ACT>
+static void narrow_fwd(const NarrowFwd& p, int sms, cudaStream_t st) {
+  const int bx = (p.across + p.per_block - 1) / p.per_block;
+  const long long rows = (p.R + 16 * p.down - 1) / (16 * p.down);
+  const unsigned by = static_cast<unsigned>(std::max<long long>(1, std::min<long long>({rows, 65535, (3ll * sms + bx - 1) / bx})));
+  auto go = [&](auto kernel) { kernel<<<dim3(bx, by), 256, 0, st>>>(p); };
+  if (!p.drop.t) go(linear_narrow_fwd_kernel<ACT, false, KeysOfLaunch>);
+  else if (p.drop.seed_dev) go(linear_narrow_fwd_kernel<ACT, true, KeysOfSeed>);
+  else go(linear_narrow_fwd_kernel<ACT, true, KeysOfLaunch>);
+}
+
 }  // namespace ttb
+
+// x, w, residual: rows of bf16 values on 16-byte boundaries; y and pre: [M, N] without gaps; N % 8 == 0, K 8 or 16
+TTB_EXPORT int ttb_linear_narrow(const ttb::GemmArgs* args, void* stream) {
+  using namespace ttb;
+  const GemmArgs& a = *args;
+  if (a.M < 1 || a.N < 1 || (a.K != 8 && a.K != 16) || (a.N % 8) || (a.lda % 8) || (a.ldb % 8) || (a.ldr % 8) || a.ldc != a.N || !a.tail ||
+      a.tail->act < 0 || a.tail->act > 2 || a.tail->drop_t > 65535)
+    return 901;
+  const TailArgs& t = *a.tail;
+  if ((reinterpret_cast<uintptr_t>(a.A) | reinterpret_cast<uintptr_t>(a.B) | reinterpret_cast<uintptr_t>(a.C) | reinterpret_cast<uintptr_t>(t.bias) |
+       reinterpret_cast<uintptr_t>(t.pre) | reinterpret_cast<uintptr_t>(a.residual)) & 15)
+    return 902;
+  const int across = (a.N + 31) / 32, per_block = across < 8 ? across : 8;
+  const NarrowFwd p{static_cast<const __nv_bfloat16*>(a.A), static_cast<const __nv_bfloat16*>(a.B), static_cast<const __nv_bfloat16*>(t.bias),
+                    static_cast<const __nv_bfloat16*>(a.residual), static_cast<__nv_bfloat16*>(a.C), static_cast<__nv_bfloat16*>(t.pre),
+                    a.lda, a.ldb, a.ldr, a.M, a.N, a.K, across, per_block, 8 / per_block,
+                    dropout_params(t.drop_t, t.drop_scale, t.seed, t.seed_dev, t.first_row)};
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (t.act == 1) narrow_fwd<1>(p, a.num_sms, st);
+  else if (t.act == 2) narrow_fwd<2>(p, a.num_sms, st);
+  else narrow_fwd<0>(p, a.num_sms, st);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? 0 : 400 + static_cast<int>(e);
+}
 
 // fp32 values that ttb_linear_narrow_bwd keeps its partial sums in
 TTB_EXPORT int ttb_linear_narrow_parts(long long R, int C, int K, int sms, long long* parts) {
