@@ -137,7 +137,7 @@ def test_few_features(M, N, K):
 def test_few_features_of_many_rows():
     """More than is walked row by row in the forward."""
     gen = torch.Generator().manual_seed(17)
-    M, N = 4100, 4104
+    M, N = 6200, 4104
     _check(_rand(gen, M, 16), _rand(gen, N, 16), _rand(gen, N), _rand(gen, M, N), None, 0.1, 5, _rand(gen, M, N))
 
 

@@ -325,9 +325,10 @@ GemmArgs product(const Tensor& a, const Tensor& b) {
 // and 8.0, 12 and 16, 27 and 26; 8 rows 6.0 and 8.0, 19 and 16, 46 and 26.
 bool few_rows(const GemmArgs& g) { return g.M <= 4 || (g.M <= 8 && static_cast<long long>(g.N) * g.K <= (1 << 23)); }
 
-// Whether the rows are walked and not tiled (linear_narrow.cu).  us, walk and tiles, with residual: 2048 x 16 -> 4096 12 and 14, 16384 x 16 -> 1024 17 and 23,
-// 4096 x 16 -> 4096 23 and 22, 6000 x 16 -> 4096 32 and 28.  With 64 features the tiles are as fast from 300 rows on.
-bool few_features(const GemmArgs& g) { return g.K <= 16 && static_cast<long long>(g.M) * g.N <= (1ll << 24); }
+// Whether the rows are walked and not tiled (linear_narrow.cu).  us, walk and tiles, with residual: 2048 x 16 -> 4096 11 and 14, 4096 x 16 -> 4096 20 and 22,
+// 6000 x 16 -> 4096 29 and 28, 8190 x 16 -> 4096 39 and 36; with GELU (tanh) and pre-activations 9 and 14, 17 and 24, 24 and 31, 32 and 35, and
+// 4096 x 16 -> 12288 45 and 59.  With 64 features the tiles are as fast from 300 rows on.
+bool few_features(const GemmArgs& g) { return g.K <= 16 && (g.tail->act || static_cast<long long>(g.M) * g.N <= 3ll << 23); }
 
 PyObject* linear_tail(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {

@@ -132,15 +132,19 @@ __global__ void __launch_bounds__(256, NarrowSmem<KT>::PER_SM) linear_narrow_bwd
   float db[8] = {}, dw[2][NT][4] = {};
   int buf = 0, half = 0;
   bool parked = false;
-  auto sums_out = [&](long long r0, int b) {
-    for (int e = tid; e < NB_ROWS * KT; e += 256) {
-      const int r = e / KT, k = e % KT;
-      if (k < p.K && r0 + r < last) {
-        const float* src = red + b * RED + r * S::LD + k;
-        constexpr int Q = NB_ROWS * S::LD;
-        p.dx[(static_cast<long long>(blockIdx.x) * p.R + r0 + r) * p.K + k] = (src[0] + src[Q]) + (src[2 * Q] + src[3 * Q]);
-      }
-    }
+  // each thread of the sums of one feature, and every 256 / KT-th row
+  const int sum_k = tid % KT, sum_r = tid / KT;
+  float* sum_to = p.dx + (blockIdx.x * p.R + first + sum_r) * p.K + sum_k;
+  const int sum_step = 256 / KT * p.K;
+  int sums_left = sum_k < p.K ? static_cast<int>(last - first) - sum_r : 0;
+  auto sums_out = [&](int b) {
+    const float* src = red + b * RED + sum_r * S::LD + sum_k;
+    constexpr int Q = NB_ROWS * S::LD;
+#pragma unroll
+    for (int i = 0; i < NB_ROWS * KT / 256; ++i, src += 256 / KT * S::LD)
+      if (i * (256 / KT) < sums_left) sum_to[i * sum_step] = (src[0] + src[Q]) + (src[2 * Q] + src[3 * Q]);
+    sum_to += NB_ROWS * p.K;
+    sums_left -= NB_ROWS;
   };
   for (long long r0 = first; r0 < last; r0 += NB_ROWS) {
     const uint32_t at = smem_u32(tile + buf * S::TILE), at_x = smem_u32(xs + buf * S::X);
@@ -196,7 +200,7 @@ __global__ void __launch_bounds__(256, NarrowSmem<KT>::PER_SM) linear_narrow_bwd
     __syncthreads();
     copy(buf == 0 ? AHEAD : buf - 1);
     nb_commit();
-    if (parked && p.dx) sums_out(r0 - NB_ROWS, half ^ 1);
+    if (parked && p.dx) sums_out(half ^ 1);
     parked = true;
     // ---- dx: 16 rows x K over 64 columns a warp
     if (p.dx) {
@@ -245,7 +249,7 @@ __global__ void __launch_bounds__(256, NarrowSmem<KT>::PER_SM) linear_narrow_bwd
   }
   nb_wait<0>();
   __syncthreads();
-  if (parked && p.dx) sums_out(first + (last - first - 1) / NB_ROWS * NB_ROWS, half ^ 1);
+  if (parked && p.dx) sums_out(half ^ 1);
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
@@ -349,11 +353,11 @@ static int narrow_act(const NarrowParams& p, const NarrowPlan& q, int act, cudaS
 }
 
 // ---------------------------------------------------------------------------------------------
-// The layer itself with up to 16 input features, where C stays in the L2: one walk over its rows.  A warp owns 32 columns, whose weights stay in
+// The layer itself with up to 16 input features, where C is small or an activation is applied: one walk over its rows.  A warp owns 32 columns, whose weights stay in
 // registers, and multiplies 16 rows at a time, the next 16 rows' loads under way.  The columns are dealt to the products' columns so that
 // a thread ends up with eight neighbouring ones of a row: 16 bytes of the residual and of C, and what one draw of the dropout is for.
-// Bound by its loads and stores; no TMEM to fill and to read, no tile to wait for.  us, and by the tiles of gemm.cu: 300 x 16 -> 4096 3.0 (5.6), with dropout
-// and residual 4.2 (6.8); 16384 x 16 -> 1024 13 (17), 21 (28), with GELU (tanh) and pre-activations 16 (30).
+// Bound by its loads and stores; no TMEM to fill and to read, no tile to wait for.  us, and by the tiles of gemm.cu: 200 x 16 -> 1152 2.1 (5.0), with dropout
+// and residual 2.5 (5.9); 16384 x 16 -> 1024 11 (17), 19 (28), with GELU (tanh) and pre-activations 14 (30).
 // ---------------------------------------------------------------------------------------------
 struct NarrowFwd {
   const __nv_bfloat16 *x, *w, *bias, *residual;
@@ -381,42 +385,44 @@ __global__ void __launch_bounds__(256, 3) linear_narrow_fwd_kernel(const NarrowF
   uint4 bias = make_uint4(0u, 0u, 0u, 0u);
   if (p.bias && live) bias = __ldg(reinterpret_cast<const uint4*>(p.bias + col));
   const Keys key(p.drop);
-  uint32_t high = 0;
+  const int step = gridDim.y * p.down * 16, first = (blockIdx.y * p.down + warp / p.per_block) * 16 + g;      // this thread's first row
+  uint64_t row = static_cast<uint64_t>(p.drop.first_row) + first;      // its place for the dropout
+  uint32_t high = static_cast<uint32_t>(row >> 32);
   PhiloxColumn column{};
-  const long long step = static_cast<long long>(gridDim.y) * p.down * 16;
-  long long r0 = (static_cast<long long>(blockIdx.y) * p.down + warp / p.per_block) * 16;
-  if (DROP) {
-    high = static_cast<uint32_t>(static_cast<uint64_t>(p.drop.first_row + r0) >> 32);
-    column = philox_column(col >> 3, high, key);
-  }
+  if (DROP) column = philox_column(col >> 3, high, key);
+  // addresses move on by steps: products of 64 bits for every row took as many instructions as all the rest
+  long long left = p.R - first;                  // rows from this thread's on
+  const __nv_bfloat16 *x = p.x + first * p.ldx + 2 * t, *residual = p.residual + first * p.ldr + col;
+  const long long out0 = static_cast<long long>(first) * p.N + col;
+  __nv_bfloat16 *y = p.y + out0, *pre = p.pre + out0;
+  const long long x_8 = 8 * p.ldx, x_step = step * p.ldx, r_8 = 8 * p.ldr, r_step = step * p.ldr, y_8 = 8ll * p.N, y_step = static_cast<long long>(step) * p.N;
+  const bool second = p.K > 8;
   uint4 rn[2];
   uint32_t xn[4];
-  auto load = [&](long long first) {
+  auto load = [&](long long there) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const long long r = first + 8 * i + g;
-      if (p.residual && live && r < p.R) rn[i] = load16_here(p.residual + r * p.ldr + col);
+      const bool in = 8 * i < there;
+      if (p.residual && live && in) rn[i] = load16_here(residual + i * r_8);
+      xn[i] = in ? __ldg(reinterpret_cast<const uint32_t*>(x + i * x_8)) : 0u;
+      xn[i + 2] = in && second ? __ldg(reinterpret_cast<const uint32_t*>(x + i * x_8 + 8)) : 0u;
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const long long r = first + 8 * i + g;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) xn[i + 2 * h] = r < p.R && 8 * h < p.K ? __ldg(reinterpret_cast<const uint32_t*>(p.x + r * p.ldx + 8 * h + 2 * t)) : 0u;
-    }
+    x += x_step;
+    residual += r_step;
   };
-  load(r0);
-  for (; r0 < p.R; r0 += step) {
+  load(left);
+  // whole warps go on for as long as one of their rows is there
+  for (; left + g > 0; left -= step, y += y_step, pre += y_step, row += step) {
     uint4 rs[2];
     float acc[4][4] = {};
 #pragma unroll
     for (int i = 0; i < 2; ++i) rs[i] = rn[i];
 #pragma unroll
     for (int j = 0; j < 4; ++j) nb_mma(acc[j], xn, wf[j][0], wf[j][1]);
-    load(r0 + step);
+    load(left - step);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const long long r = r0 + 8 * i + g;
-      if (!live || r >= p.R) continue;
+      if (!live || 8 * i >= left) continue;
       float f[8];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -432,13 +438,13 @@ __global__ void __launch_bounds__(256, 3) linear_narrow_fwd_kernel(const NarrowF
         }
       };
       if (p.bias) add(bias);
-      if (p.pre) store8(p.pre + r * p.N + col, f);
+      if (p.pre) store8(pre + i * y_8, f);
       if (ACT) {
 #pragma unroll
         for (int j = 0; j < 8; j += 2) act_pair<ACT>(f[j], f[j + 1]);
       }
       if (DROP) {
-        const uint64_t whole = static_cast<uint64_t>(p.drop.first_row + r);
+        const uint64_t whole = row + 8 * i;
         if (static_cast<uint32_t>(whole >> 32) != high) {
           high = static_cast<uint32_t>(whole >> 32);
           column = philox_column(col >> 3, high, key);
@@ -446,7 +452,7 @@ __global__ void __launch_bounds__(256, 3) linear_narrow_fwd_kernel(const NarrowF
         dropout8(f, philox(column, philox_row(static_cast<uint32_t>(whole), key), key), p.drop.t << 16, p.drop.scale);
       }
       if (p.residual) add(rs[i]);
-      store8(p.y + r * p.N + col, f);
+      store8(y + i * y_8, f);
     }
   }
 }
