@@ -318,6 +318,31 @@ def test_columns_that_are_not_finite(M, K, act):
     assert ((y[:, 3] == float("inf")) | (y[:, 3] == 0)).all() and ((y[:, 5] == 0) == (y[:, 5] == y[:, 5])).all()
 
 
+@pytest.mark.parametrize("M, N, K", [(700, 1032, 16), (1500, 1152, 520), (300, 264, 64)])
+def test_two_streams_at_once(M, N, K):
+    from torchturbo_b200.ops import ops
+
+    gen = torch.Generator().manual_seed(M)
+    sets = [[_rand(gen, *s).requires_grad_() for s in ((M, K), (N, K), (N,), (M, N))] for _ in range(2)]
+    dy = _rand(gen, M, N)
+
+    def step(x, w, b, r):
+        y = ops.linear_bias_act(x, w, b, "gelu", residual=r, dropout_p=0.1, seed=4)
+        return [y.detach(), *torch.autograd.grad(y, (x, w, b, r), dy)]
+
+    want = [step(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(6):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(step(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for steps in got[i] for a, b in zip(steps, want[i]))
+
+
 def test_result_may_be_changed_in_place():
     """The kept pre-activations are no view of the result."""
     from torchturbo_b200.ops import ops
