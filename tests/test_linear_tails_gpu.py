@@ -123,7 +123,7 @@ def test_long_sums_in_pieces(M, N, K, act, p):
 
 
 @pytest.mark.parametrize("K", [8, 16, 24, 32, 40, 64])
-@pytest.mark.parametrize("M, N", [(2, 8), (31, 256), (33, 264), (9511, 24), (5000, 1032), (700, 4104)])
+@pytest.mark.parametrize("M, N", [(2, 8), (31, 256), (33, 264), (9511, 24), (99, 21000), (5000, 1032), (700, 4104)])
 def test_few_features(M, N, K):
     """Adapters: the backward walks the gradient once, in shares of rows that end inside a step and blocks of columns that are cut."""
     from torchturbo_b200 import kernels as Kn
