@@ -443,13 +443,13 @@ Tensor backward_product(const Tensor& a, const Tensor& b, bool a_mn, int& overla
   return out;
 }
 
-// Whether the backward walks the gradient once for all that is wanted of it (linear_narrow.cu): up to 16 input features, or up to 64 of a
+// Whether the backward walks the gradient once for all that is wanted of it (linear_narrow.cu): up to 32 input features, or up to 64 of a
 // gradient so small that launches are what its time is.  us, a walk with its sums and separate passes: 8190 x 16 -> 4096 24 and 37, with dropout
-// 43 and 63, with GELU (erf) and dropout 67 and 83; 32 features 42 and 36, 62 and 62, 95 and 81; 64 features 61 and 34, but 300 rows 11 and 16,
-// with dropout 13 and 19.
+// 41 and 63, with GELU (erf) and dropout 67 and 83; 32 features 32 and 34, 49 and 60, 72 and 80; 64 features 61 and 34, but 300 rows 10 and 16,
+// with dropout 12 and 19.
 bool narrow(const Tensor& dy, const Tensor& x) {
   const long long K = x.size(1);
-  return K > 0 && (K <= 16 || (K <= 64 && dy.numel() <= (1ll << 21))) && dy.numel() > 0 && dy.size(0) < (1ll << 30);
+  return K > 0 && (K <= 32 || (K <= 64 && dy.numel() <= (1ll << 21))) && dy.numel() > 0 && dy.size(0) < (1ll << 30);
 }
 PyObject* narrow_bwd(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& z, int act, const Dropout& d, bool need_x, bool need_w, bool want_db,
                      bool f32out) {

@@ -35,7 +35,7 @@ constexpr int NB_COLS = 256, NB_ROWS = 32, NB_LD = NB_COLS + 8;      // rows of 
 template <int KT>
 struct NarrowSmem {
   static constexpr int LD = KT + 8;                                  // of x and W, and (in floats) of the sums
-  static constexpr int RING = KT <= 16 ? 2 : 3;                      // steps: one at work, the others' loads under way
+  static constexpr int RING = KT <= 32 ? 2 : 3;                      // steps: one at work, the others' loads under way
   static constexpr int TILE = NB_ROWS * NB_LD * 2, X = NB_ROWS * LD * 2, W = NB_COLS * LD * 2, RED = 4 * NB_ROWS * LD * 4;
   static constexpr int TOTAL = RING * (TILE + X) + W + 2 * RED;
   static constexpr int PER_SM = KT <= 16 ? 3 : KT <= 32 ? 2 : 1;     // blocks
