@@ -23,14 +23,12 @@ __device__ __forceinline__ float act_grad(float v, int act) {
 }
 
 // The same for pairs of values in the epilogue of a product and in its backward, where the arithmetic is the bound: half of the products in
-// packed form, and erf by Abramowitz and Stegun 7.1.26 (C. Hastings),
-//   erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2) + e,  t = 1 / (1 + p x),  x >= 0,  |e| <= 1.5e-7,
-// a fortieth of the smallest step of bf16 next to 1, whose exponential the derivative of gelu takes as well.
-__device__ __forceinline__ float tanh_approx(float x) {
-  float y;
-  asm("tanh.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
+// packed form.
+//   tanh  (1 + tanh u) / 2 = 1 / (1 + exp(-2 u)), which does not cancel where u is far below zero: values and slopes keep 2^-17 and 2^-15 of
+//         their own size from -6 on.  The hardware's hyperbolic tangent (one instruction for two) is 2^-11 off, more than all of the value at -4.
+//   erf   by Abramowitz and Stegun 7.1.26 (C. Hastings),  erfc(x) = (a1 t + ... + a5 t^5) exp(-x^2) + e,  t = 1 / (1 + p x),  x >= 0,
+//         |e| <= 1.5e-7: relative to gelu's value 0.03 of half a step of bf16 (2^-9 next to 1) at -3, 0.25 at -4, 0.8 at -5 and 2 at -6, where the
+//         value is 6e-9.  The derivative takes the same exponential.
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -57,15 +55,20 @@ __device__ __forceinline__ void gelu_erf_parts(float va, float vb, uint64_t& upp
   q = f2_fma(q, t, f2_both(0.5f * 0.254829592f));
   upper = f2_mul(f2_mul(q, t), expo);
 }
+// s = (1 + tanh u) / 2,  u = v (c + 0.044715 c v^2),  of two values
+__device__ __forceinline__ uint64_t gelu_tanh_share(uint64_t v) {
+  const float down = -2.f * 1.4426950408889634f;
+  float a, b;
+  f2_unpack(f2_mul(v, f2_fma(f2_mul(v, v), f2_both(down * 0.035677408136300125f), f2_both(down * 0.7978845608028654f))), a, b);
+  f2_unpack(f2_add(f2_pack(exp2_approx(a), exp2_approx(b)), f2_both(1.f)), a, b);
+  return f2_pack(rcp_approx(a), rcp_approx(b));
+}
 // (a, b) -> act(a), act(b)
 template <int ACT>
 __device__ __forceinline__ void act_pair(float& a, float& b) {
   if (ACT == 1) {
-    // 0.5 v (1 + tanh(v (c + 0.044715 c v^2)))
-    const uint64_t v = f2_pack(a, b), h = f2_mul(v, f2_both(0.5f));
-    float ua, ub;
-    f2_unpack(f2_mul(v, f2_fma(f2_mul(v, v), f2_both(0.035677408136300125f), f2_both(0.7978845608028654f))), ua, ub);
-    f2_unpack(f2_fma(h, f2_pack(tanh_approx(ua), tanh_approx(ub)), h), a, b);
+    // v s; of minus infinity none is left
+    f2_unpack(f2_mul(f2_pack(fmaxf(a, -3e38f), fmaxf(b, -3e38f)), gelu_tanh_share(f2_pack(a, b))), a, b);
   } else if (ACT == 2) {
     // v Phi(v) = max(v, 0) - |v| (1 - Phi(|v|)); the second term of infinity is none
     uint64_t upper, expo;
@@ -79,14 +82,12 @@ template <int ACT>
 __device__ __forceinline__ void act_slope_pair(float& a, float& b) {
   const uint64_t v = f2_pack(a, b);
   if (ACT == 1) {
-    // with u = v (c + k v^2), t = tanh u:  0.5 (1 + t) + 0.5 v (1 - t^2) (c + 3 k v^2)
-    const uint64_t v2 = f2_mul(v, v);
-    float ua, ub;
-    f2_unpack(f2_mul(v, f2_fma(v2, f2_both(0.035677408136300125f), f2_both(0.7978845608028654f))), ua, ub);
-    const uint64_t t = f2_pack(tanh_approx(ua), tanh_approx(ub));
-    const uint64_t rest = f2_fma(f2_mul(t, t), f2_both(-1.f), f2_both(1.f));
-    const uint64_t inner = f2_fma(v2, f2_both(1.5f * 0.035677408136300125f), f2_both(0.5f * 0.7978845608028654f));
-    f2_unpack(f2_fma(f2_mul(rest, v), inner, f2_fma(t, f2_both(0.5f), f2_both(0.5f))), a, b);
+    // s + s (1 - s) v 2 u',  2 u' = 2 c + 6 k v^2; from 16 on the second term is below 1e-100, so v^3 stops there
+    const uint64_t s = gelu_tanh_share(v);
+    const float most = 16.f;
+    const uint64_t w = f2_pack(fmaxf(fminf(a, most), -most), fmaxf(fminf(b, most), -most));
+    const uint64_t inner = f2_mul(w, f2_fma(f2_mul(w, w), f2_both(6.f * 0.035677408136300125f), f2_both(2.f * 0.7978845608028654f)));
+    f2_unpack(f2_fma(f2_fma(f2_mul(s, f2_both(-1.f)), s, s), inner, s), a, b);
   } else if (ACT == 2) {
     // Phi(v) + v phi(v),  Phi(v) = v > 0 ? 1 - upper : upper
     uint64_t upper, expo;
