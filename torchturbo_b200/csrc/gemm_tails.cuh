@@ -177,8 +177,9 @@ __device__ __forceinline__ void tail_store(const GemmParams& p, const CUtensorMa
 // The tensor cores' fp32 sums are cut off, not rounded, at every addition: after 2048 products of random signs they are 1.4e-6 of their
 // size too near to zero, all of them to the same side, and the bias grows with the length (1024: 6.6e-7, 512: 3.1e-7).
 // Log-probabilities leave in fp32, so their sums are run over LSE_RUN k-blocks at a time and the runs are added up in registers, rounded.
-// 4096 x 2048 x 151936 under the power cap: one run 1815 us, runs of 16 blocks 1816, of 8 blocks 1877.
-constexpr int LSE_RUN = 16;
+// 4096 x 2048 x 151936 under the power cap: one run 1815 us, runs of 16 blocks 1816, of 8 blocks 1877.  Eight, for 3 % of the time: runs of 16
+// are twice as far off as fp32 sums of rounded products (6.8e-7 and 1.9e-7 of log-probabilities in the 2-norm).
+constexpr int LSE_RUN = 8;
 
 template <int BN>
 __device__ __forceinline__ void tail_add(float (&sum)[BN / 2], uint32_t at, int cols) {
