@@ -216,6 +216,10 @@ class FSDP2Backend(BaseBackend):
         self._setup_prefetch(model)
         self._install_peer_collectives()
         self._register_vision_balance(model, compiled)
+        if peft_config is not None:
+            from ...peft import place_adapters
+
+            place_adapters(model, rank=self.rank, dp_rank=self.dp_rank, sp_rank=self.sp_rank)
         self.gradient_scaling_factor = 1.0 / self.ep_size
         return model
 

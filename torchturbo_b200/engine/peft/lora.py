@@ -25,7 +25,8 @@ class LoraConfig:
     r: int = 8
     lora_alpha: float = 16.0
     lora_dropout: float = 0.0
-    # masks by `ops.dropout` (drawn by place, never stored, the same in a recomputed forward) instead of `nn.Dropout`'s
+    # masks by `ops.dropout` (drawn by place, never stored, the same in a recomputed forward and, with ranks that share a seed, for the
+    # shards of a sequence as for the whole; ranks with other data draw others) instead of `nn.Dropout`'s
     counter_dropout: bool = False
     target_modules: list[str] | str = field(default_factory=lambda: ["all-linear"])
     use_dora: bool = False
@@ -71,6 +72,10 @@ def init_lora_tensor(t: torch.Tensor, kind: str, how: bool | str = True) -> None
 
 
 class LoRALinear(nn.Module):
+    # Of `counter_dropout`: which replica's data the layer sees, and which of equal shards of the replica's rows (`place_adapters`).
+    # Replicas' masks lie 2^40 rows apart.
+    replica, shard = 0, 0
+
     def __init__(self, base: nn.Linear, cfg: LoraConfig):
         super().__init__()
         self.base_layer = base
@@ -124,7 +129,8 @@ class LoRALinear(nn.Module):
             if self.cfg.counter_dropout:
                 from ...ops import ops
 
-                low = ops.linear(ops.dropout(x, self.cfg.lora_dropout, scale=self.cfg.scaling), self.lora_A[n].weight)
+                first = (self.replica << 40) + self.shard * (x.numel() // x.shape[-1])
+                low = ops.linear(ops.dropout(x, self.cfg.lora_dropout, scale=self.cfg.scaling, first_row=first), self.lora_A[n].weight)
                 base = ops.linear_bias_act(x, self.base_layer.weight, self.base_layer.bias)
                 return ops.linear_bias_act(low, self.lora_B[n].weight, residual=base)
             base = nn.functional.linear(x, self.base_layer.weight, self.base_layer.bias)
@@ -240,6 +246,25 @@ def apply_peft(model: nn.Module, peft_config) -> nn.Module:
     cfgs[cfg.adapter_name] = cfg
     model.peft_config = cfgs
     return model
+
+
+def place_adapters(model: nn.Module, *, rank: int, dp_rank: int, sp_rank: int) -> None:
+    """Tells every adapted layer which rows are its own, for masks that are drawn by place.  All ranks draw the same seeds, so layers that
+    see a shard of a sequence continue the mask of the shard before, and layers that see the whole on every rank of a
+    sequence-parallel group (media towers, projectors, modules with `full_sequence_rows`) draw the same one.  A tower whose media are dealt
+    out over all ranks has rows of its own on each."""
+    names = [n for a in ("vision_module_names", "vision_tower_module_names", "projector_module_names", "multi_modal_projector_module_names")
+             for n in getattr(model, a, ())]
+    for fqn, m in model.named_modules():
+        if not isinstance(m, LoRALinear):
+            continue
+        parents = [model.get_submodule(fqn[:i]) for i, c in enumerate(fqn) if c == "."]
+        if any(getattr(p, "_vision_balance_state", None) is not None for p in parents):
+            m.replica, m.shard = rank, 0
+        elif any(f".{n}." in f".{fqn}." for n in names) or any(getattr(p, "full_sequence_rows", False) for p in parents):
+            m.replica, m.shard = dp_rank, 0
+        else:
+            m.replica, m.shard = dp_rank, sp_rank
 
 
 _ADAPTER_SEGMENTS = ("lora_A", "lora_B", "lora_magnitude_vector", "lora1", "lora2")

@@ -167,6 +167,8 @@ class Compressor(nn.Module):
     """Gated pooling of every `ratio` consecutive tokens of a sequence into one row of width `head_dim`; with
     `ratio == 4` a group also pools the first half-channels of the previous group (overlap)."""
 
+    full_sequence_rows = True      # on every rank of a sequence-parallel group
+
     def __init__(self, config: Any, ratio: int, head_dim: int, dtype=None):
         super().__init__()
         self.ratio, self.head_dim, self.rd = ratio, head_dim, config.qk_rope_head_dim
