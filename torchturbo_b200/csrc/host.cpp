@@ -447,32 +447,31 @@ Tensor backward_product(const Tensor& a, const Tensor& b, bool a_mn, int& overla
 // gradient so small that launches are what its time is.  us, a walk with its sums and separate passes: 8190 x 16 -> 4096 24 and 37, with dropout
 // 41 and 63, with GELU (erf) and dropout 67 and 83; 32 features 32 and 34, 49 and 60, 72 and 80; 64 features 61 and 34, but 300 rows 10 and 16,
 // with dropout 12 and 19.
-bool narrow(const Tensor& dy, const Tensor& x) {
-  const long long K = x.size(1);
+bool narrow(const Tensor& dy, long long K) {
   return K > 0 && (K <= 32 || (K <= 64 && dy.numel() <= (1ll << 21))) && dy.numel() > 0 && dy.size(0) < (1ll << 30);
 }
 PyObject* narrow_bwd(const Tensor& dy, const Tensor& x, const Tensor& w, const Tensor& z, int act, const Dropout& d, bool need_x, bool need_w, bool want_db,
                      bool f32out) {
   check_device(dy);
-  need(is_bf16(dy) && dy.dim() == 2 && dy.is_contiguous() && on_16_bytes(dy) && dy.size(1) % 8 == 0 && is_bf16(x) && is_bf16(w) && x.size(1) % 8 == 0 &&
-           w.size(1) == x.size(1),
+  need(is_bf16(dy) && dy.dim() == 2 && dy.is_contiguous() && on_16_bytes(dy) && dy.size(1) % 8 == 0 && is_bf16(w) && w.size(1) % 8 == 0 &&
+           (!x.defined() || (is_bf16(x) && x.size(1) == w.size(1))),
        "gradients: bf16 rows without gaps, widths are multiples of eight");
   need(!z.defined() || (is_bf16(z) && z.is_contiguous() && z.sizes() == dy.sizes() && z.device() == dy.device()), "pre-activations: bf16 rows without gaps");
   const long long R = dy.size(0);
-  const int C = static_cast<int>(dy.size(1)), K = static_cast<int>(x.size(1)), num_sms = sms(dy);
+  const int C = static_cast<int>(dy.size(1)), K = static_cast<int>(w.size(1)), num_sms = sms(dy);
   const Tensor dx = need_x ? empty({R, K}, at::kBFloat16, dy) : Tensor(), dw = need_w ? empty({C, K}, at::kBFloat16, dy) : Tensor(),
                db = want_db ? empty({C}, out_type(f32out), dy) : Tensor();
   long long values = 0;
   narrow_parts(R, C, K, num_sms, &values);
   const Tensor parts = empty({values}, at::kFloat, dy);
   launch("ttb_linear_narrow_bwd", 2, [&](void* st) {
-    return ttb_linear_narrow_bwd(at_(dy), at_(z), at_(x), x.stride(0), at_(w), w.stride(0), to_(dx), to_(dw), to_(db), !f32out, f32w(parts), R, C, K, act, d.t,
+    return ttb_linear_narrow_bwd(at_(dy), at_(z), at_(x), x.defined() ? x.stride(0) : K, at_(w), w.stride(0), to_(dx), to_(dw), to_(db), !f32out, f32w(parts), R, C, K, act, d.t,
                                  d.scale, d.seed, d.dev(), d.first_row, num_sms, st);
   });
   return wrap_all(dx, dw, db);
 }
 
-// (dx, dw, db) of linear_tail, in one call: the three are four launches
+// (dx, dw, db) of linear_tail, in one call: the three are four launches.  x may be missing where dw is not wanted
 PyObject* linear_tail_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
     Args in(args, n, 14);
@@ -483,7 +482,7 @@ PyObject* linear_tail_bwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
     need((!need_x || (w.defined() && is_bf16(w) && w.dim() == 2 && w.size(0) == dy.size(1) && w.device() == dy.device())) &&
              (!need_w || (x.defined() && is_bf16(x) && x.dim() == 2 && x.size(0) == dy.size(0) && x.device() == dy.device())),
          "operands of the backward: bf16 matrices that fit the gradient");
-    if ((need_x || need_w || want_db) && x.defined() && w.defined() && narrow(dy, x))
+    if ((need_x || need_w || want_db) && w.defined() && w.dim() == 2 && narrow(dy, w.size(1)))
       return narrow_bwd(dy, x, w, z, act, d, need_x, need_w, want_db, f32out);
     Tensor dz, db, part;
     tail_gradient(dy, z, act, d, want_db, f32out, dz, db, part);

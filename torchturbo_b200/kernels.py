@@ -232,7 +232,7 @@ def linear_tail(x, weight, bias, act, residual, drop, want_pre):
 
 
 def linear_tail_bwd(dy, x, weight, z, act, drop, want_dx, want_dw, want_db, db_dtype=torch.bfloat16):
-    """(dx, dw, db) of `linear_tail`, each None unless wanted."""
+    """(dx, dw, db) of `linear_tail`, each None unless wanted; ``x`` may be None where dw is not."""
     return host().linear_tail_bwd(dy, x, weight, z, ACT[act], drop.t, drop.scale, drop.seed, drop.seed_tensor, drop.first_row, want_dx, want_dw,
                                   want_db, _is_f32(db_dtype))
 

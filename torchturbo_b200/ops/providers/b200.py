@@ -397,8 +397,9 @@ class LinearBiasActFn(torch.autograd.Function):
         back = need_x or need_w or need_b
         y, z = K.linear_tail(x, w, bias, act, residual, drop, back and K.ACT[act] != 0)
         if back:
-            # the seed is saved like an operand: moving it on before the backward is an error and not another mask
-            ctx.save_for_backward(x, w, bias, z, drop.seed_tensor)
+            # The seed is saved like an operand: moving it on before the backward is an error and not another mask.  The input is for
+            # the weight's gradient, and for a graph of the gradients where the slope depends on it; a frozen layer lets it go.
+            ctx.save_for_backward(x if need_w or z is not None else None, w, bias, z, drop.seed_tensor)
             ctx.act, ctx.drop = act, drop
         return y
 
@@ -410,6 +411,8 @@ class LinearBiasActFn(torch.autograd.Function):
             x, w, bias, z, seed = ctx.saved_tensors
             drop = _with_seed(ctx.drop, seed)
             if torch.is_grad_enabled():
+                if x is None:                    # the gradients do not depend on it
+                    x = w.new_zeros(dy.shape[0], w.shape[1]).requires_grad_(need_x)
                 y = N.linear_bias_act_ref(x, w, bias, ctx.act, None, drop)
                 dx, dw, db = _graph_of_gradients(y, (x, w, bias), (need_x, need_w, need_b), dy)
             else:
