@@ -28,10 +28,10 @@ class Dropout:
 NONE = Dropout(0, 1.0, 0, None, 0)
 
 
-def dropout_args(p: float, seed, first_row: int = 0, scale: float = 1.0) -> Dropout:
-    """Checks a dropout's arguments.  `seed`: an integer in [0, 2^63), an int64 tensor of one value (read when the kernel runs: a captured
-    step draws new masks when the tensor is moved on), or None for one drawn from torch's CPU generator (so that `torch.manual_seed`
-    and the restored generator state of activation checkpointing apply)."""
+def dropout_args(p: float, seed, first_row: int = 0, scale: float = 1.0, device: torch.device | None = None) -> Dropout:
+    """Checks a dropout's arguments.  `seed`: an integer in [0, 2^63), an int64 tensor of one value on the `device` of the rows (read
+    when the kernel runs: a captured step draws new masks when the tensor is moved on), or None for one drawn from torch's CPU
+    generator (so that `torch.manual_seed` and the restored generator state of activation checkpointing apply)."""
     if p == 0.0 and scale == 1.0 and first_row == 0:
         return NONE
     if not 0.0 <= p <= 1.0:
@@ -46,6 +46,8 @@ def dropout_args(p: float, seed, first_row: int = 0, scale: float = 1.0) -> Drop
     if isinstance(seed, torch.Tensor):
         if seed.dtype != torch.int64 or seed.numel() != 1:
             raise ValueError("a seed tensor is one int64 value")
+        if device is not None and seed.device != device:      # as the kernels' launch functions have it
+            raise AssertionError(f"a seed tensor is one int64 value on the device of the rows, {device}, got one on {seed.device}")
         seed, tensor = 0, seed.detach()
     elif seed is None:
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():

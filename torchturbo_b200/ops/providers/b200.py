@@ -432,7 +432,7 @@ class B200LinearBiasAct(_B200Op):
     backward is one pass over them and the incoming gradient, and the two products."""
 
     def __call__(self, x, weight, bias=None, act=None, *, residual=None, dropout_p=0.0, seed=None, first_row=0):
-        drop = dropout_args(dropout_p, seed, first_row)
+        drop = dropout_args(dropout_p, seed, first_row, device=x.device)
         if not _ok(x, weight, bias, residual) or act not in K.ACT or weight.dim() != 2 or x.dim() == 0 or weight.shape[0] % 8 or weight.shape[1] % 8 or not weight.numel() \
                 or drop.t > 65535 or _traced(x, weight, bias, residual):
             N.check_linear_bias_act(x, weight, bias, act, residual)
@@ -468,7 +468,7 @@ class B200Dropout(_B200Op):
 
     def __call__(self, x, p, seed=None, *, residual=None, scale=1.0, first_row=0):
         N.check_dropout(x, residual)
-        drop = dropout_args(p, seed, first_row, scale)
+        drop = dropout_args(p, seed, first_row, scale, x.device)
         if not x.is_cuda or x.dtype not in (BF16, torch.float32) or not x.numel() or drop.t > 65535 or _traced(x, residual):
             return dropout_ref(x, drop, residual)
         if _differentiated(x, residual):

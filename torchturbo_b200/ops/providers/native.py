@@ -104,7 +104,7 @@ class TorchDropout(OpImpl):
 
     def __call__(self, x, p, seed=None, *, residual=None, scale=1.0, first_row=0):
         check_dropout(x, residual)
-        return dropout_ref(x, dropout_args(p, seed, first_row, scale), residual)
+        return dropout_ref(x, dropout_args(p, seed, first_row, scale, x.device), residual)
 
 
 def check_linear_bias_act(x, weight, bias, act, residual) -> None:
@@ -140,7 +140,7 @@ class TorchLinearBiasAct(OpImpl):
 
     def __call__(self, x, weight, bias=None, act=None, *, residual=None, dropout_p=0.0, seed=None, first_row=0):
         check_linear_bias_act(x, weight, bias, act, residual)
-        return linear_bias_act_ref(x, weight, bias, act, residual, dropout_args(dropout_p, seed, first_row))
+        return linear_bias_act_ref(x, weight, bias, act, residual, dropout_args(dropout_p, seed, first_row, device=x.device))
 
 
 @_native("qkv_bias_rope")
