@@ -52,7 +52,7 @@ def dropout_args(p: float, seed, first_row: int = 0, scale: float = 1.0, device:
     elif seed is None:
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise ValueError("a captured dropout needs a seed: pass an int64 tensor and move it on between replays")
-        seed = int(torch.randint(0, 2 ** 62, (1,)))
+        seed = int(torch.randint(0, 2 ** 62, (1,), device="cpu"))
     elif isinstance(seed, bool) or not isinstance(seed, int) or not 0 <= seed < 2 ** 63:
         raise ValueError(f"a seed is an integer in [0, 2^63), got {seed!r}")
     return Dropout(t, factor, seed, tensor, first_row)
