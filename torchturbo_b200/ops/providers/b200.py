@@ -1062,10 +1062,11 @@ class LinearLogprobsFn(torch.autograd.Function):
 
 @_custom("linear_logprobs", "tcgen05_linear_logprobs")
 class B200LinearLogprobs(_B200Op):
-    def __call__(self, hidden, weight, targets, *, want_entropy: bool = False):
+    def __call__(self, hidden, weight, targets, *, want_entropy: bool = False, chunk: int = 1024):
+        """`chunk`: of the plain formulation, where the kernels do not take the call."""
         N.check_linear_logprobs(hidden, weight, targets)
         if not _ok(hidden, weight) or hidden.shape[-1] % 8 or _traced(hidden, weight):
-            return N.TorchLinearLogprobs()(hidden, weight, targets, want_entropy=want_entropy)
+            return N.TorchLinearLogprobs()(hidden, weight, targets, want_entropy=want_entropy, chunk=chunk)
         flat = targets if targets.dim() == 1 else targets.reshape(-1)
         flat = flat.long().contiguous()
         if _differentiated(hidden, weight):
