@@ -71,6 +71,17 @@ def init_lora_tensor(t: torch.Tensor, kind: str, how: bool | str = True) -> None
             nn.init.kaiming_uniform_(t.view(-1, t.shape[-1]), a=math.sqrt(5))
 
 
+def _product(x, w, bias=None, residual=None):
+    """`residual + x W^T + bias` in one product.  Widths that its kernel does not take (a rank of 4) stay in the layer's type, where the
+    operator's plain form would copy the operands to fp32."""
+    from ...ops import ops
+
+    if w.shape[0] % 8 or w.shape[1] % 8:
+        y = nn.functional.linear(x, w, bias)
+        return y if residual is None else residual + y
+    return ops.linear_bias_act(x, w, bias, residual=residual)
+
+
 class LoRALinear(nn.Module):
     # Of `counter_dropout`: which replica's data the layer sees, and which of equal shards of the replica's rows (`place_adapters`).
     # Replicas' masks lie 2^40 rows apart.
@@ -131,8 +142,7 @@ class LoRALinear(nn.Module):
 
                 first = (self.replica << 40) + self.shard * (x.numel() // x.shape[-1])
                 low = ops.linear(ops.dropout(x, self.cfg.lora_dropout, scale=self.cfg.scaling, first_row=first), self.lora_A[n].weight)
-                base = ops.linear_bias_act(x, self.base_layer.weight, self.base_layer.bias)
-                return ops.linear_bias_act(low, self.lora_B[n].weight, residual=base)
+                return _product(low, self.lora_B[n].weight, residual=_product(x, self.base_layer.weight, self.base_layer.bias))
             base = nn.functional.linear(x, self.base_layer.weight, self.base_layer.bias)
             return base + self.lora_B[n](self.lora_A[n](self.dropout(x))) * self.cfg.scaling
         return nn.functional.linear(x, self.weight, self.bias)
