@@ -92,8 +92,8 @@ TTB_EXPORT int ttb_logprobs_slots(int, int, int, int, int*);
 TTB_EXPORT int ttb_logprobs_join(const float*, const float*, const long long*, const int*, const int*, int, int, long long, long long, float*,
                             float*, float*, void*);
 TTB_EXPORT int ttb_rows_with_targets(const long long*, long long, long long, int*, int*, long long*, int*, float*, void*);
-TTB_EXPORT int ttb_gather_rows(const void*, long long, const int*, const int*, void*, long long, int, void*);
-TTB_EXPORT int ttb_scatter_rows(const void*, int, const int*, void*, long long, int, void*);
+TTB_EXPORT int ttb_gather_rows(const void*, long long, const int*, const int*, void*, long long, int, int, void*);
+TTB_EXPORT int ttb_scatter_rows(const void*, int, const int*, void*, long long, int, int, void*);
 TTB_EXPORT int ttb_dropout(const void*, const void*, void*, int, long long, int, unsigned, float, unsigned long long, const unsigned long long*,
                             long long, int, void*);
 TTB_EXPORT int ttb_tail_row_blocks(long long, int, int);

@@ -545,7 +545,7 @@ PyObject* logprobs_fwd(PyObject*, PyObject* const* args, Py_ssize_t n) {
         return ttb_rows_with_targets(static_cast<const long long*>(at_(targets)), M, g.N, static_cast<int*>(to_(rows)), static_cast<int*>(to_(place)),
                                      static_cast<long long*>(to_(tc)), static_cast<int*>(to_(count)), f32w(logp), st);
       });
-      launch("ttb_gather_rows", 1, [&](void* st) { return ttb_gather_rows(at_(h), h.stride(0), i32(rows), i32(count), to_(hc), M, static_cast<int>(K), st); });
+      launch("ttb_gather_rows", 1, [&](void* st) { return ttb_gather_rows(at_(h), h.stride(0), i32(rows), i32(count), to_(hc), M, static_cast<int>(K), g.num_sms, st); });
       g.A = hc.const_data_ptr(); g.lda = K;
       g.part_rows = i32(count);
     }
@@ -622,7 +622,7 @@ PyObject* scatter_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
     need(place.scalar_type() == at::kInt && place.is_contiguous() && place.dim() == 1 && place.device() == x.device(), "places of rows are int32");
     const Tensor out = empty({place.numel(), x.size(1)}, at::kBFloat16, x);
     launch("ttb_scatter_rows", 1, [&](void* st) {
-      return ttb_scatter_rows(at_(x), !is_bf16(x), i32(place), to_(out), place.numel(), static_cast<int>(x.size(1)), st);
+      return ttb_scatter_rows(at_(x), !is_bf16(x), i32(place), to_(out), place.numel(), static_cast<int>(x.size(1)), sms(x), st);
     });
     return wrap(out);
   });

@@ -186,11 +186,11 @@ TTB_EXPORT int ttb_rows_with_targets(const long long* targets, long long T, long
 }
 
 // x: rows of `cols` bf16 values, `ld` apart; out: [T rounded up to 256, cols] without gaps, T at least *count
-TTB_EXPORT int ttb_gather_rows(const void* x, long long ld, const int* rows, const int* count, void* out, long long T, int cols, void* stream) {
+TTB_EXPORT int ttb_gather_rows(const void* x, long long ld, const int* rows, const int* count, void* out, long long T, int cols, int sms, void* stream) {
   using namespace ttb;
   if (cols % 8 || ld % 8) return 901;
   if (T == 0) return 0;
-  const long long blocks = T < 148 * 8 ? T : 148 * 8;
+  const long long blocks = T < 8ll * sms ? T : 8ll * sms;
   gather_rows_kernel<<<static_cast<unsigned>(blocks), 256, 0, static_cast<cudaStream_t>(stream)>>>(static_cast<const uint4*>(x), ld / 8, rows, count,
                                                                                                    static_cast<uint4*>(out), cols / 8);
   const cudaError_t e = cudaGetLastError();
@@ -198,11 +198,11 @@ TTB_EXPORT int ttb_gather_rows(const void* x, long long ld, const int* rows, con
 }
 
 // x: [.., cols] fp32 or bf16; out: [R, cols] bf16
-TTB_EXPORT int ttb_scatter_rows(const void* x, int fp32, const int* place, void* out, long long R, int cols, void* stream) {
+TTB_EXPORT int ttb_scatter_rows(const void* x, int fp32, const int* place, void* out, long long R, int cols, int sms, void* stream) {
   using namespace ttb;
   if (cols % 8) return 901;
   if (R == 0) return 0;
-  const unsigned blocks = static_cast<unsigned>(R < 148 * 8 ? R : 148 * 8);
+  const unsigned blocks = static_cast<unsigned>(R < 8ll * sms ? R : 8ll * sms);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (fp32) scatter_rows_kernel<<<blocks, 256, 0, st>>>(static_cast<const float*>(x), place, static_cast<__nv_bfloat16*>(out), R, cols);
   else scatter_rows_kernel<<<blocks, 256, 0, st>>>(static_cast<const __nv_bfloat16*>(x), place, static_cast<__nv_bfloat16*>(out), R, cols);
