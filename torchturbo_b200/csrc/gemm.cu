@@ -448,7 +448,7 @@ gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUt
       }
     }
   } else if (warp < 2 + L::WARPS) {
-    // ------------------------------------------------------------ epilogue (warps 2..9)
+    // ------------------------------------------------------------ epilogue (warps 2..9, of a product with a tail 2..17)
     const int lane_group = warp & 3;  // TMEM lanes [32*lane_group, +32) are the ones this warp may touch
     const int col_half = (warp - 2) >> 2;  // which half of the tile's column chunks this warp stores
     int acc = 0;
