@@ -15,7 +15,6 @@ import torch
 import torch.nn as nn
 
 from ...engine.metrics.flops import VLMFlops
-from ...ops import ops
 from ...parallel import FSDPPlanSpec, VisionBalanceMode, VisionBalanceSpec
 from ..bailing_hybrid.model import BailingWeightConverter, get_parallel_plan as text_plan
 from ..bailing_hybrid.modeling import BailingModel, BailingMoeV3Config
@@ -26,7 +25,7 @@ from ..modules.transformer import CausalLMOutput
 from ..modules.vision import GridVisionBalanceIO
 from ..qwen3.modeling import LMHead
 from ..qwen3_5.modeling import as_dtype, init_hybrid_weights
-from ..qwen3_vl.modeling import Qwen3VLVisionConfig, VisionTower
+from ..qwen3_vl.modeling import Qwen3VLVisionConfig, VisionTower, linear_tail
 from ..registry import register_model
 
 
@@ -67,12 +66,14 @@ class BailingVLModel(BailingModel):
 
 class _Projector(nn.Sequential):
     """`Linear - GELU - Linear` under the checkpoint's names (`linear_proj.0`, `linear_proj.2`), evaluated with the fused
-    bias + activation operator.  It is called as a module, never read parameter by parameter from outside: as an FSDP
-    unit of its own its weights are only gathered inside its forward."""
+    bias + activation operator (`fused_linear_tails` of the vision configuration: in the products' epilogues).  It is called
+    as a module, never read parameter by parameter from outside: as an FSDP unit of its own its weights are only gathered
+    inside its forward."""
+
+    fused = False
 
     def forward(self, feats):
-        a, b = self[0], self[2]
-        return ops.bias_act(ops.linear(ops.bias_act(ops.linear(feats, a.weight), a.bias, "gelu"), b.weight), b.bias)
+        return linear_tail(self.fused, linear_tail(self.fused, feats, self[0], "gelu"), self[2])
 
 
 class BailingMoeV3VLForConditionalGenerationBase(nn.Module):
@@ -86,6 +87,7 @@ class BailingMoeV3VLForConditionalGenerationBase(nn.Module):
         vin = vc.hidden_size * vc.spatial_merge_size ** 2 if getattr(vc, "disable_merger_proj", False) else vc.out_hidden_size
         self.linear_proj = _Projector(nn.Linear(vin, tc.hidden_size, bias=True, dtype=dtype), nn.GELU(),
                                       nn.Linear(tc.hidden_size, tc.hidden_size, bias=True, dtype=dtype))
+        self.linear_proj.fused = bool(getattr(vc, "fused_linear_tails", False))
         self.lm_head = LMHead(tc.hidden_size, tc.vocab_size, bias=False, dtype=dtype)
         n = int(getattr(tc, "num_nextn_predict_layers", 0) or 0)
         self.mtp = nn.ModuleList([self.model.make_nextn_layer(tc.num_hidden_layers + i, dtype) for i in range(n)]) if n else None

@@ -31,6 +31,7 @@ from ...ops import ops
 from ..config import ModelConfig
 from ..modules.mixers import apply_partial_rope
 from ..modules.vision import GridVisionBalanceIO
+from ..qwen3_vl.modeling import linear_tail
 
 
 class MoonViTConfig(ModelConfig):
@@ -147,19 +148,20 @@ class MoonViTBlock(nn.Module):
         self.mlp = _MLP2(C, cfg.vt_intermediate_size, dtype)
         self.wqkv = nn.Linear(C, 3 * C, dtype=dtype)
         self.wo = nn.Linear(C, C, dtype=dtype)
+        self.fused = bool(getattr(cfg, "fused_linear_tails", False))
 
     def forward(self, x, cos, sin, cu, max_len):
         P = x.shape[0]
         h = ops.layer_norm(x, self.norm0.weight, self.norm0.bias, self.norm0.eps)
-        qkv = ops.bias_act(ops.linear(h, self.wqkv.weight), self.wqkv.bias).view(P, 3, self.n_heads, self.head_dim)
+        qkv = linear_tail(self.fused, h, self.wqkv).view(P, 3, self.n_heads, self.head_dim)
         q = apply_partial_rope(qkv[:, 0].contiguous(), cos, sin, interleaved=True)
         k = apply_partial_rope(qkv[:, 1].contiguous(), cos, sin, interleaved=True)
         a = ops.attention(q.contiguous(), k.contiguous(), qkv[:, 2].contiguous(), cu, max_len, causal=False,
                           scale=1.0 / math.sqrt(self.head_dim))
-        x = ops.bias_act(ops.linear(a.reshape(P, -1), self.wo.weight), self.wo.bias, residual=x)
+        x = linear_tail(self.fused, a.reshape(P, -1), self.wo, residual=x)
         h = ops.layer_norm(x, self.norm1.weight, self.norm1.bias, self.norm1.eps)
-        h = ops.bias_act(ops.linear(h, self.mlp.fc0.weight), self.mlp.fc0.bias, "gelu_tanh")
-        return ops.bias_act(ops.linear(h, self.mlp.fc1.weight), self.mlp.fc1.bias, residual=x)
+        h = linear_tail(self.fused, h, self.mlp.fc0, "gelu_tanh")
+        return linear_tail(self.fused, h, self.mlp.fc1, residual=x)
 
 
 class _Encoder(nn.Module):
@@ -232,12 +234,12 @@ class PatchMergerMLP(nn.Module):
         self.pre_norm = nn.LayerNorm(C, eps=cfg.projector_ln_eps, dtype=dtype)
         self.proj = nn.Sequential(nn.Linear(C * self.unit, C * self.unit, dtype=dtype), nn.GELU(),
                                   nn.Linear(C * self.unit, cfg.text_hidden_size, dtype=dtype))
+        self.fused = bool(getattr(cfg, "fused_linear_tails", False))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         rows = x.shape[0]
         h = ops.layer_norm(x.reshape(rows * self.unit, -1), self.pre_norm.weight, self.pre_norm.bias, self.pre_norm.eps)
-        h = ops.bias_act(ops.linear(h.reshape(rows, -1), self.proj[0].weight), self.proj[0].bias, "gelu")
-        return ops.bias_act(ops.linear(h, self.proj[2].weight), self.proj[2].bias)
+        return linear_tail(self.fused, linear_tail(self.fused, h.reshape(rows, -1), self.proj[0], "gelu"), self.proj[2])
 
 
 class TemporalPoolVisionBalanceIO(GridVisionBalanceIO):
