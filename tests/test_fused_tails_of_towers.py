@@ -60,3 +60,14 @@ def test_bailing_projector_takes_the_vision_configuration(fused, calls):
     feats = torch.randn(6, other.linear_proj[0].in_features, generator=torch.Generator().manual_seed(1))
     want, y = model.linear_proj(feats), other.linear_proj(feats)
     assert len(calls) == (2 if fused else 0) and torch.allclose(y, want, rtol=1e-5, atol=1e-6)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("inner, outer", [(64, 50), (60, 48)])
+def test_other_widths_keep_their_separate_passes(device, inner, outer, calls):
+    """Widths that are no multiple of eight: the operands are not copied to fp32 for a product with a tail."""
+    torch.manual_seed(0)
+    lin = torch.nn.Linear(inner, outer, device=device, dtype=torch.bfloat16)
+    x, r = (torch.randn(9, n, device=device, dtype=torch.bfloat16) for n in (inner, outer))
+    got = [shared.linear_tail(fused, x, lin, "gelu", residual=r) for fused in (True, False)]
+    assert torch.equal(*got) and not calls

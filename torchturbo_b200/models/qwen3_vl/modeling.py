@@ -99,10 +99,12 @@ class _VisionMLP(nn.Module):
 
 def linear_tail(fused: bool, x, lin, act=None, residual=None):
     """A biased layer with what follows it: one product whose epilogue does it all (`ops.linear_bias_act`: what the product adds up is not
-    rounded before the bias), or a pass of its own after the product."""
-    if fused:
-        return ops.linear_bias_act(x, lin.weight, lin.bias, act, residual=residual)
-    return ops.bias_act(ops.linear(x, lin.weight), lin.bias, act, residual=residual)
+    rounded before the bias), or a pass of its own after the product.  The latter also for widths that the product's kernel does not take:
+    the operator's plain form would copy the operands to fp32."""
+    w = lin.weight
+    if fused and w.shape[0] % 8 == 0 and w.shape[1] % 8 == 0:
+        return ops.linear_bias_act(x, w, lin.bias, act, residual=residual)
+    return ops.bias_act(ops.linear(x, w), lin.bias, act, residual=residual)
 
 
 _ACTS = {"gelu_pytorch_tanh": "gelu_tanh", "gelu_tanh": "gelu_tanh", "gelu": "gelu"}
