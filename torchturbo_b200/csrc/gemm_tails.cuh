@@ -3,13 +3,13 @@
 //   tail_store    C = residual + dropout(act(z)), z = product + bias; z itself is kept in bf16 where the backward needs it (it reads z for
 //                 act'(z) only).  Everything up to C's one rounding stays fp32.  Under long sums the tail is hidden; of short ones it is the
 //                 whole kernel, bound by the latency of its arithmetic: sixteen warps instead of eight took a sum of 16 products, 8190 x 4096 of them,
-//                 with GELU (tanh) from 36 to 30 us, with dropout and residual from 52 to 48 (the product alone, written at the rate of a fill: 22; residual
-//                 and all at the rate of a copy: 31).  3001 x 1152 -> 4304 with bias, GELU and pre-activations 38 us, the product alone 32.
+//                 with dropout and residual from 52 to 48 us (residual and all at the rate of a copy: 31).  3001 x 1152 -> 4304 with bias, GELU (tanh) and
+//                 pre-activations 30 us in short runs, with GELU (erf) 32, with the bias alone 26.
 //   tail_stats    of each row's logits in this tile and half of its columns: largest, sum of exponentials, and for the entropy their sum
 //                 weighted by the distance from the largest (logprobs.cu joins them).  All in powers of two: with m the largest times
 //                 log2(e) as rounded to fp32, d = l log2(e) - m is one fma, 2^d one instruction, and log2 sum 2^(l log2 e) = m + log2 s is
-//                 exact in m whatever its rounding was.  Hidden under sums of 512 and more: 4096 x 2048 x 151936 under the power cap 1816 us,
-//                 1404 TFLOP/s, where the product that stores its results takes 1925.
+//                 exact in m whatever its rounding was.  Nearly hidden under sums of 512: 4096 x 2048 x 151936 under the power cap 1877 us,
+//                 1358 TFLOP/s, where the product that stores its results takes 1925.
 //   tail_dlogits  gradient of the logits, formed again from the same operands:  p = 2^(l log2 e - lse log2 e),
 //                 dl = g (1[target] - p) - e p (l - lse + H), rounded to bf16, the type in which the two products behind it take it.  Of few
 //                 rows one value, the target's, is most of a row, and its rounding would not average out: what it left out goes to a

@@ -326,8 +326,8 @@ GemmArgs product(const Tensor& a, const Tensor& b) {
 bool few_rows(const GemmArgs& g) { return g.M <= 4 || (g.M <= 8 && static_cast<long long>(g.N) * g.K <= (1 << 23)); }
 
 // Whether the rows are walked and not tiled (linear_narrow.cu).  us, walk and tiles, with residual: 2048 x 16 -> 4096 11 and 14, 4096 x 16 -> 4096 20 and 22,
-// 6000 x 16 -> 4096 29 and 28, 8190 x 16 -> 4096 39 and 36; with GELU (tanh) and pre-activations 9 and 14, 17 and 24, 24 and 31, 32 and 35, and
-// 4096 x 16 -> 12288 45 and 59.  With 64 features the tiles are as fast from 300 rows on.
+// 6000 x 16 -> 4096 29 and 28, 8190 x 16 -> 4096 39 and 36; with GELU (tanh) and pre-activations 13 and 20,
+// 18 and 29, 25 and 38, 34 and 43, and 4096 x 16 -> 12288 48 and 67 (the tiles' figures of 24 features, one k-block like 16).  With 64 features the tiles are as fast from 300 rows on.
 bool few_features(const GemmArgs& g) { return g.K <= 16 && (g.tail->act || static_cast<long long>(g.M) * g.N <= 3ll << 23); }
 
 PyObject* linear_tail(PyObject*, PyObject* const* args, Py_ssize_t n) {

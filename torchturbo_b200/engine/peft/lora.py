@@ -3,8 +3,8 @@
 The model blocks read `module.weight` and feed it to fused kernels, so an adapted layer exposes the *effective*
 weight `W + (alpha / r) * B @ A` (DoRA: column-normalised and rescaled by a learned magnitude) through the same
 attribute: the low-rank factors are the only trainable tensors, gradients reach them through the merge, and the
-hot kernels stay unchanged.  Fused expert tensors get one pair of factors per expert (`GroupedLoRA`), merged with a
-batched matmul.  Parameter names follow the PEFT convention (`base_layer.weight`, `lora_A.<adapter>.weight`,
+hot kernels stay unchanged.  Dropout acts in layers that are called as modules: a merged weight has no input to drop.
+Fused expert tensors get one pair of factors per expert (`GroupedLoRA`), merged with a batched matmul.  Parameter names follow the PEFT convention (`base_layer.weight`, `lora_A.<adapter>.weight`,
 `lora_B.<adapter>.weight`, `lora_magnitude_vector.<adapter>.weight`) so adapter checkpoints interoperate
 (engine/peft/lora.py:54-739 and engine/peft/weights.py:78-350 of the reference).
 """

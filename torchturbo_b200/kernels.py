@@ -166,8 +166,10 @@ def gemm_splits(M: int, N: int, K: int, sms: int) -> int:
 def wave_splits(M: int, N: int, K: int, sms: int) -> int:
     """Pieces along K for a product of many k-blocks whose tiles of 256 x 256 (pairs of CTAs) leave a wave partly empty: ``s`` pieces take
     ``ceil(tiles s / pairs) / s`` whole waves, of 0.37 us a k-block, but ``s`` fp32 results are written at 2.5 TB/s, read at 6 and their
-    sum written once more.  1501 x 4096 x 32003 (96 tiles on 74 pairs) 349 -> 306 us in three pieces; 4096 x 2048 x 50688 would go from
-    602 to 611 in four."""
+    sum written once more.  us in one piece, in the rule's
+    number of them and in the best of 1 .. 6 and 8: 1501 x 4096 x 32003 347, 334 (3) and 314 (2); 4096 x 2048 x 50688 607, 607 (1), 607;
+    1024 x 2048 x 151936 858, 470 (2), 468 (4); 2048 x 2048 x 75968 441, 441 (1), 441; 700 x 4096 x 32000 230, 192 (3), 157 (6);
+    512 x 2048 x 151936 741, 244 (4), 244; 3000 x 4096 x 32003 595, 595 (1), 595; 2048 x 1024 x 50000 340, 186 (2), 164 (4)."""
     tiles, pairs, blocks = ((M + 255) // 256) * ((N + 255) // 256), sms // 2, (K + 63) // 64
     if M <= 128 or N <= 128 or N % 8 or 2 * tiles < pairs:
         return gemm_splits(M, N, K, sms)
